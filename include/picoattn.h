@@ -62,6 +62,7 @@ typedef struct CUstream_st* picoattn_stream_t;
 #define PICOATTN_DEV_BAD_POS      0x1u  /* pos[b] < 0, >= max_seq_len or >= max_ctx */
 #define PICOATTN_DEV_MISALIGNED   0x2u  /* a cache pointer not 16-byte aligned */
 #define PICOATTN_DEV_TIMEOUT      0x4u  /* a bounded barrier wait gave up */
+#define PICOATTN_DEV_BAD_PAGE     0x8u  /* a page table entry in use outside [0, n_pages) */
 
 /* RoPE pairing.  NEOX = TensorOps::rope_qwen (cpp/tensor.hpp:201-283, element i
  * with i+hd/2).  INTERLEAVED = rope_llama's scalar definition (element 2i with
@@ -73,6 +74,7 @@ typedef struct CUstream_st* picoattn_stream_t;
 /* Element type of q/k/v inputs. */
 #define PICOATTN_DTYPE_F32 0
 #define PICOATTN_DTYPE_F16 1
+#define PICOATTN_DTYPE_BF16 2  /* picoattn_rope and the paged cache only */
 
 /* Model shape as the reference's config map holds it (cpp/model.hpp:33-47). */
 typedef struct {
@@ -567,6 +569,160 @@ int32_t picoattn_gguf_upload(const picoattn_gguf_t* model, void* arena, size_t a
  * attn_k_norm, *_b) their fp32 copy (type PICOATTN_WT_F32). */
 int32_t picoattn_gguf_arena_tensor(const picoattn_gguf_t* model, const void* arena, int32_t layer, const char* key,
                                    const void** dev_ptr, int32_t* type);
+
+/* ---------------------------------------------------------------------- */
+/* Rotary positions on their own                                           */
+/* ---------------------------------------------------------------------- */
+/* The reference rotates whole heads inside its attention step
+ * (cpp/model.hpp:351-352) with an unscaled table (cpp/model.hpp:1008-1017);
+ * partial rotation, scaled tables and the gradient have no counterpart there. */
+
+/* How the frequencies of a table are scaled for contexts longer than the model
+ * was trained on; f_i = rope_freq_base^(-2i/rot_dim), i < rot_dim/2. */
+#define PICOATTN_ROPE_SCALE_NONE     0  /* f_i */
+#define PICOATTN_ROPE_SCALE_LINEAR   1  /* f_i / factor: positions interpolated */
+#define PICOATTN_ROPE_SCALE_NTK      2  /* base * factor^(rot_dim/(rot_dim-2)); rot_dim > 2 */
+#define PICOATTN_ROPE_SCALE_BY_PARTS 3  /* (1-w) f_i/factor + w f_i, w = clamp((r_i-low)/(high-low), 0, 1)
+                                           with r_i = orig_ctx f_i / (2 pi), the turns of pair i over
+                                           the trained context (YaRN, Peng et al. 2023) */
+typedef struct {
+    int32_t rot_dim;    /* elements of each head that rotate: even, 2..head_dim; 0: head_dim */
+    int32_t kind;       /* PICOATTN_ROPE_SCALE_* */
+    float   factor;     /* context extension, >= 1 (ignored by NONE) */
+    int32_t orig_ctx;   /* trained context length (BY_PARTS) */
+    float   low, high;  /* turns below / above which a pair is interpolated / left alone (BY_PARTS; low < high) */
+    float   mscale;     /* cos and sin are multiplied by it (1: plain rotation); > 0 */
+} picoattn_rope_scaling_t;
+
+/* Fills HOST arrays cos_out/sin_out [max_seq_len][rot_dim/2] for the config's
+ * rope_freq_base; angles in fp64, rounded once to fp32 (picoattn_rope_table
+ * keeps the reference's fp32 angles instead). */
+int32_t picoattn_rope_scaled_table(const picoattn_config_t* cfg, const picoattn_rope_scaling_t* scaling,
+                                   float* cos_out, float* sin_out);
+
+/* The heads of one tensor, one row of n_heads*head_dim elements per token. */
+typedef struct {
+    const void* x;          /* first token's row */
+    int64_t     x_stride;   /* elements from a token's row to the next (>= 0; 0: one row for all) */
+    void*       out;        /* may equal x (with the same stride): rotated in place */
+    int64_t     out_stride; /* >= n_heads*head_dim */
+    int32_t     n_heads;
+} picoattn_rope_rows_t;
+
+/*
+ * Rotates the first rot_dim elements of every head of q, and of k when given,
+ * by the table row of the token's position, and copies the others.
+ *   dtype     PICOATTN_DTYPE_F32, _F16 or _BF16, of x and out; each product and
+ *             sum in fp32, the result rounded to nearest even once
+ *   rope_mode PICOATTN_ROPE_NEOX (pairs i, i + rot_dim/2) or _INTERLEAVED (2i, 2i + 1)
+ *   head_dim  even, 2..1024; rot_dim even, 2..head_dim
+ *   inverse   non-zero: rotates by the opposite angles.  It is the rotation's
+ *             transpose, so it takes the gradient of the output to the
+ *             gradient of the input (tables scaled by mscale: times mscale again)
+ *   pos       [n_tok] int32 device; one outside [0, table_rows) sets
+ *             PICOATTN_DEV_BAD_POS and its output rows are NaN
+ *   rope_cos, rope_sin  [table_rows][rot_dim/2] fp32 device, 4-byte aligned
+ *   workspace at least 256 bytes (the status word)
+ * x and out may be any element-aligned addresses; an output that overlaps an
+ * input without being in place, or the other output, is PICOATTN_EINVAL.  (The
+ * rows of q and k may interleave, as in one q|k|v projection's output.)
+ */
+int32_t picoattn_rope(int32_t dtype, int32_t rope_mode, int32_t head_dim, int32_t rot_dim, int32_t inverse,
+                      int32_t n_tok, const int32_t* pos, int32_t table_rows,
+                      const float* rope_cos, const float* rope_sin,
+                      const picoattn_rope_rows_t* q, const picoattn_rope_rows_t* k,
+                      void* workspace, size_t workspace_bytes, picoattn_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Paged KV cache: append and attention for ragged batches                 */
+/* ---------------------------------------------------------------------- */
+/* The reference holds one slab of max_seq_len rows (cpp/model.hpp:1003-1006).
+ * Here the rows of many sequences live in pages of one pool per layer; a page
+ * table lists each sequence's pages in order, so a sequence holds only the
+ * pages it uses.  Any n_kv_heads, up to 128 q heads per KV head, head_dim 64 or
+ * 128 (the other picoattn_config_t limits do not apply). */
+typedef struct {
+    int32_t n_pages;    /* pages per layer */
+    int32_t page_size;  /* rows per page: 16, 32, 64, 128 or 256 */
+    int32_t dtype;      /* PICOATTN_DTYPE_F16 or PICOATTN_DTYPE_BF16 */
+    void*   k;          /* [n_layers][n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
+    void*   v;
+} picoattn_paged_cache_t;
+
+/* The sequences of one step.  Sequence b has the new tokens q_start[b] ..
+ * q_start[b+1]-1 (rows of q, k, v and out; none is allowed), the last of them
+ * at position kv_len[b]-1: kv_len counts the new tokens.  Rows of q, k, v and
+ * out outside [q_start[0], q_start[n_seqs]) are neither read nor written, so a
+ * captured step may be padded.  The three bounds are host values, the lengths
+ * device values: a sequence with more than max_new new tokens, a kv_len above
+ * max_len or below its new tokens, or rows outside [0, n_tok) sets
+ * PICOATTN_DEV_BAD_POS, leaves the cache as it was, and its q_out / out rows
+ * (those inside [0, n_tok)) are NaN. */
+typedef struct {
+    int32_t n_seqs;            /* at least 1 */
+    int32_t n_tok;             /* rows of q, k, v, out; at least 1 */
+    int32_t max_new;           /* most new tokens of a sequence */
+    int32_t max_len;           /* most rows of a sequence; <= page_cols*page_size and <= max_seq_len */
+    int32_t page_cols;         /* entries per page table row */
+    const int32_t* page_table; /* device [n_seqs][page_cols]; entries past a sequence's rows are not read */
+    const int32_t* q_start;    /* device [n_seqs+1], not decreasing */
+    const int32_t* kv_len;     /* device [n_seqs] */
+} picoattn_paged_batch_t;
+
+/* PICOATTN_OK, EINVAL or EUNSUPPORTED for a config with a cache description. */
+int32_t picoattn_paged_check(const picoattn_config_t* cfg, const picoattn_paged_cache_t* cache);
+
+/* Bytes of a workspace for picoattn_paged_append and picoattn_paged_attn on
+ * batches of up to n_seqs sequences, whatever their lengths (0: the config or
+ * n_seqs is not accepted).  Call picoattn_workspace_init once on it; calls that
+ * may run at the same time need workspaces of their own. */
+size_t picoattn_paged_workspace_size(const picoattn_config_t* cfg, int32_t n_seqs);
+
+/*
+ * The new tokens' keys and values into their pages, and their queries made
+ * ready for picoattn_paged_attn: QK-RMSNorm (when the weights are given), RoPE of
+ * the first rot_dim elements at the token's position, rounding to the cache's
+ * type (F16 by the reference's rule as in picoattn_decode, BF16 to nearest even).
+ *   in_dtype  PICOATTN_DTYPE_F32, _F16 or _BF16 of q, k and v
+ *   q, k, v   [n_tok] rows of heads; q_stride, k_stride, v_stride: elements from
+ *             a token's row to the next (a q|k|v projection's output needs no
+ *             split).  q and q_out may both be NULL
+ *   q_out     [n_tok][n_heads*head_dim] in the cache's type, not overlapping q, k, v
+ *   rope_cos, rope_sin  [max_seq_len][rot_dim/2] (picoattn_rope_table or
+ *             picoattn_rope_scaled_table)
+ *   rot_dim   multiple of 16, 16..head_dim
+ * q, k, v and q_out 16-byte aligned with strides of whole 16 bytes.  A page table entry
+ * outside [0, n_pages) sets PICOATTN_DEV_BAD_PAGE and the row is not stored.
+ * Two sequences that share a page must not both append to it.
+ */
+int32_t picoattn_paged_append(const picoattn_config_t* cfg, const picoattn_paged_cache_t* cache, int32_t layer,
+                              const picoattn_paged_batch_t* batch, int32_t in_dtype,
+                              const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                              const void* v, int64_t v_stride,
+                              const float* q_norm_w, const float* k_norm_w,
+                              const float* rope_cos, const float* rope_sin, int32_t rot_dim, void* q_out,
+                              void* workspace, size_t workspace_bytes, picoattn_stream_t stream);
+
+/*
+ * Causal attention of the batch's new tokens over their sequences' pages (rows
+ * already appended): out[t] = softmax(q[t] K^T / sqrt(head_dim)) V over rows
+ * 0..pos of the token's sequence, for single tokens, drafts, chunks and whole
+ * prompts, mixed as they come.
+ *   q         [n_tok] rows of n_heads*head_dim in the cache's type (q_out of
+ *             picoattn_paged_append), q_stride elements apart; 16-byte aligned,
+ *             whole 16 bytes
+ *   out_dtype the cache's type or PICOATTN_DTYPE_F32
+ *   out       [n_tok][n_heads*head_dim], 16-byte aligned
+ * Scores, sums and outputs accumulate in fp32; the weights exp(s - max) are
+ * rounded to the cache's type for the product with V.  A page table entry
+ * outside [0, n_pages) sets PICOATTN_DEV_BAD_PAGE and the outputs that would
+ * have read it are NaN (others of that sequence may be).  Rows past a sequence's length are never used, whatever
+ * they hold.
+ */
+int32_t picoattn_paged_attn(const picoattn_config_t* cfg, const picoattn_paged_cache_t* cache, int32_t layer,
+                            const picoattn_paged_batch_t* batch, const void* q, int64_t q_stride,
+                            int32_t out_dtype, void* out,
+                            void* workspace, size_t workspace_bytes, picoattn_stream_t stream);
 
 #ifdef __cplusplus
 }

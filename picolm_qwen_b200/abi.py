@@ -33,6 +33,7 @@ KVCP_MAGIC = 0x4B564350
 DEV_BAD_POS = 0x1
 DEV_MISALIGNED = 0x2
 DEV_TIMEOUT = 0x4
+DEV_BAD_PAGE = 0x8
 
 STAGE_PREPARE = 0x1
 STAGE_ATTEND = 0x2
@@ -49,6 +50,12 @@ ROPE_NEOX = 0
 ROPE_INTERLEAVED = 1
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2  # rope and the paged cache only
+
+ROPE_SCALE_NONE = 0
+ROPE_SCALE_LINEAR = 1
+ROPE_SCALE_NTK = 2
+ROPE_SCALE_BY_PARTS = 3
 
 # projection weight formats (GGUF tensor types)
 WT_F32 = 1
@@ -112,8 +119,33 @@ class FfnWeights(C.Structure):
     ]
 
 
+class RopeScaling(C.Structure):
+    """picoattn_rope_scaling_t."""
+    _fields_ = [("rot_dim", C.c_int32), ("kind", C.c_int32), ("factor", C.c_float), ("orig_ctx", C.c_int32),
+                ("low", C.c_float), ("high", C.c_float), ("mscale", C.c_float)]
+
+
+class RopeRows(C.Structure):
+    """picoattn_rope_rows_t: the heads of one tensor."""
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("n_heads", C.c_int32)]
+
+
+class PagedCacheDesc(C.Structure):
+    """picoattn_paged_cache_t."""
+    _fields_ = [("n_pages", C.c_int32), ("page_size", C.c_int32), ("dtype", C.c_int32), ("k", C.c_void_p),
+                ("v", C.c_void_p)]
+
+
+class PagedBatchDesc(C.Structure):
+    """picoattn_paged_batch_t."""
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "n_tok", "max_new", "max_len", "page_cols")] + \
+        [(n, C.c_void_p) for n in ("page_table", "q_start", "kv_len")]
+
+
 _P = C.c_void_p
 _I = C.c_int32
+_L = C.c_int64
 _Z = C.c_size_t
 _CFG = C.POINTER(Config)
 
@@ -182,6 +214,15 @@ PROTOTYPES = {
     "picoattn_decode_block_workspace_size": (_Z, [_CFG, _I, _I, _I, _I]),
     "picoattn_decode_block": (_I, [_CFG, _I, _I, _I, _I, _I, _P, C.POINTER(LayerWeights), _P, C.POINTER(FfnWeights),
                                    _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "picoattn_rope_scaled_table": (_I, [_CFG, C.POINTER(RopeScaling), _P, _P]),
+    "picoattn_rope": (_I, [_I, _I, _I, _I, _I, _I, _P, _I, _P, _P, C.POINTER(RopeRows), C.POINTER(RopeRows), _P, _Z,
+                           _P]),
+    "picoattn_paged_check": (_I, [_CFG, C.POINTER(PagedCacheDesc)]),
+    "picoattn_paged_workspace_size": (_Z, [_CFG, _I]),
+    "picoattn_paged_append": (_I, [_CFG, C.POINTER(PagedCacheDesc), _I, C.POINTER(PagedBatchDesc), _I, _P, _L, _P, _L,
+                                   _P, _L, _P, _P, _P, _P, _I, _P, _P, _Z, _P]),
+    "picoattn_paged_attn": (_I, [_CFG, C.POINTER(PagedCacheDesc), _I, C.POINTER(PagedBatchDesc), _P, _L, _I, _P, _P,
+                                 _Z, _P]),
 }
 
 _lib = None

@@ -1,0 +1,132 @@
+// paged_common.cuh -- element types, rotations and the ragged batch of the
+// rotary and paged-cache kernels.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "device_common.cuh"
+#include "paged_internal.h"
+
+namespace picoattn {
+
+// Sixteen-byte pieces of each element type as fp32 values and back.  pack()
+// rounds to nearest even; store_cache() is the rounding of a cache row, which
+// for fp16 is the reference's half-up rule (f32_to_f16_ref).
+template <class T>
+struct Elem;
+
+template <>
+struct Elem<float> {
+    static constexpr int V = 4;  // elements per 16 bytes
+    static __device__ __forceinline__ void unpack(const uint4& w, float* x) {
+        x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y);
+        x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float* x) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    static __device__ __forceinline__ float load(const float* p) { return *p; }
+    static __device__ __forceinline__ float round(float x) { return x; }
+};
+
+template <>
+struct Elem<__half> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return pack_half2(lo, hi); }
+    static __device__ __forceinline__ uint32_t cache2(float lo, float hi) { return f32x2_to_f16_ref(lo, hi); }
+    static __device__ __forceinline__ void unpack(const uint4& w, float* x) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float* x) {
+        return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    }
+    static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
+    static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+};
+
+template <>
+struct Elem<__nv_bfloat16> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint32_t cache2(float lo, float hi) { return pack2(lo, hi); }
+    static __device__ __forceinline__ void unpack(const uint4& w, float* x) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {  // a bf16 is the upper half of the fp32 of its value
+            x[2 * i] = __uint_as_float(u[i] << 16);
+            x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float* x) {
+        return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
+    }
+    static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+};
+
+// (x0, x1) -> (x0 c - x1 s, x0 s + x1 c), products and sums rounded one by one
+// as in the attention step's prep kernels, so a rotated key rounds to the same
+// cache bits there and here.
+__device__ __forceinline__ void rotate_pair(float& x0, float& x1, float c, float s) {
+    const float a = x0, b = x1;
+    x0 = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+    x1 = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
+}
+
+// Where a lane's two 16-byte pieces (V elements each) of a head lie, so that
+// both members of every pair it rotates are its own.  Lane p of the hd/(2V) a
+// head takes: rotated part first (NeoX: pieces p of both halves; interleaved:
+// two adjacent pieces), then the part that stays, two adjacent pieces a lane.
+// rot_dim is a multiple of 2V.
+struct PieceAt {
+    int a, b;      // first elements of the two pieces
+    int pair;      // first table column (rotated lanes)
+    bool rotated;
+};
+template <int V>
+__device__ __forceinline__ PieceAt piece_at(int p, int rot, bool neox) {
+    PieceAt r;
+    r.rotated = 2 * V * p < rot;
+    if (r.rotated && neox) r.a = V * p, r.b = rot / 2 + V * p, r.pair = V * p;
+    else r.a = 2 * V * p, r.b = 2 * V * p + V, r.pair = V * p;
+    return r;
+}
+
+// Rotates the lane's 2V elements x with its V table entries.
+template <int V>
+__device__ __forceinline__ void rotate_pieces(float* x, const float* c, const float* s, bool neox) {
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        if (neox) rotate_pair(x[j], x[V + j], c[j], s[j]);
+        else rotate_pair(x[2 * j], x[2 * j + 1], c[j], s[j]);
+    }
+}
+
+// ---- the ragged batch ---------------------------------------------------------
+
+struct SeqSpan {
+    int t0, n, len;  // first row, new tokens, cache rows with the new tokens
+    bool ok;         // within the host's bounds (n == 0: nothing to do)
+};
+
+__device__ __forceinline__ SeqSpan seq_span(const PagedBatch& a, int b) {
+    SeqSpan s;
+    s.t0 = a.q_start[b];
+    const int t1 = a.q_start[b + 1];
+    s.len = a.kv_len[b];
+    s.n = t1 - s.t0;  // wraps only for spans that fail the range test
+    s.ok = s.t0 >= 0 && t1 >= s.t0 && t1 <= a.n_tok && s.n <= a.max_new && s.len >= s.n && s.len <= a.max_len;
+    return s;
+}
+
+}  // namespace picoattn

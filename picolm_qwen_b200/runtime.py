@@ -102,6 +102,218 @@ def logits(x: torch.Tensor, output_norm_w: torch.Tensor, w_out: torch.Tensor, w_
               "picoattn_logits")
 
 
+_DTYPES = {torch.float32: abi.DTYPE_F32, torch.float16: abi.DTYPE_F16, torch.bfloat16: abi.DTYPE_BF16}
+
+
+def _dtype(t: torch.Tensor) -> int:
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise TypeError(f"dtype {t.dtype}: float32, float16 or bfloat16")
+    return d
+
+
+def _heads(t: torch.Tensor, n: int, hd: int, what: str) -> int:
+    """The row stride of t, [n, heads, hd] or [n, heads*hd], each row's heads contiguous."""
+    st = t.stride()
+    if t.dim() == 3:
+        if t.shape[0] != n or t.shape[2] != hd or st[2] != 1 or (st[1] != hd and t.shape[1] != 1):
+            raise ValueError(f"{what}: [{n}, heads, {hd}] with contiguous heads, got {tuple(t.shape)} strides {st}")
+    elif t.dim() != 2 or t.shape[0] != n or t.shape[1] % hd or st[1] != 1:
+        raise ValueError(f"{what}: [{n}, heads, {hd}] or [{n}, heads*{hd}], got {tuple(t.shape)} strides {st}")
+    return st[0]
+
+
+def _same_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _launch_stream(device: torch.device, stream) -> int:
+    """The stream to launch on; the call is made with its tensors' device current."""
+    if stream is not None:
+        return stream.cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on_device(device: torch.device, call, *args) -> int:
+    """call(*args) with `device` current, whichever device the caller has current."""
+    if torch.cuda.current_device() == device.index:
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
+
+
+def status_workspace(device: str | torch.device = "cuda") -> torch.Tensor:
+    """A workspace for calls that need only the status word (`rope`)."""
+    return torch.zeros(256, dtype=torch.uint8, device=device)
+
+
+def workspace_status(ws: torch.Tensor) -> int:
+    """The sticky device status bits (abi.DEV_*) of a workspace; synchronises and clears them."""
+    v = C.c_uint32(0)
+    abi.check(_on_device(ws.device, abi.lib().picoattn_workspace_status, ws.data_ptr(),
+                         _launch_stream(ws.device, None), C.byref(v)), "workspace_status")
+    return v.value
+
+
+def rope_scaled_table(cfg: abi.Config, rot_dim: int = 0, kind: int = abi.ROPE_SCALE_NONE, factor: float = 1.0,
+                      orig_ctx: int = 0, low: float = 1.0, high: float = 32.0,
+                      mscale: float = 1.0) -> tuple[np.ndarray, np.ndarray]:
+    """Host RoPE tables [max_seq_len, rot_dim/2] for scaled contexts and partial heads."""
+    half = (rot_dim or cfg.head_dim) // 2
+    cos = np.empty((cfg.max_seq_len, half), np.float32)
+    sin = np.empty((cfg.max_seq_len, half), np.float32)
+    sc = abi.RopeScaling(rot_dim, kind, factor, orig_ctx, low, high, mscale)
+    abi.check(abi.lib().picoattn_rope_scaled_table(C.byref(cfg), C.byref(sc), cos.ctypes.data, sin.ctypes.data),
+              "picoattn_rope_scaled_table")
+    return cos, sin
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
+         q_out: torch.Tensor, k_out: torch.Tensor | None, workspace: torch.Tensor,
+         rope_mode: int = abi.ROPE_NEOX, inverse: bool = False, stream: torch.cuda.Stream | None = None) -> None:
+    """q_out, k_out = q, k [n_tok, heads, head_dim] rotated by pos [n_tok] int32
+    (the first 2 * rope_cos.shape[1] elements of each head); the outputs may be
+    the inputs.  inverse: the opposite rotation, which is the backward pass."""
+    n, heads, hd = q.shape
+    dev = q.device
+    half = rope_cos.shape[1]
+    if pos.dtype != torch.int32 or pos.shape != (n,) or pos.stride(0) != 1 and n > 1:
+        raise ValueError(f"pos: [{n}] int32")
+    _check_table(rope_cos, rope_sin, half)
+    if q_out.dtype != q.dtype or q_out.shape != q.shape or (k is None) != (k_out is None):
+        raise ValueError("q_out: like q; k and k_out both or neither")
+    _same_device(dev, k=k, pos=pos, rope_cos=rope_cos, rope_sin=rope_sin, q_out=q_out, k_out=k_out,
+                 workspace=workspace)
+    rows = abi.RopeRows(q.data_ptr(), _heads(q, n, hd, "q"), q_out.data_ptr(), _heads(q_out, n, hd, "q_out"), heads)
+    krows = None
+    if k is not None:
+        if k.dtype != q.dtype or k_out.dtype != q.dtype or k_out.shape != k.shape:
+            raise ValueError("k, k_out: of q's type and one shape")
+        krows = C.byref(abi.RopeRows(k.data_ptr(), _heads(k, n, hd, "k"), k_out.data_ptr(),
+                                     _heads(k_out, n, hd, "k_out"), k.shape[1]))
+    st = _on_device(dev, abi.lib().picoattn_rope, _dtype(q), rope_mode, hd, 2 * half, 1 if inverse else 0, n,
+                    pos.data_ptr(), rope_cos.shape[0], rope_cos.data_ptr(), rope_sin.data_ptr(), C.byref(rows), krows,
+                    workspace.data_ptr(), workspace.numel(), _launch_stream(dev, stream))
+    if st:
+        abi.check(st, "picoattn_rope")
+
+
+def _check_table(cos: torch.Tensor, sin: torch.Tensor, half: int, rows: int = 1) -> None:
+    for t in (cos, sin):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[0] < rows or \
+                not t.is_contiguous():
+            raise ValueError(f"rope tables: contiguous fp32 [>= {rows}, {half}], got {tuple(t.shape)} {t.dtype}")
+
+
+class PagedBatch:
+    """The sequences of one step (picoattn_paged_batch_t) with the workspace its calls use.
+
+    page_table [n_seqs, page_cols], q_start [n_seqs+1], kv_len [n_seqs]: int32 on the
+    cache's device; their values may change between calls (a captured step reads
+    them when it is replayed).  n_tok: rows of q, k, v and out; max_new, max_len:
+    bounds on a sequence's new tokens and rows.  Steps that may run at the same
+    time need batches of their own."""
+
+    def __init__(self, cache: "PagedCache", page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
+                 n_tok: int, max_new: int, max_len: int):
+        n = kv_len.numel()
+        for name, t, shape in (("page_table", page_table, (n, page_table.shape[-1])), ("q_start", q_start, (n + 1,)),
+                               ("kv_len", kv_len, (n,))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"{name}: contiguous int32 {shape}, got {tuple(t.shape)} {t.dtype}")
+        _same_device(cache.device, page_table=page_table, q_start=q_start, kv_len=kv_len)
+        self.tensors = (page_table, q_start, kv_len)  # kept alive with the struct
+        self.n_tok = n_tok
+        self.desc = abi.PagedBatchDesc(n, n_tok, max_new, max_len, page_table.shape[1], page_table.data_ptr(),
+                                       q_start.data_ptr(), kv_len.data_ptr())
+        ws = abi.lib().picoattn_paged_workspace_size(C.byref(cache.cfg), n)
+        if ws == 0:
+            raise abi.PicoAttnError(abi.PICOATTN_EUNSUPPORTED, "paged_workspace_size")
+        self.workspace = torch.zeros(ws, dtype=torch.uint8, device=cache.device)
+        self.ref, self.ws_ptr, self.ws_bytes = C.byref(self.desc), self.workspace.data_ptr(), ws
+
+    def status(self) -> int:
+        return workspace_status(self.workspace)
+
+
+class PagedCache:
+    """Keys and values of many sequences in pages [n_layers, n_pages, n_kv_heads,
+    page_size, head_dim] (fp16 or bf16): append a ragged batch's new tokens and
+    attend over them.  The caller deals the pages out (PagedBatch.page_table)."""
+
+    def __init__(self, cfg: abi.Config, page_size: int, n_pages: int | None = None,
+                 dtype: torch.dtype = torch.float16, device: str | torch.device = "cuda",
+                 k_pool: torch.Tensor | None = None, v_pool: torch.Tensor | None = None):
+        if k_pool is None:
+            shape = (cfg.n_layers, n_pages, cfg.n_kv_heads, page_size, cfg.head_dim)
+            k_pool = torch.zeros(shape, dtype=dtype, device=device)
+            v_pool = torch.zeros(shape, dtype=dtype, device=device)
+        want = (cfg.n_layers, k_pool.shape[1], cfg.n_kv_heads, page_size, cfg.head_dim)
+        for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
+            if tuple(t.shape) != want or t.dtype != k_pool.dtype or not t.is_contiguous():
+                raise ValueError(f"{name}: contiguous {want}, got {tuple(t.shape)} {t.dtype}")
+        self.cfg, self.k_pool, self.v_pool, self.device = cfg, k_pool, v_pool, k_pool.device
+        _same_device(self.device, v_pool=v_pool)
+        self.dtype = k_pool.dtype
+        self.desc = abi.PagedCacheDesc(k_pool.shape[1], page_size, _dtype(k_pool), k_pool.data_ptr(),
+                                       v_pool.data_ptr())
+        self.cfg_ref, self.ref = C.byref(cfg), C.byref(self.desc)
+        abi.check(abi.lib().picoattn_paged_check(self.cfg_ref, self.ref), "picoattn_paged_check")
+
+    def batch(self, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, n_tok: int, max_new: int,
+              max_len: int) -> PagedBatch:
+        return PagedBatch(self, page_table, q_start, kv_len, n_tok, max_new, max_len)
+
+    def append(self, layer: int, batch: PagedBatch, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+               rope_cos: torch.Tensor, rope_sin: torch.Tensor, q_out: torch.Tensor | None,
+               q_norm_w: torch.Tensor | None = None, k_norm_w: torch.Tensor | None = None,
+               stream: torch.cuda.Stream | None = None) -> None:
+        """k, v [n_tok, n_kv_heads, head_dim] into their pages, q [n_tok, n_heads,
+        head_dim] rotated into q_out (of the cache's type); the first
+        2 * rope_cos.shape[1] elements of each head rotate."""
+        n, hd, dev = batch.n_tok, self.cfg.head_dim, self.device
+        half = rope_cos.shape[1]
+        _check_table(rope_cos, rope_sin, half, self.cfg.max_seq_len)
+        for name, t, heads in (("q", q, self.cfg.n_heads), ("k", k, self.cfg.n_kv_heads),
+                               ("v", v, self.cfg.n_kv_heads)):
+            if t is not None and (t.dtype != k.dtype or t.numel() != n * heads * hd):
+                raise ValueError(f"{name}: [{n}, {heads}, {hd}] of one type, got {tuple(t.shape)} {t.dtype}")
+        if q_out is not None and (q_out.dtype != self.dtype or not q_out.is_contiguous() or
+                                  q_out.numel() != n * self.cfg.n_heads * hd):
+            raise ValueError(f"q_out: contiguous [{n}, {self.cfg.n_heads}, {hd}] {self.dtype}")
+        for w in (q_norm_w, k_norm_w):
+            if w is not None and (w.dtype != torch.float32 or w.numel() != hd or not w.is_contiguous()):
+                raise ValueError(f"norm weights: contiguous fp32 [{hd}]")
+        _same_device(dev, q=q, k=k, v=v, rope_cos=rope_cos, rope_sin=rope_sin, q_out=q_out, q_norm_w=q_norm_w,
+                     k_norm_w=k_norm_w)
+        st = _on_device(dev, abi.lib().picoattn_paged_append, self.cfg_ref, self.ref, layer, batch.ref, _dtype(k),
+                        abi.ptr(q), 0 if q is None else _heads(q, n, hd, "q"), k.data_ptr(), _heads(k, n, hd, "k"),
+                        v.data_ptr(), _heads(v, n, hd, "v"), abi.ptr(q_norm_w), abi.ptr(k_norm_w),
+                        rope_cos.data_ptr(), rope_sin.data_ptr(), 2 * half, abi.ptr(q_out), batch.ws_ptr,
+                        batch.ws_bytes, _launch_stream(dev, stream))
+        if st:
+            abi.check(st, "picoattn_paged_append")
+
+    def attend(self, layer: int, batch: PagedBatch, q: torch.Tensor, out: torch.Tensor,
+               stream: torch.cuda.Stream | None = None) -> None:
+        """out [n_tok, n_heads, head_dim] (the cache's type or fp32) = causal attention
+        of the rotated queries q (the cache's type) over their sequences' rows."""
+        n, hd, dev = batch.n_tok, self.cfg.head_dim, self.device
+        size = n * self.cfg.n_heads * hd
+        if q.dtype != self.dtype or q.numel() != size:
+            raise ValueError(f"q: [{n}, {self.cfg.n_heads}, {hd}] {self.dtype}, got {tuple(q.shape)} {q.dtype}")
+        if out.numel() != size or not out.is_contiguous():
+            raise ValueError(f"out: contiguous [{n}, {self.cfg.n_heads}, {hd}]")
+        _same_device(dev, q=q, out=out)
+        st = _on_device(dev, abi.lib().picoattn_paged_attn, self.cfg_ref, self.ref, layer, batch.ref, q.data_ptr(),
+                        _heads(q, n, hd, "q"), _dtype(out), out.data_ptr(), batch.ws_ptr, batch.ws_bytes,
+                        _launch_stream(dev, stream))
+        if st:
+            abi.check(st, "picoattn_paged_attn")
+
+
 class AttnState:
     """KV caches of n_seqs sequences in the reference layout plus RoPE tables.
 
