@@ -61,11 +61,11 @@ __global__ void __launch_bounds__(128) paged_attn_rows_kernel(PagedAttnArgs a) {
 }  // namespace
 
 size_t paged_workspace_bytes(const picoattn_config_t& cfg, int n_seqs) {
-    (void)cfg, (void)n_seqs;
-    return kWsHeaderBytes;
+    return kWsHeaderBytes + paged_few_bytes(cfg.head_dim, n_seqs);
 }
 
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t stream) {
+    if (paged_few_fits(a)) return launch_paged_few(a, stream);
     const unsigned grid = (unsigned)std::min<long long>(((long long)a.b.n_tok * a.hq + 3) / 4, 1 << 20);
     auto go = [&](auto kernel) { return launch_pdl(kernel, dim3(grid), dim3(128), 0, stream, a); };
     if (a.dtype == PICOATTN_DTYPE_F16)

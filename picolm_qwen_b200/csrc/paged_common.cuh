@@ -112,6 +112,11 @@ __device__ __forceinline__ void rotate_pieces(float* x, const float* c, const fl
     }
 }
 
+// Orders this thread's shared-memory writes before later async-proxy (TMA) accesses of them.
+__device__ __forceinline__ void fence_proxy_async_shared() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
 // ---- the ragged batch ---------------------------------------------------------
 
 struct SeqSpan {

@@ -1,0 +1,516 @@
+// paged_few.cu -- paged attention of sequences with few query rows: at most 16
+// rows (new tokens x q heads of a KV head) per KV head, single tokens and drafts.
+//
+// Bound by HBM: each K and V row is read once for all the q heads and new tokens
+// that share it, ~4 * 16 flop per two bytes.  A stream is the rows of one KV head
+// of one sequence; all streams are concatenated in units of 16 rows and cut into
+// equal slices, one per CTA (two CTAs per SM), so every CTA moves the same bytes
+// whatever the mix of lengths.  A producer warp copies tiles of 64 or 128 rows
+// into a three-stage ring (bulk copies of at most 16 rows: inside a page); four
+// warps take 16 keys of a tile each: S = Q K^T by m16n8k16 products (the 16 query
+// rows are the M side), online softmax in fp32 registers in the log2 domain,
+// O += P V.  The four warps' (max, sum, O) are joined in shared memory at the end
+// of a stream's part; a stream inside one slice is written as output, the parts
+// of others go to the workspace and a merge kernel joins them.
+#include <algorithm>
+#include <cmath>
+
+#include "paged_common.cuh"
+
+namespace picoattn {
+
+namespace {
+
+constexpr int kRows = 16;      // query rows (M of the products)
+constexpr int kUnit = 16;      // cache rows per unit
+constexpr int kWarps = 4;      // compute warps
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kStages = 3;
+constexpr int kMinUnits = 4;   // least units per CTA: a slice shorter than a tile gains nothing
+
+template <int HD>
+struct Few {
+    static constexpr int T = 8192 / HD;        // cache rows per tile: 16 KB of K
+    static constexpr int GR = T / 8;           // a tile is 8 groups of GR rows, each padded by 16 bytes
+    static constexpr int ROW = HD * 2;
+    static constexpr int GS = GR * ROW + 16;   // group stride: 8 rows of a product, one per group, on 8 bank quads
+    static constexpr int TILE = 8 * GS;
+    static constexpr int RG = T / 16;          // 16-key groups per tile
+    static constexpr int off_prefix = 128;     // [kThreads + 1] first unit of each thread's sequences
+    static constexpr int off_ml = off_prefix + 8 * (kThreads + 1) + 8;  // [kWarps][16] (max, sum)
+    static constexpr int off_join = off_ml + 8 * kWarps * kRows;
+    static constexpr int JS = 36;              // floats per row of the join buffer (32 columns, padded)
+    static constexpr int off_tiles = (off_join + 4 * kWarps * kRows * JS + 127) / 128 * 128;
+    static constexpr int bytes = off_tiles + kStages * 2 * TILE;
+    static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs per SM");
+};
+
+struct FewArgs {
+    PagedAttnArgs a;
+    long long* prefix;  // [n_seqs + 1] first unit of each sequence
+    float2* part_ml;    // [2 * grid][16]
+    float* part_o;      // [2 * grid][16][hd]
+};
+
+__device__ __forceinline__ long long seq_units(const SeqSpan& s, int hkv) {
+    return s.ok && s.n > 0 ? (long long)hkv * ((s.len + kUnit - 1) / kUnit) : 0;
+}
+// CTAs in use, and the units [first(i), first(i + 1)) of CTA i
+__device__ __forceinline__ int ctas_used(long long units, int grid) {
+    return (int)min((long long)grid, (units + kMinUnits - 1) / kMinUnits);
+}
+__device__ __forceinline__ long long first_unit(long long i, long long units, int ctas) { return i * units / ctas; }
+__device__ __forceinline__ int cta_of(long long unit, long long units, int ctas) {
+    int i = (int)(unit * ctas / units);
+    while (i + 1 < ctas && first_unit(i + 1, units, ctas) <= unit) i++;
+    while (i > 0 && first_unit(i, units, ctas) > unit) i--;
+    return i;
+}
+
+template <class T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value) {
+        mma_16816(d, a, b0, b1);
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
+// Four output columns of a row, in the output's type.
+template <class T>
+__device__ __forceinline__ void store_out4(const PagedAttnArgs& a, size_t at, const float4& v) {
+    if (a.out_dtype == PICOATTN_DTYPE_F32)
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+    else
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
+            make_uint2(Elem<T>::pack2(v.x, v.y), Elem<T>::pack2(v.z, v.w));
+}
+
+// Calls fn(b, span, head, u0, u1, units of the stream) for each part of the
+// units [c0, c1), in order.  chunk: first units of each thread's `per` sequences.
+template <class F>
+__device__ __forceinline__ void for_each_part(const PagedAttnArgs& a, const long long* chunk, int per, long long c0,
+                                              long long c1, F&& fn) {
+    int lo = 0, hi = kThreads;  // the last thread whose first unit is <= c0
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (chunk[mid] <= c0) lo = mid;
+        else hi = mid;
+    }
+    long long base = chunk[lo];
+    for (int b = lo * per; b < a.b.n_seqs && base < c1; b++) {
+        const SeqSpan sp = seq_span(a.b, b);
+        const long long n = seq_units(sp, a.hkv);
+        if (base + n > c0) {
+            const int per_head = (sp.len + kUnit - 1) / kUnit;
+            long long at = max(base, c0);
+            const long long end = min(base + n, c1);
+            while (at < end) {
+                const int h = (int)((at - base) / per_head);
+                const int u0 = (int)(at - base - (long long)h * per_head);
+                const int u1 = (int)min((long long)per_head, u0 + (end - at));
+                fn(b, sp, h, u0, u1, per_head);
+                at += u1 - u0;
+            }
+        }
+        base += n;
+    }
+}
+
+template <class T, int HD>
+__global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
+    using F = Few<HD>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const PagedAttnArgs& a = fa.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+    uint64_t* empty = full + kStages;
+    int* poison = reinterpret_cast<int*>(empty + kStages);  // [kStages] the tile read a page that does not exist
+    long long* warp_tot = reinterpret_cast<long long*>(smem + 64);  // [kWarps + 1]
+    long long* chunk = reinterpret_cast<long long*>(smem + F::off_prefix);
+    float2* ml = reinterpret_cast<float2*>(smem + F::off_ml);
+    float* join = reinterpret_cast<float*>(smem + F::off_join);
+    uint8_t* tiles = smem + F::off_tiles;
+
+    pdl_trigger();
+    if (tid == 0) {
+        for (int s = 0; s < kStages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], kWarps);
+        fence_mbar_init();
+    }
+    pdl_wait();
+    // first units of every thread's sequences
+    const int per = (a.b.n_seqs + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, a.b.n_seqs), b1 = min(b0 + per, a.b.n_seqs);
+    long long mine = 0;
+    for (int b = b0; b < b1; b++) {
+        const SeqSpan sp = seq_span(a.b, b);
+        if (!sp.ok && blockIdx.x == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+        mine += seq_units(sp, a.hkv);
+    }
+    long long incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_tot[warp] = incl;
+    __syncthreads();
+    long long first = incl - mine;
+    for (int w = 0; w < warp; w++) first += warp_tot[w];
+    chunk[tid] = first;
+    if (tid == kThreads - 1) chunk[kThreads] = first + mine;
+    if (blockIdx.x == 0) {  // for the merge kernel
+        long long run = first;
+        for (int b = b0; b < b1; b++) {
+            fa.prefix[b] = run;
+            run += seq_units(seq_span(a.b, b), a.hkv);
+        }
+        if (tid == kThreads - 1) fa.prefix[a.b.n_seqs] = first + mine;
+    }
+    __syncthreads();
+    const long long units = chunk[kThreads];
+    const int ctas = ctas_used(units, gridDim.x);
+    if ((int)blockIdx.x >= ctas) return;
+    const long long c0 = first_unit(blockIdx.x, units, ctas), c1 = first_unit(blockIdx.x + 1, units, ctas);
+
+    if (warp == kWarps) {
+        // ---------------- producer: lanes 0-7 the K groups, 8-15 the V groups ----------------
+        int t = 0;
+        const uint8_t* pool = static_cast<const uint8_t*>(lane & 8 ? a.v_pool : a.k_pool);
+        for_each_part(a, chunk, per, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int) {
+            const int r1 = min(u1 * kUnit, sp.len);
+            const int* table = a.b.page_table + (size_t)b * a.b.page_cols;
+            for (int row0 = u0 * kUnit; row0 < r1; row0 += F::T, t++) {
+                const int s = t % kStages;
+                const int g0 = row0 + F::GR * (lane & 7);
+                const bool copy = lane < 16 && g0 < r1;
+                const int page = copy ? table[g0 >> a.b.page_shift] : 0;
+                const bool bad = page < 0 || page >= a.b.n_pages;
+                const int any_bad = __any_sync(0xffffffffu, bad);
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, copy)) * (uint32_t)(F::GR * F::ROW);
+                if (t >= kStages) mbar_wait(&empty[s], (uint32_t)((t / kStages - 1) & 1), a.b.status);
+                if (lane == 0) {
+                    if (any_bad) atomicOr(a.b.status, PICOATTN_DEV_BAD_PAGE);
+                    poison[s] = any_bad;
+                    mbar_arrive_expect_tx(&full[s], bytes);
+                }
+                __syncwarp();
+                if (copy) {
+                    const size_t row = ((size_t)(bad ? 0 : page) * a.hkv + h) * a.b.page_size + (g0 & (a.b.page_size - 1));
+                    bulk_g2s(tiles + (s * 2 + (lane >> 3)) * F::TILE + (lane & 7) * F::GS, pool + row * F::ROW,
+                             F::GR * F::ROW, &full[s]);
+                }
+            }
+        });
+        return;
+    }
+
+    // ---------------- compute warps ----------------
+    const int gid = lane >> 2, tig = lane & 3;
+    // ldmatrix rows (matrix lane >> 3, its row lane & 7 = tile group): K (keys 0-7 | dims 0-7, keys 0-7 | dims 8-15,
+    // keys 8-15 | ..), V transposed (keys 0-7 | dims 0-7, keys 8-15 | dims 0-7, ..); key 8j + q of 16-key group rg is
+    // tile row GR q + 2 rg + j
+    const uint32_t k_lane = (uint32_t)((lane & 7) * F::GS + (lane >> 4) * F::ROW + ((lane >> 3) & 1) * 16);
+    const uint32_t v_lane = (uint32_t)((lane & 7) * F::GS + ((lane >> 3) & 1) * F::ROW + (lane >> 4) * 16);
+    const uint32_t tiles_u32 = smem_u32(tiles);
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);
+    int t = 0;
+    for_each_part(a, chunk, per, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
+        const int rows = sp.n * a.g;  // <= kRows
+        uint32_t qa[HD / 16][4];
+        int lim[2];  // keys below it are visible to the lane's rows gid, gid + 8
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const int r = gid + 8 * half;
+            const int i = r / a.g;
+            lim[half] = sp.len - sp.n + i + 1;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(
+                static_cast<const T*>(a.q) + (sp.t0 + i) * a.qs + (size_t)(h * a.g + r - i * a.g) * HD + 2 * tig);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk++) {
+                qa[kk][half] = r < rows ? src[8 * kk] : 0u;
+                qa[kk][2 + half] = r < rows ? src[8 * kk + 4] : 0u;
+            }
+        }
+        float m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};
+        float o[HD / 8][4];
+#pragma unroll
+        for (int i = 0; i < HD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        const int r1 = min(u1 * kUnit, sp.len);
+        for (int row0 = u0 * kUnit; row0 < r1; row0 += F::T, t++) {
+            const int s = t % kStages;
+            mbar_wait(&full[s], (uint32_t)((t / kStages) & 1), a.b.status);
+            const uint32_t kbase = tiles_u32 + (uint32_t)(s * 2 * F::TILE), vbase = kbase + F::TILE;
+            const int valid = r1 - row0;
+            if (poison[s]) l[0] = l[1] = __int_as_float(0x7fc00000);
+            const bool mask = row0 + F::T > sp.len - sp.n + 1 || valid < F::T;
+            const int lim0 = min(lim[0] - row0, valid), lim1 = min(lim[1] - row0, valid);
+#pragma unroll
+            for (int rg = warp; rg < F::RG; rg += kWarps) {
+                if (2 * rg >= valid) continue;
+                if (valid < F::T) {
+                    // rows past the part hold anything: their V must not meet the zero weights as a NaN.  This warp
+                    // alone reads the rows of its key groups
+                    for (int e = lane; e < 16 * (F::ROW / 16); e += 32) {
+                        const int key = e / (F::ROW / 16), q = key & 7, u = 2 * rg + (key >> 3);
+                        if (F::GR * q + u >= valid)
+                            *reinterpret_cast<uint4*>(tiles + (s * 2 + 1) * F::TILE + q * F::GS + u * F::ROW +
+                                                      (e % (F::ROW / 16)) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_shared();  // before the ring's next copy into these rows
+                    __syncwarp();
+                }
+                const uint32_t goff = (uint32_t)(2 * rg * F::ROW);
+                float sc[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk++) {
+                    uint32_t bk[4];
+                    ldsm_x4(bk, kbase + goff + k_lane + (uint32_t)kk * 32u);
+                    mma16<T>(sc[0], qa[kk], bk[0], bk[1]);
+                    mma16<T>(sc[1], qa[kk], bk[2], bk[3]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        sc[j][e] *= scale;
+                        if (mask && F::GR * (2 * tig + (e & 1)) + 2 * rg + j >= (e < 2 ? lim0 : lim1))
+                            sc[j][e] = -INFINITY;
+                    }
+                float mx0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
+                float mx1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3]));
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+                const float mn0 = fmaxf(m[0], mx0), mn1 = fmaxf(m[1], mx1);
+                const float f0 = ex2(m[0] - mn0), f1 = ex2(m[1] - mn1);
+                m[0] = mn0;
+                m[1] = mn1;
+                float p[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    p[j][0] = ex2(sc[j][0] - mn0);
+                    p[j][1] = ex2(sc[j][1] - mn0);
+                    p[j][2] = ex2(sc[j][2] - mn1);
+                    p[j][3] = ex2(sc[j][3] - mn1);
+                }
+                l[0] = l[0] * f0 + ((p[0][0] + p[0][1]) + (p[1][0] + p[1][1]));
+                l[1] = l[1] * f1 + ((p[0][2] + p[0][3]) + (p[1][2] + p[1][3]));
+                if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
+#pragma unroll
+                    for (int i = 0; i < HD / 8; i++) {
+                        o[i][0] *= f0, o[i][1] *= f0;
+                        o[i][2] *= f1, o[i][3] *= f1;
+                    }
+                }
+                const uint32_t pa[4] = {Elem<T>::pack2(p[0][0], p[0][1]), Elem<T>::pack2(p[0][2], p[0][3]),
+                                        Elem<T>::pack2(p[1][0], p[1][1]), Elem<T>::pack2(p[1][2], p[1][3])};
+#pragma unroll
+                for (int dt = 0; dt < HD / 16; dt++) {
+                    uint32_t bv[4];
+                    ldsm_x4_t(bv, vbase + goff + v_lane + (uint32_t)dt * 32u);
+                    mma16<T>(o[2 * dt], pa, bv[0], bv[1]);
+                    mma16<T>(o[2 * dt + 1], pa, bv[2], bv[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+
+        // join the four warps' (max, sum, O): thread (row tid / 8, four columns)
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+            if (tig == 0) ml[warp * kRows + gid + 8 * half] = make_float2(m[half], l[half]);
+        }
+        named_bar_sync(1, 32 * kWarps);
+        float wgt[2];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            float M = ml[gid + 8 * half].x;
+#pragma unroll
+            for (int w = 1; w < kWarps; w++) M = fmaxf(M, ml[w * kRows + gid + 8 * half].x);
+            wgt[half] = ex2(m[half] - M);
+        }
+        const int jr = tid >> 3, jc = (tid & 7) * 4;
+        float M = ml[jr].x, Ls = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) M = fmaxf(M, ml[w * kRows + jr].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) Ls += ml[w * kRows + jr].y * ex2(ml[w * kRows + jr].x - M);
+        const bool whole = u0 == 0 && u1 == stream_units;
+        const size_t slot = 2 * (size_t)blockIdx.x + (u0 == 0 ? 1 : 0);
+        const int ji = jr / a.g;
+        const size_t orow = ((size_t)(sp.t0 + ji) * a.hq + (size_t)(h * a.g + jr - ji * a.g)) * HD;
+        if (!whole && (tid & 7) == 0 && jr < rows) fa.part_ml[slot * kRows + jr] = make_float2(M, Ls);
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float* d = join + (warp * kRows + gid) * F::JS + 8 * i + 2 * tig;
+                *reinterpret_cast<float2*>(d) = make_float2(o[4 * c + i][0] * wgt[0], o[4 * c + i][1] * wgt[0]);
+                *reinterpret_cast<float2*>(d + 8 * F::JS) = make_float2(o[4 * c + i][2] * wgt[1], o[4 * c + i][3] * wgt[1]);
+            }
+            named_bar_sync(1, 32 * kWarps);
+            if (jr < rows) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) {
+                    const float4 x = *reinterpret_cast<const float4*>(join + (w * kRows + jr) * F::JS + jc);
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                }
+                if (whole) {
+                    const float inv = 1.0f / Ls;
+                    store_out4<T>(a, orow + 32 * c + jc, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                } else {
+                    *reinterpret_cast<float4*>(fa.part_o + (slot * kRows + jr) * HD + 32 * c + jc) = v;
+                }
+            }
+            named_bar_sync(1, 32 * kWarps);
+        }
+    });
+}
+
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the parts of one
+// query row of a stream cut across CTAs; block (row, stream), thread (part
+// group, four columns).  All loads of a row's first parts are in flight at
+// once: the merge is one round trip to L2.  Rows of a sequence outside the
+// host's bounds become NaN here.
+constexpr int kMergeThreads = 128;
+constexpr int kMaxParts = 2 * 256;  // CTAs of the attention kernel
+
+template <class T, int HD>
+__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs fa, int grid) {
+    constexpr int C4 = HD / 4, NG = kMergeThreads / C4, RPT = 40 / NG;
+    __shared__ float w_s[kMaxParts], red[kMergeThreads / 32][2];
+    __shared__ float4 acc_s[kMergeThreads];
+    pdl_trigger();
+    pdl_wait();
+    const PagedAttnArgs& a = fa.a;
+    const int tid = threadIdx.x, c4 = tid % C4, grp = tid / C4;
+    const int b = (int)(blockIdx.y / a.hkv), h = (int)(blockIdx.y % a.hkv), r = blockIdx.x;
+    const SeqSpan sp = seq_span(a.b, b);
+    if (!sp.ok) {
+        const int t0 = max(sp.t0, 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
+        const float nan = __int_as_float(0x7fc00000);
+        for (long long x = r; x < (long long)(t1 - t0) * a.g; x += gridDim.x)
+            for (int c = tid; c < C4; c += kMergeThreads)
+                store_out4<T>(a, ((size_t)(t0 + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * c,
+                              make_float4(nan, nan, nan, nan));
+        return;
+    }
+    if (r >= sp.n * a.g) return;
+    const long long units = fa.prefix[a.b.n_seqs];
+    const int per_head = (sp.len + kUnit - 1) / kUnit, ctas = ctas_used(units, grid);
+    const long long s0 = fa.prefix[b] + (long long)h * per_head;
+    const int lo = cta_of(s0, units, ctas), hi = cta_of(s0 + per_head - 1, units, ctas);
+    if (lo == hi) return;  // written by the attention kernel
+    const int parts = hi - lo + 1;
+    auto slot = [&](int p) -> size_t {  // the first part begins its stream, the others are their CTA's first
+        const bool begins = p == 0;
+        return ((size_t)(lo + p) * 2 + (begins ? 1 : 0)) * kRows + r;
+    };
+    float4 v[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+        const int p = grp + i * NG;
+        if (p < parts) v[i] = __ldcg(reinterpret_cast<const float4*>(fa.part_o + slot(p) * HD) + c4);
+    }
+    float M = -INFINITY;
+    float2 x[kMaxParts / kMergeThreads];
+#pragma unroll
+    for (int i = 0; i < kMaxParts / kMergeThreads; i++) {
+        const int p = tid + i * kMergeThreads;
+        x[i] = p < parts ? __ldcg(fa.part_ml + slot(p)) : make_float2(-INFINITY, 0.f);
+        M = fmaxf(M, x[i].x);
+    }
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if ((tid & 31) == 0) red[tid >> 5][0] = M;
+    __syncthreads();
+    for (int w = 0; w < kMergeThreads / 32; w++) M = fmaxf(M, red[w][0]);
+    float L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaxParts / kMergeThreads; i++) {
+        const int p = tid + i * kMergeThreads;
+        if (p < parts) {
+            const float w = ex2(x[i].x - M);
+            w_s[p] = w;
+            L += w * x[i].y;
+        }
+    }
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if ((tid & 31) == 0) red[tid >> 5][1] = L;
+    __syncthreads();
+    L = 0.f;
+    for (int w = 0; w < kMergeThreads / 32; w++) L += red[w][1];
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int p, const float4& y) {
+        const float w = w_s[p];
+        acc.x += w * y.x, acc.y += w * y.y, acc.z += w * y.z, acc.w += w * y.w;
+    };
+#pragma unroll
+    for (int i = 0; i < RPT; i++)
+        if (grp + i * NG < parts) add(grp + i * NG, v[i]);
+    for (int p = grp + RPT * NG; p < parts; p += NG)
+        add(p, __ldcg(reinterpret_cast<const float4*>(fa.part_o + slot(p) * HD) + c4));
+    acc_s[tid] = acc;
+    __syncthreads();
+    if (grp == 0) {
+        for (int g = 1; g < NG; g++) {
+            const float4 y = acc_s[g * C4 + c4];
+            acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+        }
+        const float inv = 1.0f / L;
+        const int i = r / a.g;
+        store_out4<T>(a, ((size_t)(sp.t0 + i) * a.hq + (size_t)(h * a.g + r - i * a.g)) * HD + 4 * c4,
+                      make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
+}
+
+int max_grid() { return std::min(2 * device_sm_count(), kMaxParts); }
+
+template <class T, int HD>
+cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
+    using F = Few<HD>;
+    static PerDeviceOnce setup;
+    cudaError_t e = setup.run([] {
+        return cudaFuncSetAttribute(paged_few_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::bytes);
+    });
+    if (e != cudaSuccess) return e;
+    const long long units = (long long)a.b.n_seqs * a.hkv * ((a.b.max_len + kUnit - 1) / kUnit);
+    const int grid = (int)std::min<long long>(max_grid(), (units + kMinUnits - 1) / kMinUnits);
+    FewArgs fa{};
+    fa.a = a;
+    fa.part_ml = reinterpret_cast<float2*>(a.ws);
+    fa.part_o = reinterpret_cast<float*>(a.ws + (size_t)2 * max_grid() * kRows * 8);
+    fa.prefix = reinterpret_cast<long long*>(a.ws + (size_t)2 * max_grid() * kRows * (8 + 4 * HD));
+    e = launch_pdl(paged_few_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)F::bytes, stream, fa);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(paged_few_merge_kernel<T, HD>, dim3(a.b.max_new * a.g, a.b.n_seqs * a.hkv), dim3(kMergeThreads), 0,
+                      stream, fa, grid);
+}
+
+}  // namespace
+
+bool paged_few_fits(const PagedAttnArgs& a) {
+    return (long long)a.b.max_new * a.g <= kRows && (long long)a.b.n_seqs * a.hkv <= 65535;
+}
+
+size_t paged_few_bytes(int hd, int n_seqs) {
+    return align_up((size_t)2 * max_grid() * kRows * (8 + 4 * hd) + (size_t)(n_seqs + 1) * 8, 256);
+}
+
+cudaError_t launch_paged_few(const PagedAttnArgs& a, cudaStream_t stream) {
+    if (a.dtype == PICOATTN_DTYPE_F16)
+        return a.hd == 64 ? launch_types<__half, 64>(a, stream) : launch_types<__half, 128>(a, stream);
+    return a.hd == 64 ? launch_types<__nv_bfloat16, 64>(a, stream) : launch_types<__nv_bfloat16, 128>(a, stream);
+}
+
+}  // namespace picoattn
