@@ -606,32 +606,40 @@ typedef struct {
     int64_t     x_stride;   /* elements from a token's row to the next (>= 0; 0: one row for all) */
     void*       out;        /* may equal x (with the same stride): rotated in place */
     int64_t     out_stride; /* >= n_heads*head_dim */
-    int32_t     n_heads;
+    int64_t     n_heads;
 } picoattn_rope_rows_t;
+
+typedef struct {
+    int32_t dtype;            /* PICOATTN_DTYPE_F32, _F16 or _BF16, of every x and out */
+    int32_t rope_mode;        /* PICOATTN_ROPE_NEOX (pairs i, i + rot_dim/2) or _INTERLEAVED (2i, 2i + 1) */
+    int32_t head_dim;         /* even, 2..1024 */
+    int32_t rot_dim;          /* even, 2..head_dim */
+    int32_t inverse;          /* non-zero: the opposite angles */
+    int32_t n_tok;            /* at least 1 */
+    int32_t table_rows;
+    int32_t n_tensors;        /* 1: q alone; 2: q and k */
+    const int32_t* pos;       /* device [n_tok] */
+    const float* rope_cos;    /* device [table_rows][rot_dim/2], 4-byte aligned */
+    const float* rope_sin;
+    picoattn_rope_rows_t q, k;
+} picoattn_rope_args_t;
 
 /*
  * Rotates the first rot_dim elements of every head of q, and of k when given,
- * by the table row of the token's position, and copies the others.
- *   dtype     PICOATTN_DTYPE_F32, _F16 or _BF16, of x and out; each product and
- *             sum in fp32, the result rounded to nearest even once
- *   rope_mode PICOATTN_ROPE_NEOX (pairs i, i + rot_dim/2) or _INTERLEAVED (2i, 2i + 1)
- *   head_dim  even, 2..1024; rot_dim even, 2..head_dim
- *   inverse   non-zero: rotates by the opposite angles.  It is the rotation's
- *             transpose, so it takes the gradient of the output to the
- *             gradient of the input (tables scaled by mscale: times mscale again)
- *   pos       [n_tok] int32 device; one outside [0, table_rows) sets
- *             PICOATTN_DEV_BAD_POS and its output rows are NaN
- *   rope_cos, rope_sin  [table_rows][rot_dim/2] fp32 device, 4-byte aligned
+ * by the table row of the token's position, and copies the others: each product
+ * and sum in fp32, the result rounded to nearest even once.
+ *   inverse   is the rotation's transpose, so it takes the gradient of the output
+ *             to the gradient of the input (tables scaled by mscale: times mscale
+ *             again)
+ *   pos       one outside [0, table_rows) sets PICOATTN_DEV_BAD_POS and its output
+ *             rows are NaN
  *   workspace at least 256 bytes (the status word)
  * x and out may be any element-aligned addresses; an output that overlaps an
  * input without being in place, or the other output, is PICOATTN_EINVAL.  (The
  * rows of q and k may interleave, as in one q|k|v projection's output.)
  */
-int32_t picoattn_rope(int32_t dtype, int32_t rope_mode, int32_t head_dim, int32_t rot_dim, int32_t inverse,
-                      int32_t n_tok, const int32_t* pos, int32_t table_rows,
-                      const float* rope_cos, const float* rope_sin,
-                      const picoattn_rope_rows_t* q, const picoattn_rope_rows_t* k,
-                      void* workspace, size_t workspace_bytes, picoattn_stream_t stream);
+int32_t picoattn_rope(const picoattn_rope_args_t* args, void* workspace, size_t workspace_bytes,
+                      picoattn_stream_t stream);
 
 /* ---------------------------------------------------------------------- */
 /* Paged KV cache: append and attention for ragged batches                 */
@@ -652,7 +660,7 @@ typedef struct {
 /* The sequences of one step.  Sequence b has the new tokens q_start[b] ..
  * q_start[b+1]-1 (rows of q, k, v and out; none is allowed), the last of them
  * at position kv_len[b]-1: kv_len counts the new tokens.  Rows of q, k, v and
- * out outside [q_start[0], q_start[n_seqs]) are neither read nor written, so a
+ * out outside [q_start[0], q_start[n_seqs]) are not used and not written, so a
  * captured step may be padded.  The three bounds are host values, the lengths
  * device values: a sequence with more than max_new new tokens, a kv_len above
  * max_len or below its new tokens, or rows outside [0, n_tok) sets
@@ -678,29 +686,35 @@ int32_t picoattn_paged_check(const picoattn_config_t* cfg, const picoattn_paged_
  * may run at the same time need workspaces of their own. */
 size_t picoattn_paged_workspace_size(const picoattn_config_t* cfg, int32_t n_seqs);
 
+/* Inputs and output of picoattn_paged_append. */
+typedef struct {
+    int32_t in_dtype;       /* PICOATTN_DTYPE_F32, _F16 or _BF16 of q, k and v */
+    int32_t rot_dim;        /* multiple of 16, 16..head_dim */
+    const void* q;          /* [n_tok] rows of n_heads heads; q and q_out may both be NULL */
+    int64_t q_stride;       /* elements from a token's row to the next (a q|k|v projection's output needs no split) */
+    const void* k;          /* [n_tok] rows of n_kv_heads heads */
+    int64_t k_stride;
+    const void* v;
+    int64_t v_stride;
+    const float* q_norm_w;  /* [head_dim] QK-RMSNorm weights, or both NULL */
+    const float* k_norm_w;
+    const float* rope_cos;  /* [max_seq_len][rot_dim/2] (picoattn_rope_table or picoattn_rope_scaled_table) */
+    const float* rope_sin;
+    void* q_out;            /* [n_tok][n_heads*head_dim] in the cache's type, not overlapping q, k, v */
+} picoattn_paged_append_args_t;
+
 /*
  * The new tokens' keys and values into their pages, and their queries made
  * ready for picoattn_paged_attn: QK-RMSNorm (when the weights are given), RoPE of
  * the first rot_dim elements at the token's position, rounding to the cache's
- * type (F16 by the reference's rule as in picoattn_decode, BF16 to nearest even).
- *   in_dtype  PICOATTN_DTYPE_F32, _F16 or _BF16 of q, k and v
- *   q, k, v   [n_tok] rows of heads; q_stride, k_stride, v_stride: elements from
- *             a token's row to the next (a q|k|v projection's output needs no
- *             split).  q and q_out may both be NULL
- *   q_out     [n_tok][n_heads*head_dim] in the cache's type, not overlapping q, k, v
- *   rope_cos, rope_sin  [max_seq_len][rot_dim/2] (picoattn_rope_table or
- *             picoattn_rope_scaled_table)
- *   rot_dim   multiple of 16, 16..head_dim
- * q, k, v and q_out 16-byte aligned with strides of whole 16 bytes.  A page table entry
- * outside [0, n_pages) sets PICOATTN_DEV_BAD_PAGE and the row is not stored.
- * Two sequences that share a page must not both append to it.
+ * type (k and v in F16 by the reference's rule as in picoattn_decode; q_out and
+ * BF16 to nearest even).  q, k, v and q_out 16-byte aligned, strides whole 16
+ * bytes.  A page table entry outside [0, n_pages) sets PICOATTN_DEV_BAD_PAGE and
+ * the row is not stored.  Two sequences that share a page must not both append
+ * to it.
  */
 int32_t picoattn_paged_append(const picoattn_config_t* cfg, const picoattn_paged_cache_t* cache, int32_t layer,
-                              const picoattn_paged_batch_t* batch, int32_t in_dtype,
-                              const void* q, int64_t q_stride, const void* k, int64_t k_stride,
-                              const void* v, int64_t v_stride,
-                              const float* q_norm_w, const float* k_norm_w,
-                              const float* rope_cos, const float* rope_sin, int32_t rot_dim, void* q_out,
+                              const picoattn_paged_batch_t* batch, const picoattn_paged_append_args_t* args,
                               void* workspace, size_t workspace_bytes, picoattn_stream_t stream);
 
 /*

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libpicoattn.so")
@@ -128,7 +129,26 @@ class RopeScaling(C.Structure):
 class RopeRows(C.Structure):
     """picoattn_rope_rows_t: the heads of one tensor."""
     _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
-                ("n_heads", C.c_int32)]
+                ("n_heads", C.c_int64)]
+
+
+class RopeArgs(C.Structure):
+    """picoattn_rope_args_t."""
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "rope_mode", "head_dim", "rot_dim", "inverse", "n_tok", "table_rows",
+                                         "n_tensors")] + \
+        [(n, C.c_void_p) for n in ("pos", "rope_cos", "rope_sin")] + [("q", RopeRows), ("k", RopeRows)]
+
+
+class PagedAppendArgs(C.Structure):
+    """picoattn_paged_append_args_t."""
+    _fields_ = [("in_dtype", C.c_int32), ("rot_dim", C.c_int32), ("q", C.c_void_p), ("q_stride", C.c_int64),
+                ("k", C.c_void_p), ("k_stride", C.c_int64), ("v", C.c_void_p), ("v_stride", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("q_norm_w", "k_norm_w", "rope_cos", "rope_sin", "q_out")]
+
+
+# the same two structs for struct.pack: one conversion for all fields of a call
+ROPE_ARGS = struct.Struct("=8i 3Q QqQqq QqQqq")
+PAGED_APPEND_ARGS = struct.Struct("=2i QqQqQq 5Q")
 
 
 class PagedCacheDesc(C.Structure):
@@ -215,14 +235,11 @@ PROTOTYPES = {
     "picoattn_decode_block": (_I, [_CFG, _I, _I, _I, _I, _I, _P, C.POINTER(LayerWeights), _P, C.POINTER(FfnWeights),
                                    _P, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "picoattn_rope_scaled_table": (_I, [_CFG, C.POINTER(RopeScaling), _P, _P]),
-    "picoattn_rope": (_I, [_I, _I, _I, _I, _I, _I, _P, _I, _P, _P, C.POINTER(RopeRows), C.POINTER(RopeRows), _P, _Z,
-                           _P]),
+    "picoattn_rope": (_I, [_P, _P, _Z, _P]),
     "picoattn_paged_check": (_I, [_CFG, C.POINTER(PagedCacheDesc)]),
     "picoattn_paged_workspace_size": (_Z, [_CFG, _I]),
-    "picoattn_paged_append": (_I, [_CFG, C.POINTER(PagedCacheDesc), _I, C.POINTER(PagedBatchDesc), _I, _P, _L, _P, _L,
-                                   _P, _L, _P, _P, _P, _P, _I, _P, _P, _Z, _P]),
-    "picoattn_paged_attn": (_I, [_CFG, C.POINTER(PagedCacheDesc), _I, C.POINTER(PagedBatchDesc), _P, _L, _I, _P, _P,
-                                 _Z, _P]),
+    "picoattn_paged_append": (_I, [_P, _P, _I, _P, _P, _P, _Z, _P]),
+    "picoattn_paged_attn": (_I, [_P, _P, _I, _P, _P, _L, _I, _P, _P, _Z, _P]),
 }
 
 _lib = None

@@ -23,6 +23,7 @@
 //          of longer sequences go to partial slots.
 //   merge  log-sum-exp combination of the pieces of each sequence that was
 //          split across CTAs.
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <utility>
@@ -1307,9 +1308,13 @@ cudaError_t launch_decode_hd(const DecodeArgs& a_in, const DecodePlan& plan, cud
 }  // namespace
 
 int device_sm_count() {
+    static std::atomic<int> seen[64];  // per device, 0: not asked yet
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    const bool slot = dev >= 0 && dev < 64;
+    if (slot && (n = seen[dev].load(std::memory_order_relaxed)) > 0) return n;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    if (slot) seen[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 

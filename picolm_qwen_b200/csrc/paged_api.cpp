@@ -46,14 +46,14 @@ bool rows_overlap(const void* p, int64_t ps, int64_t pw, const void* q, int64_t 
 constexpr int64_t kMaxStride = int64_t(1) << 28;   // keeps n_tok * stride in bytes inside 64 bits
 
 int32_t rope_rows(const picoattn_rope_rows_t* r, int32_t hd, int32_t n_tok, size_t es, RopeRows* out) {
-    if (!r->x || !r->out || r->n_heads <= 0) return PICOATTN_EINVAL;
-    const int64_t w = (int64_t)r->n_heads * hd;
+    if (!r->x || !r->out || r->n_heads <= 0 || r->n_heads > (1 << 20)) return PICOATTN_EINVAL;
+    const int64_t w = r->n_heads * hd;
     if (r->x_stride < 0 || r->x_stride > kMaxStride || r->out_stride < w || r->out_stride > kMaxStride)
         return PICOATTN_EINVAL;
     if (!aligned(r->x, es) || !aligned(r->out, es)) return PICOATTN_EINVAL;
     const bool in_place = r->x == r->out && (r->x_stride == r->out_stride || n_tok == 1);
     if (!in_place && rows_overlap(r->x, r->x_stride, w, r->out, r->out_stride, w, n_tok, es)) return PICOATTN_EINVAL;
-    *out = {r->x, r->out, r->x_stride, r->out_stride, r->n_heads};
+    *out = {r->x, r->out, r->x_stride, r->out_stride, (int)r->n_heads};
     return PICOATTN_OK;
 }
 
@@ -65,6 +65,8 @@ int32_t batch_check(const picoattn_config_t* cfg, const picoattn_paged_cache_t* 
     if (!aligned(b->page_table, 4) || !aligned(b->q_start, 4) || !aligned(b->kv_len, 4)) return PICOATTN_EINVAL;
     if (layer < 0 || layer >= cfg->n_layers) return PICOATTN_EINVAL;
     if (b->n_seqs <= 0 || b->n_tok <= 0 || b->max_new <= 0 || b->page_cols <= 0) return PICOATTN_EINVAL;
+    // the kernels count heads of tokens in 32 bits
+    if ((int64_t)b->n_tok * (cfg->n_heads + 2 * (int64_t)cfg->n_kv_heads) > INT32_MAX) return PICOATTN_EUNSUPPORTED;
     if (b->max_len <= 0 || b->max_len > cfg->max_seq_len || b->max_new > b->max_len ||
         b->max_len > (int64_t)b->page_cols * c->page_size)
         return PICOATTN_ERANGE;
@@ -120,33 +122,34 @@ int32_t picoattn_rope_scaled_table(const picoattn_config_t* c, const picoattn_ro
     return PICOATTN_OK;
 }
 
-int32_t picoattn_rope(int32_t dtype, int32_t rope_mode, int32_t head_dim, int32_t rot_dim, int32_t inverse,
-                      int32_t n_tok, const int32_t* pos, int32_t table_rows, const float* rope_cos,
-                      const float* rope_sin, const picoattn_rope_rows_t* q, const picoattn_rope_rows_t* k,
-                      void* workspace, size_t workspace_bytes, picoattn_stream_t stream) {
-    if (!dtype_ok(dtype) || !mode_ok(rope_mode)) return PICOATTN_EINVAL;
-    if (head_dim < 2 || head_dim % 2 || rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim) return PICOATTN_EINVAL;
-    if (head_dim > 1024) return PICOATTN_EUNSUPPORTED;
-    if (n_tok <= 0 || table_rows <= 0 || !pos || !rope_cos || !rope_sin || !q) return PICOATTN_EINVAL;
-    if (!aligned(pos, 4) || !aligned(rope_cos, 4) || !aligned(rope_sin, 4)) return PICOATTN_EINVAL;
-    const size_t es = elem_size(dtype);
+int32_t picoattn_rope(const picoattn_rope_args_t* r, void* workspace, size_t workspace_bytes,
+                      picoattn_stream_t stream) {
+    if (!r || !dtype_ok(r->dtype) || !mode_ok(r->rope_mode)) return PICOATTN_EINVAL;
+    const int32_t hd = r->head_dim, n = r->n_tok;
+    if (hd < 2 || hd % 2 || r->rot_dim < 2 || r->rot_dim % 2 || r->rot_dim > hd) return PICOATTN_EINVAL;
+    if (hd > 1024) return PICOATTN_EUNSUPPORTED;
+    if (n <= 0 || r->table_rows <= 0 || !r->pos || !r->rope_cos || !r->rope_sin) return PICOATTN_EINVAL;
+    if (r->n_tensors != 1 && r->n_tensors != 2) return PICOATTN_EINVAL;
+    if (!aligned(r->pos, 4) || !aligned(r->rope_cos, 4) || !aligned(r->rope_sin, 4)) return PICOATTN_EINVAL;
+    const size_t es = elem_size(r->dtype);
+    const picoattn_rope_rows_t &q = r->q, &k = r->k;
     RopeArgs a{};
-    int32_t st = rope_rows(q, head_dim, n_tok, es, &a.t[0]);
-    if (st == PICOATTN_OK && k) st = rope_rows(k, head_dim, n_tok, es, &a.t[1]);
+    int32_t st = rope_rows(&q, hd, n, es, &a.t[0]);
+    if (st == PICOATTN_OK && r->n_tensors == 2) st = rope_rows(&k, hd, n, es, &a.t[1]);
     if (st != PICOATTN_OK) return st;
-    if (k) {  // neither output may touch the other tensor
-        const int64_t qw = (int64_t)q->n_heads * head_dim, kw = (int64_t)k->n_heads * head_dim;
-        if (rows_overlap(q->out, q->out_stride, qw, k->out, k->out_stride, kw, n_tok, es) ||
-            rows_overlap(q->out, q->out_stride, qw, k->x, k->x_stride, kw, n_tok, es) ||
-            rows_overlap(k->out, k->out_stride, kw, q->x, q->x_stride, qw, n_tok, es))
+    if (r->n_tensors == 2) {  // neither output may touch the other tensor
+        const int64_t qw = q.n_heads * hd, kw = k.n_heads * hd;
+        if (rows_overlap(q.out, q.out_stride, qw, k.out, k.out_stride, kw, n, es) ||
+            rows_overlap(q.out, q.out_stride, qw, k.x, k.x_stride, kw, n, es) ||
+            rows_overlap(k.out, k.out_stride, kw, q.x, q.x_stride, qw, n, es))
             return PICOATTN_EINVAL;
     }
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < kWsHeaderBytes) return PICOATTN_ENOSPACE;
     st = picoattn_device_check();
     if (st != PICOATTN_OK) return st;
-    a.dtype = dtype, a.mode = rope_mode, a.hd = head_dim, a.rot = rot_dim, a.inverse = inverse ? 1 : 0;
-    a.n_tok = n_tok, a.table_rows = table_rows;
-    a.pos = pos, a.cos_t = rope_cos, a.sin_t = rope_sin;
+    a.dtype = r->dtype, a.mode = r->rope_mode, a.hd = hd, a.rot = r->rot_dim, a.inverse = r->inverse ? 1 : 0;
+    a.n_tok = n, a.table_rows = r->table_rows;
+    a.pos = r->pos, a.cos_t = r->rope_cos, a.sin_t = r->rope_sin;
     a.status = static_cast<unsigned int*>(workspace);
     return cuda_status(launch_rope(a, (cudaStream_t)stream));
 }
@@ -176,41 +179,40 @@ size_t picoattn_paged_workspace_size(const picoattn_config_t* c, int32_t n_seqs)
 }
 
 int32_t picoattn_paged_append(const picoattn_config_t* cfg, const picoattn_paged_cache_t* cache, int32_t layer,
-                              const picoattn_paged_batch_t* batch, int32_t in_dtype, const void* q, int64_t q_stride,
-                              const void* k, int64_t k_stride, const void* v, int64_t v_stride, const float* q_norm_w,
-                              const float* k_norm_w, const float* rope_cos, const float* rope_sin, int32_t rot_dim,
-                              void* q_out, void* workspace, size_t workspace_bytes, picoattn_stream_t stream) {
+                              const picoattn_paged_batch_t* batch, const picoattn_paged_append_args_t* r,
+                              void* workspace, size_t workspace_bytes, picoattn_stream_t stream) {
     PagedAppendArgs a{};
     int32_t st = batch_check(cfg, cache, batch, layer, workspace, workspace_bytes, &a.b);
     if (st != PICOATTN_OK) return st;
-    if (!dtype_ok(in_dtype) || !k || !v || !rope_cos || !rope_sin || (q == nullptr) != (q_out == nullptr))
+    if (!r || !dtype_ok(r->in_dtype) || !r->k || !r->v || !r->rope_cos || !r->rope_sin ||
+        (r->q == nullptr) != (r->q_out == nullptr) || (r->q_norm_w == nullptr) != (r->k_norm_w == nullptr))
         return PICOATTN_EINVAL;
-    if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return PICOATTN_EINVAL;
-    if (!aligned(rope_cos, 4) || !aligned(rope_sin, 4) || !aligned(q_norm_w, 4) || !aligned(k_norm_w, 4))
+    if (!aligned(r->rope_cos, 4) || !aligned(r->rope_sin, 4) || !aligned(r->q_norm_w, 4) || !aligned(r->k_norm_w, 4))
         return PICOATTN_EINVAL;
-    if (rot_dim <= 0 || rot_dim % 2 || rot_dim > cfg->head_dim) return PICOATTN_EINVAL;
-    if (rot_dim % 16) return PICOATTN_EUNSUPPORTED;
-    const size_t es = elem_size(in_dtype);
+    if (r->rot_dim <= 0 || r->rot_dim % 2 || r->rot_dim > cfg->head_dim) return PICOATTN_EINVAL;
+    if (r->rot_dim % 16) return PICOATTN_EUNSUPPORTED;
+    const size_t es = elem_size(r->in_dtype);
     const int64_t qw = (int64_t)cfg->n_heads * cfg->head_dim, kw = (int64_t)cfg->n_kv_heads * cfg->head_dim;
     const int64_t n = batch->n_tok, per16 = 16 / (int64_t)es;
     auto rows_ok = [&](const void* p, int64_t stride) {
         return aligned(p, 16) && stride >= 0 && stride <= kMaxStride && stride % per16 == 0;
     };
-    if ((q && !rows_ok(q, q_stride)) || !rows_ok(k, k_stride) || !rows_ok(v, v_stride)) return PICOATTN_EINVAL;
-    if (q_out) {
-        if (!aligned(q_out, 16)) return PICOATTN_EINVAL;
-        const Extent o = extent(q_out, n, qw, qw, 2);
-        if (overlap(o, extent(q, n, q_stride, qw, es)) || overlap(o, extent(k, n, k_stride, kw, es)) ||
-            overlap(o, extent(v, n, v_stride, kw, es)))
+    if ((r->q && !rows_ok(r->q, r->q_stride)) || !rows_ok(r->k, r->k_stride) || !rows_ok(r->v, r->v_stride))
+        return PICOATTN_EINVAL;
+    if (r->q_out) {
+        if (!aligned(r->q_out, 16)) return PICOATTN_EINVAL;
+        const Extent o = extent(r->q_out, n, qw, qw, 2);
+        if (overlap(o, extent(r->q, n, r->q_stride, qw, es)) || overlap(o, extent(r->k, n, r->k_stride, kw, es)) ||
+            overlap(o, extent(r->v, n, r->v_stride, kw, es)))
             return PICOATTN_EINVAL;
     }
     st = picoattn_device_check();
     if (st != PICOATTN_OK) return st;
     const size_t slab = layer * layer_elems(cfg, cache);
-    a.hq = cfg->n_heads, a.hkv = cfg->n_kv_heads, a.hd = cfg->head_dim, a.rot = rot_dim, a.mode = cfg->rope_mode;
-    a.in_dtype = in_dtype, a.cache_dtype = cache->dtype, a.eps = cfg->qk_norm_eps;
-    a.q = q, a.k = k, a.v = v, a.qs = q_stride, a.ks = k_stride, a.vs = v_stride;
-    a.qn_w = q_norm_w, a.kn_w = k_norm_w, a.cos_t = rope_cos, a.sin_t = rope_sin, a.q_out = q_out;
+    a.hq = cfg->n_heads, a.hkv = cfg->n_kv_heads, a.hd = cfg->head_dim, a.rot = r->rot_dim, a.mode = cfg->rope_mode;
+    a.in_dtype = r->in_dtype, a.cache_dtype = cache->dtype, a.eps = cfg->qk_norm_eps;
+    a.q = r->q, a.k = r->k, a.v = r->v, a.qs = r->q_stride, a.ks = r->k_stride, a.vs = r->v_stride;
+    a.qn_w = r->q_norm_w, a.kn_w = r->k_norm_w, a.cos_t = r->rope_cos, a.sin_t = r->rope_sin, a.q_out = r->q_out;
     a.k_pool = static_cast<uint16_t*>(cache->k) + slab, a.v_pool = static_cast<uint16_t*>(cache->v) + slab;
     return cuda_status(launch_paged_append(a, (cudaStream_t)stream));
 }

@@ -5,6 +5,7 @@
 // (fp32, when the weights are given), rotation of the first rot_dim elements at
 // the token's position kv_len - n_new + i, rounding to the cache's type.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_common.cuh"
 
@@ -25,21 +26,6 @@ __device__ __forceinline__ int seq_of(const PagedBatch& a, int t, int lane) {
     return b;
 }
 
-// The lane's two pieces of one head, widened to fp32.
-template <class TI>
-__device__ __forceinline__ void load_pieces(float (&x)[16], const TI* head, const PieceAt& at) {
-    if constexpr (sizeof(TI) == 4) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            Elem<float>::unpack(*reinterpret_cast<const uint4*>(head + at.a + 4 * i), x + 4 * i);
-            Elem<float>::unpack(*reinterpret_cast<const uint4*>(head + at.b + 4 * i), x + 8 + 4 * i);
-        }
-    } else {
-        Elem<TI>::unpack(*reinterpret_cast<const uint4*>(head + at.a), x);
-        Elem<TI>::unpack(*reinterpret_cast<const uint4*>(head + at.b), x + 8);
-    }
-}
-
 template <class TC, bool CACHE>
 __device__ __forceinline__ void store_pieces(const float (&x)[16], TC* head, const PieceAt& at) {
     uint32_t w[8];
@@ -51,93 +37,144 @@ __device__ __forceinline__ void store_pieces(const float (&x)[16], TC* head, con
 }
 
 // A warp step = up to HPS heads of one kind (q, k or v) of one token, hd/16
-// lanes a head.
+// lanes a head; a unit = up to kSteps steps of one kind of one token.  Bound by
+// instruction issue as much as by memory (about 130 instructions per step of
+// 512 elements): the loads of a unit are issued first, its token's sequence,
+// position, page and table entries are found while they travel, and units are
+// numbered kind by kind, so that the warps of an SM run the same code.
+constexpr int kSteps = 2;
+
+struct AppendSplit {
+    int q_per, kv_per;            // units per token: q; k (and as many v)
+    unsigned q_units, kv_units;   // all q units, all k (or v) units
+};
+
 template <class TI, class TC, int HD>
-__global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(PagedAppendArgs a) {
-    constexpr int LPH = HD / 16, HPS = 32 / LPH;
+__global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(PagedAppendArgs a, AppendSplit sp) {
+    constexpr int LPH = HD / 16, HPS = 32 / LPH, W = sizeof(TI) == 4 ? 4 : 2, E = 16 / sizeof(TI);
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int p = lane % LPH;
     const bool neox = a.mode == PICOATTN_ROPE_NEOX;
-    const int qsteps = a.q ? (a.hq + HPS - 1) / HPS : 0, ksteps = (a.hkv + HPS - 1) / HPS;
-    const int per_tok = qsteps + 2 * ksteps;
-    const long long steps = (long long)a.b.n_tok * per_tok;
-    for (long long u = (long long)blockIdx.x * kAppendWarps + warp; u < steps; u += (long long)gridDim.x * kAppendWarps) {
-        const int tok = (int)(u / per_tok);
-        int st = (int)(u - (long long)tok * per_tok);
-        const int kind = st < qsteps ? 0 : (st < qsteps + ksteps ? 1 : 2);
-        st -= kind == 0 ? 0 : (kind == 1 ? qsteps : qsteps + ksteps);
-        const int heads = kind == 0 ? a.hq : a.hkv;
-        const int h = st * HPS + lane / LPH;
-        const bool live = h < heads;
-        const int b = seq_of(a.b, tok, lane);
-        if (b >= a.b.n_seqs) continue;            // a row behind the last sequence
-        const SeqSpan sp = seq_span(a.b, b);
-        if (tok < sp.t0) continue;                // a row before the first sequence
-        const PieceAt at = piece_at<8>(p, a.rot, neox);
-        TC* q_out = static_cast<TC*>(a.q_out) + ((long long)tok * a.hq + h) * HD;
-        if (!sp.ok) {
-            if (lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
-            float nan[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) nan[j] = __int_as_float(0x7fc00000);
-            if (kind == 0 && live) store_pieces<TC, false>(nan, q_out, at);
-            continue;
-        }
-        const int pos = sp.len - sp.n + (tok - sp.t0);
+    const PieceAt at = piece_at<8>(lane % LPH, a.rot, neox);
+    const bool vec = (((uintptr_t)a.cos_t | (uintptr_t)a.sin_t | (uintptr_t)a.qn_w | (uintptr_t)a.kn_w) & 15) == 0;
+    const unsigned units = sp.q_units + 2 * sp.kv_units;
+    for (unsigned u = blockIdx.x * kAppendWarps + warp; u < units; u += gridDim.x * kAppendWarps) {
+        const int kind = u < sp.q_units ? 0 : (u < sp.q_units + sp.kv_units ? 1 : 2);
+        const unsigned i0 = u - (kind == 0 ? 0 : (kind == 1 ? sp.q_units : sp.q_units + sp.kv_units));
+        const unsigned per = kind == 0 ? sp.q_per : sp.kv_per, tok = i0 / per;
+        const int h0 = (int)(i0 - tok * per) * (kSteps * HPS) + lane / LPH, heads = kind == 0 ? a.hq : a.hkv;
         const TI* src = static_cast<const TI*>(kind == 0 ? a.q : (kind == 1 ? a.k : a.v)) +
-                        tok * (kind == 0 ? a.qs : (kind == 1 ? a.ks : a.vs)) + (long long)(live ? h : 0) * HD;
-        float x[16];
-        load_pieces(x, src, at);
-        if (kind != 2) {
-            if (a.qn_w) {
-                const float* w = kind == 0 ? a.qn_w : a.kn_w;
-                float ss = 0.f;
+                        tok * (kind == 0 ? a.qs : (kind == 1 ? a.ks : a.vs)) + h0 * HD;
+        uint4 w[kSteps][W];
 #pragma unroll
-                for (int j = 0; j < 16; j++) ss += x[j] * x[j];
+        for (int i = 0; i < kSteps; i++)
 #pragma unroll
-                for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(ss / (float)HD, a.eps)));
+            for (int j = 0; j < W; j++)
+                w[i][j] = h0 + i * HPS < heads
+                              ? *reinterpret_cast<const uint4*>(src + i * HPS * HD + (j < W / 2 ? at.a + E * j
+                                                                                               : at.b + E * (j - W / 2)))
+                              : make_uint4(0, 0, 0, 0);
+        const int b = seq_of(a.b, (int)tok, lane);
+        if (b >= a.b.n_seqs) continue;       // a row behind the last sequence
+        const SeqSpan span = seq_span(a.b, b);
+        if ((int)tok < span.t0) continue;    // a row before the first sequence
+        if (!span.ok && lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+        const int pos = span.ok ? span.len - span.n + ((int)tok - span.t0) : 0;
+        TC* dst = static_cast<TC*>(a.q_out) + ((long long)tok * a.hq + h0) * HD;
+        int hop = HPS * HD;
+        if (kind != 0) {
+            if (!span.ok) continue;
+            const int page = a.b.page_table[(size_t)b * a.b.page_cols + (pos >> a.b.page_shift)];
+            if (page < 0 || page >= a.b.n_pages) {
+                if (lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_PAGE);
+                continue;
+            }
+            dst = static_cast<TC*>(kind == 1 ? a.k_pool : a.v_pool) +
+                  (((size_t)page * a.hkv + h0) * a.b.page_size + (pos & (a.b.page_size - 1))) * HD;
+            hop *= a.b.page_size;
+        }
+        if (kind == 2) {  // v: the cache's rounding alone
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    x[j] = __fmul_rn(__fmul_rn(x[j], scale), w[at.a + j]);
-                    x[8 + j] = __fmul_rn(__fmul_rn(x[8 + j], scale), w[at.b + j]);
+            for (int i = 0; i < kSteps; i++) {
+                if (h0 + i * HPS >= heads) break;
+                if constexpr (std::is_same<TI, TC>::value) {  // the bits themselves
+                    *reinterpret_cast<uint4*>(dst + (size_t)i * hop + at.a) = w[i][0];
+                    *reinterpret_cast<uint4*>(dst + (size_t)i * hop + at.b) = w[i][1];
+                } else {
+                    float x[16];
+#pragma unroll
+                    for (int j = 0; j < W; j++) Elem<TI>::unpack(w[i][j], x + E * j);
+                    store_pieces<TC, true>(x, dst + (size_t)i * hop, at);
                 }
             }
-            if (at.rotated) {
-                const float* cr = a.cos_t + (size_t)pos * (a.rot / 2) + at.pair;
-                const float* sr = a.sin_t + (size_t)pos * (a.rot / 2) + at.pair;
-                float c[8], s[8];
+            continue;
+        }
+        float c[8], s[8], g[16];
+        if (at.rotated) {
+            load_f32<8>(c, a.cos_t + (size_t)pos * (a.rot / 2) + at.pair, vec);
+            load_f32<8>(s, a.sin_t + (size_t)pos * (a.rot / 2) + at.pair, vec);
+        }
+        if (a.qn_w) {
+            const float* nw = kind == 0 ? a.qn_w : a.kn_w;
+            load_f32<8>(g, nw + at.a, vec);
+            load_f32<8>(g + 8, nw + at.b, vec);
+        }
 #pragma unroll
-                for (int j = 0; j < 8; j++) c[j] = cr[j], s[j] = sr[j];
+        for (int i = 0; i < kSteps; i++) {
+            float x[16];
+#pragma unroll
+            for (int j = 0; j < W; j++) Elem<TI>::unpack(w[i][j], x + E * j);
+            if (a.qn_w) {
+                uint64_t s2 = 0;
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) s2 = f2_fma(f2_pack(x[j], x[j + 1]), f2_pack(x[j], x[j + 1]), s2);
+                float lo, hi;
+                f2_unpack(s2, lo, hi);
+                float ss = lo + hi;
+#pragma unroll
+                for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
+#pragma unroll
+                for (int j = 0; j < 16; j += 2)
+                    f2_unpack(f2_mul(f2_mul(f2_pack(x[j], x[j + 1]), f2_pack(r, r)), f2_pack(g[j], g[j + 1])), x[j],
+                              x[j + 1]);
+                // the sums above follow another order than the reference's, so the
+                // rotation need not round as it does either
+                if (at.rotated) rotate_pieces_fused<8>(x, c, s, neox);
+            } else if (at.rotated) {
                 rotate_pieces<8>(x, c, s, neox);
             }
+            if (h0 + i * HPS >= heads) continue;
+            if (kind == 1) {
+                store_pieces<TC, true>(x, dst + (size_t)i * hop, at);
+            } else {
+                if (!span.ok) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) x[j] = __int_as_float(0x7fc00000);
+                }
+                store_pieces<TC, false>(x, dst + (size_t)i * hop, at);
+            }
         }
-        if (kind == 0) {
-            if (live) store_pieces<TC, false>(x, q_out, at);
-            continue;
-        }
-        const int page = a.b.page_table[(size_t)b * a.b.page_cols + (pos >> a.b.page_shift)];
-        if (page < 0 || page >= a.b.n_pages) {
-            if (lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_PAGE);
-            continue;
-        }
-        TC* pool = static_cast<TC*>(kind == 1 ? a.k_pool : a.v_pool);
-        const size_t row = ((size_t)page * a.hkv + h) * a.b.page_size + (pos & (a.b.page_size - 1));
-        if (live) store_pieces<TC, true>(x, pool + row * HD, at);
     }
+}
+
+template <class TI, class TC, int HD>
+cudaError_t launch_hd(const PagedAppendArgs& a, cudaStream_t stream) {
+    constexpr int HPU = kSteps * 32 / (HD / 16);  // heads per unit
+    AppendSplit sp{};
+    sp.q_per = a.q ? (a.hq + HPU - 1) / HPU : 0;
+    sp.kv_per = (a.hkv + HPU - 1) / HPU;
+    const long long units = (long long)a.b.n_tok * (sp.q_per + 2 * sp.kv_per);
+    sp.q_units = (unsigned)a.b.n_tok * sp.q_per;
+    sp.kv_units = (unsigned)a.b.n_tok * sp.kv_per;
+    const unsigned grid = (unsigned)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, 32LL * device_sm_count());
+    return launch_pdl(paged_append_kernel<TI, TC, HD>, dim3(grid), dim3(kAppendWarps * 32), 0, stream, a, sp);
 }
 
 template <class TI, class TC>
 cudaError_t launch_types(const PagedAppendArgs& a, cudaStream_t stream) {
-    const int hps = 32 / (a.hd / 16);
-    const long long steps =
-        (long long)a.b.n_tok * ((a.q ? (a.hq + hps - 1) / hps : 0) + 2 * ((a.hkv + hps - 1) / hps));
-    const unsigned grid =
-        (unsigned)std::min<long long>((steps + kAppendWarps - 1) / kAppendWarps, 8LL * device_sm_count());
-    return launch_pdl(a.hd == 64 ? paged_append_kernel<TI, TC, 64> : paged_append_kernel<TI, TC, 128>, dim3(grid),
-                      dim3(kAppendWarps * 32), 0, stream, a);
+    return a.hd == 64 ? launch_hd<TI, TC, 64>(a, stream) : launch_hd<TI, TC, 128>(a, stream);
 }
 
 template <class TC>

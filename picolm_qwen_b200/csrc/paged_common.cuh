@@ -83,6 +83,22 @@ __device__ __forceinline__ void rotate_pair(float& x0, float& x1, float c, float
     x1 = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
 }
 
+// N consecutive fp32 of a table or weight row, which need only 4-byte alignment:
+// in 16-byte loads where `vec` says that its rows start on 16 bytes.
+template <int N>
+__device__ __forceinline__ void load_f32(float* x, const float* p, bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p + j);
+            x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = p[j];
+    }
+}
+
 // Where a lane's two 16-byte pieces (V elements each) of a head lie, so that
 // both members of every pair it rotates are its own.  Lane p of the hd/(2V) a
 // head takes: rotated part first (NeoX: pieces p of both halves; interleaved:
@@ -102,13 +118,38 @@ __device__ __forceinline__ PieceAt piece_at(int p, int rot, bool neox) {
     return r;
 }
 
-// Rotates the lane's 2V elements x with its V table entries.
+// Rotates the lane's 2V elements x with its V table entries, each product and
+// sum rounded (rotate_pair).
 template <int V>
 __device__ __forceinline__ void rotate_pieces(float* x, const float* c, const float* s, bool neox) {
 #pragma unroll
     for (int j = 0; j < V; j++) {
         if (neox) rotate_pair(x[j], x[V + j], c[j], s[j]);
         else rotate_pair(x[2 * j], x[2 * j + 1], c[j], s[j]);
+    }
+}
+
+// The same with one product of each output fused into the sum (one rounding
+// less), in packed pairs of fp32 where the layout gives them (the same bits): a
+// third of the instructions.
+__device__ __forceinline__ void rotate_pair_fused(float& x0, float& x1, float c, float s) {
+    const float a = x0, b = x1;
+    x0 = __fmaf_rn(a, c, -__fmul_rn(b, s));
+    x1 = __fmaf_rn(a, s, __fmul_rn(b, c));
+}
+template <int V>
+__device__ __forceinline__ void rotate_pieces_fused(float* x, const float* c, const float* s, bool neox) {
+    if (neox) {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+            const uint64_t c2 = f2_pack(c[j], c[j + 1]), s2 = f2_pack(s[j], s[j + 1]), n2 = f2_pack(-s[j], -s[j + 1]);
+            const uint64_t x0 = f2_pack(x[j], x[j + 1]), x1 = f2_pack(x[V + j], x[V + j + 1]);
+            f2_unpack(f2_fma(x0, c2, f2_mul(x1, n2)), x[j], x[j + 1]);
+            f2_unpack(f2_fma(x0, s2, f2_mul(x1, c2)), x[V + j], x[V + j + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) rotate_pair_fused(x[2 * j], x[2 * j + 1], c[j], s[j]);
     }
 }
 

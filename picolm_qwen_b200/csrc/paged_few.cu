@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
 // once: the merge is one round trip to L2.  Rows of a sequence outside the
 // host's bounds become NaN here.
 constexpr int kMergeThreads = 128;
-constexpr int kMaxParts = 2 * 256;  // CTAs of the attention kernel
+constexpr int kMaxParts = 512;  // most CTAs of the attention kernel; sizes the workspace
 
 template <class T, int HD>
 __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs fa, int grid) {
@@ -474,8 +474,6 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     }
 }
 
-int max_grid() { return std::min(2 * device_sm_count(), kMaxParts); }
-
 template <class T, int HD>
 cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     using F = Few<HD>;
@@ -485,12 +483,12 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     });
     if (e != cudaSuccess) return e;
     const long long units = (long long)a.b.n_seqs * a.hkv * ((a.b.max_len + kUnit - 1) / kUnit);
-    const int grid = (int)std::min<long long>(max_grid(), (units + kMinUnits - 1) / kMinUnits);
+    const int grid = (int)std::min<long long>(std::min(2 * device_sm_count(), kMaxParts), (units + kMinUnits - 1) / kMinUnits);
     FewArgs fa{};
     fa.a = a;
     fa.part_ml = reinterpret_cast<float2*>(a.ws);
-    fa.part_o = reinterpret_cast<float*>(a.ws + (size_t)2 * max_grid() * kRows * 8);
-    fa.prefix = reinterpret_cast<long long*>(a.ws + (size_t)2 * max_grid() * kRows * (8 + 4 * HD));
+    fa.part_o = reinterpret_cast<float*>(a.ws + (size_t)2 * kMaxParts * kRows * 8);
+    fa.prefix = reinterpret_cast<long long*>(a.ws + (size_t)2 * kMaxParts * kRows * (8 + 4 * HD));
     e = launch_pdl(paged_few_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)F::bytes, stream, fa);
     if (e != cudaSuccess) return e;
     return launch_pdl(paged_few_merge_kernel<T, HD>, dim3(a.b.max_new * a.g, a.b.n_seqs * a.hkv), dim3(kMergeThreads), 0,
@@ -504,7 +502,7 @@ bool paged_few_fits(const PagedAttnArgs& a) {
 }
 
 size_t paged_few_bytes(int hd, int n_seqs) {
-    return align_up((size_t)2 * max_grid() * kRows * (8 + 4 * hd) + (size_t)(n_seqs + 1) * 8, 256);
+    return align_up((size_t)2 * kMaxParts * kRows * (8 + 4 * hd) + (size_t)(n_seqs + 1) * 8, 256);
 }
 
 cudaError_t launch_paged_few(const PagedAttnArgs& a, cudaStream_t stream) {

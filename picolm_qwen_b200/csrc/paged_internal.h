@@ -38,7 +38,6 @@ struct RopeRows {
 struct RopeArgs {
     RopeRows t[2];  // q, k (heads 0: none)
     int dtype, mode, hd, rot, inverse, n_tok, table_rows;
-    int vec;        // every row starts on 16 bytes
     const int* pos;
     const float* cos_t;
     const float* sin_t;

@@ -12,8 +12,8 @@ namespace picoattn {
 
 namespace {
 
-// One warp rotates the pairs (and copies the rest) of one head of one token,
-// an element pair per lane: any head_dim, rot_dim and alignment.
+// Any head_dim, rot_dim and alignment: one warp rotates the pairs (and copies
+// the rest) of one head of one token, an element pair per lane.
 template <class T>
 __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
     pdl_trigger();
@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
         for (int i = lane; i < half; i += 32) {
             const int e0 = a.mode == PICOATTN_ROPE_NEOX ? i : 2 * i, e1 = a.mode == PICOATTN_ROPE_NEOX ? i + half : 2 * i + 1;
             float x0 = Elem<T>::load(x + e0), x1 = Elem<T>::load(x + e1);
-            rotate_pair(x0, x1, cr[i], a.inverse ? -sr[i] : sr[i]);
+            rotate_pair_fused(x0, x1, cr[i], a.inverse ? -sr[i] : sr[i]);
             y[e0] = Elem<T>::round(x0);
             y[e1] = Elem<T>::round(x1);
         }
@@ -50,16 +50,120 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
     }
 }
 
+// The same with 16-byte accesses: a lane holds two pieces of V elements of a
+// head (both members of its pairs, piece_at), LPH = hd / 2V lanes a head, so a
+// warp step takes 32 / LPH heads of one token.  Memory-bound (one read and one
+// write of every element): a unit is up to kSteps steps of one tensor of one
+// token, whose loads are all issued before the first rotation and which share
+// the lane's table entries.
+constexpr int kSteps = 4;
+
+struct RopeSplit {
+    int lph_shift, per_unit, q_units, units_per_tok;  // per_unit: steps of a unit
+    unsigned units;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) rope_vec_kernel(RopeArgs a, RopeSplit sp) {
+    constexpr int V = Elem<T>::V;
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int hps = 32 >> sp.lph_shift;
+    const bool neox = a.mode == PICOATTN_ROPE_NEOX;
+    const PieceAt at = piece_at<V>(lane & ((1 << sp.lph_shift) - 1), a.rot, neox);
+    const bool vec = (((uintptr_t)a.cos_t | (uintptr_t)a.sin_t) & 15) == 0 && a.rot % 8 == 0;  // whole rows
+    for (unsigned u = blockIdx.x * 8 + (threadIdx.x >> 5); u < sp.units; u += gridDim.x * 8) {
+        const unsigned tok = u / (unsigned)sp.units_per_tok;
+        int part = (int)(u - tok * (unsigned)sp.units_per_tok);
+        const bool second = part >= sp.q_units;
+        if (second) part -= sp.q_units;
+        const RopeRows& r = a.t[second ? 1 : 0];
+        const int pos = a.pos[tok];
+        const int h0 = part * sp.per_unit * hps + (lane >> sp.lph_shift);
+        const T* src = static_cast<const T*>(r.x) + tok * r.x_stride + (long long)h0 * a.hd;
+        T* dst = static_cast<T*>(r.out) + tok * r.out_stride + (long long)h0 * a.hd;
+        const bool ok = pos >= 0 && pos < a.table_rows;
+        if (!ok && lane == 0) atomicOr(a.status, PICOATTN_DEV_BAD_POS);
+        // an element that stays need not move when the rotation is in place
+        const bool still = ok && !at.rotated && src == dst;
+        const int n = still ? 0 : min(sp.per_unit, (r.heads - h0 + hps - 1) / hps);
+        const int hop = hps * a.hd;
+        uint4 w[kSteps][2];
+#pragma unroll
+        for (int i = 0; i < kSteps; i++)
+            if (i < n) {
+                w[i][0] = *reinterpret_cast<const uint4*>(src + i * hop + at.a);
+                w[i][1] = *reinterpret_cast<const uint4*>(src + i * hop + at.b);
+            }
+        float c[V], s[V];
+        if (ok && at.rotated) {
+            load_f32<V>(c, a.cos_t + (size_t)pos * (a.rot / 2) + at.pair, vec);
+            load_f32<V>(s, a.sin_t + (size_t)pos * (a.rot / 2) + at.pair, vec);
+            if (a.inverse) {
+#pragma unroll
+                for (int j = 0; j < V; j++) s[j] = -s[j];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) {
+            if (i >= n) break;
+            if (at.rotated || !ok) {
+                float x[2 * V];
+                Elem<T>::unpack(w[i][0], x);
+                Elem<T>::unpack(w[i][1], x + V);
+                if (ok) {
+                    rotate_pieces_fused<V>(x, c, s, neox);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2 * V; j++) x[j] = __int_as_float(0x7fc00000);
+                }
+                w[i][0] = Elem<T>::pack(x);
+                w[i][1] = Elem<T>::pack(x + V);
+            }
+            *reinterpret_cast<uint4*>(dst + i * hop + at.a) = w[i][0];
+            *reinterpret_cast<uint4*>(dst + i * hop + at.b) = w[i][1];
+        }
+    }
+}
+
+template <class T>
+cudaError_t launch_type(const RopeArgs& a, cudaStream_t stream) {
+    constexpr int V = Elem<T>::V;
+    const int sms = device_sm_count();
+    const int lph = a.hd / (2 * V);
+    bool vec = a.hd % (2 * V) == 0 && lph <= 32 && (lph & (lph - 1)) == 0 && a.rot % (2 * V) == 0;
+    for (const RopeRows& r : a.t)
+        if (r.heads && ((((uintptr_t)r.x | (uintptr_t)r.out) & 15) || r.x_stride % V || r.out_stride % V)) vec = false;
+    RopeSplit sp{};
+    if (vec) {
+        while ((1 << sp.lph_shift) < lph) sp.lph_shift++;
+        const int hps = 32 / lph, qs = (a.t[0].heads + hps - 1) / hps, ks = (a.t[1].heads + hps - 1) / hps;
+        // Several steps a unit once that still gives every SM its warps; below, a
+        // step a unit: the call is as short as one round of loads
+        for (sp.per_unit = kSteps; sp.per_unit > 1; sp.per_unit /= 2)
+            if ((long long)a.n_tok * ((qs + ks) / sp.per_unit) >= 32LL * sms) break;
+        sp.q_units = (qs + sp.per_unit - 1) / sp.per_unit;
+        sp.units_per_tok = sp.q_units + (ks + sp.per_unit - 1) / sp.per_unit;
+        const long long units = (long long)a.n_tok * sp.units_per_tok;
+        if (units < (1LL << 31)) {  // the kernel counts in 32 bits
+            sp.units = (unsigned)units;
+            const unsigned grid = (unsigned)std::min<long long>((units + 7) / 8, 32LL * sms);
+            return launch_pdl(rope_vec_kernel<T>, dim3(grid), dim3(256), 0, stream, a, sp);
+        }
+    }
+    const long long units = (long long)a.n_tok * (a.t[0].heads + a.t[1].heads);
+    const unsigned grid = (unsigned)std::min<long long>((units + 7) / 8, 8LL * sms);
+    return launch_pdl(rope_kernel<T>, dim3(grid), dim3(256), 0, stream, a);
+}
+
 }  // namespace
 
 cudaError_t launch_rope(const RopeArgs& a, cudaStream_t stream) {
-    const long long units = (long long)a.n_tok * (a.t[0].heads + a.t[1].heads);
-    const unsigned grid = (unsigned)std::min<long long>((units + 7) / 8, 8LL * device_sm_count());
-    auto go = [&](auto kernel) { return launch_pdl(kernel, dim3(grid), dim3(256), 0, stream, a); };
     switch (a.dtype) {
-        case PICOATTN_DTYPE_F32: return go(rope_kernel<float>);
-        case PICOATTN_DTYPE_F16: return go(rope_kernel<__half>);
-        default: return go(rope_kernel<__nv_bfloat16>);
+        case PICOATTN_DTYPE_F32: return launch_type<float>(a, stream);
+        case PICOATTN_DTYPE_F16: return launch_type<__half>(a, stream);
+        default: return launch_type<__nv_bfloat16>(a, stream);
     }
 }
 

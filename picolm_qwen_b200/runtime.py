@@ -104,6 +104,10 @@ def logits(x: torch.Tensor, output_norm_w: torch.Tensor, w_out: torch.Tensor, w_
 
 _DTYPES = {torch.float32: abi.DTYPE_F32, torch.float16: abi.DTYPE_F16, torch.bfloat16: abi.DTYPE_BF16}
 
+# the current stream's handle without building a Stream object, where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def _dtype(t: torch.Tensor) -> int:
     d = _DTYPES.get(t.dtype)
@@ -112,36 +116,46 @@ def _dtype(t: torch.Tensor) -> int:
     return d
 
 
-def _heads(t: torch.Tensor, n: int, hd: int, what: str) -> int:
+def _heads(t: torch.Tensor, n: int, heads: int, hd: int, what: str) -> int:
     """The row stride of t, [n, heads, hd] or [n, heads*hd], each row's heads contiguous."""
-    st = t.stride()
-    if t.dim() == 3:
-        if t.shape[0] != n or t.shape[2] != hd or st[2] != 1 or (st[1] != hd and t.shape[1] != 1):
-            raise ValueError(f"{what}: [{n}, heads, {hd}] with contiguous heads, got {tuple(t.shape)} strides {st}")
-    elif t.dim() != 2 or t.shape[0] != n or t.shape[1] % hd or st[1] != 1:
-        raise ValueError(f"{what}: [{n}, heads, {hd}] or [{n}, heads*{hd}], got {tuple(t.shape)} strides {st}")
-    return st[0]
+    shape, st = t.shape, t.stride()
+    if len(shape) == 3:
+        if shape == (n, heads, hd) and st[2] == 1 and (st[1] == hd or heads == 1):
+            return st[0]
+    elif shape == (n, heads * hd) and st[1] == 1:
+        return st[0]
+    raise ValueError(f"{what}: [{n}, {heads}, {hd}] or [{n}, {heads * hd}] with contiguous rows, got {tuple(shape)} "
+                     f"strides {st}")
 
 
-def _same_device(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _check_table(cos: torch.Tensor, sin: torch.Tensor, rows: int) -> int:
+    """rot_dim of a pair of tables."""
+    shape = cos.shape
+    if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and len(shape) == 2 and sin.shape == shape and
+            shape[0] >= rows and cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError(f"rope tables: contiguous fp32 [>= {rows}, rot_dim/2], got {tuple(shape)} {cos.dtype}, "
+                         f"{tuple(sin.shape)} {sin.dtype}")
+    return 2 * shape[1]
 
 
-def _launch_stream(device: torch.device, stream) -> int:
-    """The stream to launch on; the call is made with its tensors' device current."""
-    if stream is not None:
-        return stream.cuda_stream
-    return torch.cuda.current_stream(device).cuda_stream
+def _same_device(index: int, what: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: a tensor on {t.device}, the others on device {index}")
 
 
-def _on_device(device: torch.device, call, *args) -> int:
-    """call(*args) with `device` current, whichever device the caller has current."""
-    if torch.cuda.current_device() == device.index:
-        return call(*args)
-    with torch.cuda.device(device):
-        return call(*args)
+def _launch(index: int, stream, what: str, call, *args) -> None:
+    """call(*args, stream) with device `index` current (whichever the caller has), its error raised."""
+    if index < 0:
+        raise ValueError(f"{what}: tensors on the CPU")
+    handle = _raw_stream(index) if stream is None else stream.cuda_stream
+    if torch.cuda.current_device() == index:
+        st = call(*args, handle)
+    else:
+        with torch.cuda.device(index):
+            st = call(*args, handle)
+    if st:
+        abi.check(st, what)
 
 
 def status_workspace(device: str | torch.device = "cuda") -> torch.Tensor:
@@ -152,8 +166,8 @@ def status_workspace(device: str | torch.device = "cuda") -> torch.Tensor:
 def workspace_status(ws: torch.Tensor) -> int:
     """The sticky device status bits (abi.DEV_*) of a workspace; synchronises and clears them."""
     v = C.c_uint32(0)
-    abi.check(_on_device(ws.device, abi.lib().picoattn_workspace_status, ws.data_ptr(),
-                         _launch_stream(ws.device, None), C.byref(v)), "workspace_status")
+    _launch(ws.get_device(), None, "workspace_status",
+            lambda handle: abi.lib().picoattn_workspace_status(ws.data_ptr(), handle, C.byref(v)))
     return v.value
 
 
@@ -177,34 +191,26 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, rope_cos: t
     (the first 2 * rope_cos.shape[1] elements of each head); the outputs may be
     the inputs.  inverse: the opposite rotation, which is the backward pass."""
     n, heads, hd = q.shape
-    dev = q.device
-    half = rope_cos.shape[1]
-    if pos.dtype != torch.int32 or pos.shape != (n,) or pos.stride(0) != 1 and n > 1:
-        raise ValueError(f"pos: [{n}] int32")
-    _check_table(rope_cos, rope_sin, half)
-    if q_out.dtype != q.dtype or q_out.shape != q.shape or (k is None) != (k_out is None):
-        raise ValueError("q_out: like q; k and k_out both or neither")
-    _same_device(dev, k=k, pos=pos, rope_cos=rope_cos, rope_sin=rope_sin, q_out=q_out, k_out=k_out,
-                 workspace=workspace)
-    rows = abi.RopeRows(q.data_ptr(), _heads(q, n, hd, "q"), q_out.data_ptr(), _heads(q_out, n, hd, "q_out"), heads)
-    krows = None
-    if k is not None:
-        if k.dtype != q.dtype or k_out.dtype != q.dtype or k_out.shape != k.shape:
-            raise ValueError("k, k_out: of q's type and one shape")
-        krows = C.byref(abi.RopeRows(k.data_ptr(), _heads(k, n, hd, "k"), k_out.data_ptr(),
-                                     _heads(k_out, n, hd, "k_out"), k.shape[1]))
-    st = _on_device(dev, abi.lib().picoattn_rope, _dtype(q), rope_mode, hd, 2 * half, 1 if inverse else 0, n,
-                    pos.data_ptr(), rope_cos.shape[0], rope_cos.data_ptr(), rope_sin.data_ptr(), C.byref(rows), krows,
-                    workspace.data_ptr(), workspace.numel(), _launch_stream(dev, stream))
-    if st:
-        abi.check(st, "picoattn_rope")
-
-
-def _check_table(cos: torch.Tensor, sin: torch.Tensor, half: int, rows: int = 1) -> None:
-    for t in (cos, sin):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[0] < rows or \
-                not t.is_contiguous():
-            raise ValueError(f"rope tables: contiguous fp32 [>= {rows}, {half}], got {tuple(t.shape)} {t.dtype}")
+    dt, index = q.dtype, q.get_device()
+    rot = _check_table(rope_cos, rope_sin, 1)
+    if pos.dtype is not torch.int32 or pos.shape != (n,) or not pos.is_contiguous():
+        raise ValueError(f"pos: contiguous int32 [{n}], got {tuple(pos.shape)} {pos.dtype}")
+    if q_out.dtype is not dt or (k is None) != (k_out is None):
+        raise ValueError("q_out: of q's type; k and k_out both or neither")
+    _same_device(index, "rope", pos, rope_cos, rope_sin, q_out, k, k_out, workspace)
+    rows = (q.data_ptr(), _heads(q, n, heads, hd, "q"), q_out.data_ptr(), _heads(q_out, n, heads, hd, "q_out"), heads)
+    if k is None:
+        krows = (0, 0, 0, 0, 0)
+    else:
+        kh = k.shape[1]
+        if k.dtype is not dt or k_out.dtype is not dt:
+            raise ValueError("k, k_out: of q's type")
+        krows = (k.data_ptr(), _heads(k, n, kh, hd, "k"), k_out.data_ptr(), _heads(k_out, n, kh, hd, "k_out"), kh)
+    _launch(index, stream, "picoattn_rope", abi.lib().picoattn_rope,
+            abi.ROPE_ARGS.pack(_dtype(q), rope_mode, hd, rot, 1 if inverse else 0, n, rope_cos.shape[0],
+                               1 if k is None else 2, pos.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
+                               *rows, *krows),
+            workspace.data_ptr(), workspace.numel())
 
 
 class PagedBatch:
@@ -223,7 +229,7 @@ class PagedBatch:
                                ("kv_len", kv_len, (n,))):
             if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"{name}: contiguous int32 {shape}, got {tuple(t.shape)} {t.dtype}")
-        _same_device(cache.device, page_table=page_table, q_start=q_start, kv_len=kv_len)
+        _same_device(cache.index, "batch", page_table, q_start, kv_len)
         self.tensors = (page_table, q_start, kv_len)  # kept alive with the struct
         self.n_tok = n_tok
         self.desc = abi.PagedBatchDesc(n, n_tok, max_new, max_len, page_table.shape[1], page_table.data_ptr(),
@@ -232,7 +238,7 @@ class PagedBatch:
         if ws == 0:
             raise abi.PicoAttnError(abi.PICOATTN_EUNSUPPORTED, "paged_workspace_size")
         self.workspace = torch.zeros(ws, dtype=torch.uint8, device=cache.device)
-        self.ref, self.ws_ptr, self.ws_bytes = C.byref(self.desc), self.workspace.data_ptr(), ws
+        self.ref, self.ws_ptr, self.ws_bytes = C.addressof(self.desc), self.workspace.data_ptr(), ws
 
     def status(self) -> int:
         return workspace_status(self.workspace)
@@ -255,12 +261,14 @@ class PagedCache:
             if tuple(t.shape) != want or t.dtype != k_pool.dtype or not t.is_contiguous():
                 raise ValueError(f"{name}: contiguous {want}, got {tuple(t.shape)} {t.dtype}")
         self.cfg, self.k_pool, self.v_pool, self.device = cfg, k_pool, v_pool, k_pool.device
-        _same_device(self.device, v_pool=v_pool)
+        self.index = k_pool.get_device()
+        _same_device(self.index, "PagedCache", v_pool)
         self.dtype = k_pool.dtype
         self.desc = abi.PagedCacheDesc(k_pool.shape[1], page_size, _dtype(k_pool), k_pool.data_ptr(),
                                        v_pool.data_ptr())
-        self.cfg_ref, self.ref = C.byref(cfg), C.byref(self.desc)
-        abi.check(abi.lib().picoattn_paged_check(self.cfg_ref, self.ref), "picoattn_paged_check")
+        self.cfg_ref, self.ref = C.addressof(cfg), C.addressof(self.desc)
+        self.shape = (cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, cfg.max_seq_len)
+        abi.check(abi.lib().picoattn_paged_check(C.byref(cfg), C.byref(self.desc)), "picoattn_paged_check")
 
     def batch(self, page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, n_tok: int, max_new: int,
               max_len: int) -> PagedBatch:
@@ -273,45 +281,44 @@ class PagedCache:
         """k, v [n_tok, n_kv_heads, head_dim] into their pages, q [n_tok, n_heads,
         head_dim] rotated into q_out (of the cache's type); the first
         2 * rope_cos.shape[1] elements of each head rotate."""
-        n, hd, dev = batch.n_tok, self.cfg.head_dim, self.device
-        half = rope_cos.shape[1]
-        _check_table(rope_cos, rope_sin, half, self.cfg.max_seq_len)
-        for name, t, heads in (("q", q, self.cfg.n_heads), ("k", k, self.cfg.n_kv_heads),
-                               ("v", v, self.cfg.n_kv_heads)):
-            if t is not None and (t.dtype != k.dtype or t.numel() != n * heads * hd):
-                raise ValueError(f"{name}: [{n}, {heads}, {hd}] of one type, got {tuple(t.shape)} {t.dtype}")
-        if q_out is not None and (q_out.dtype != self.dtype or not q_out.is_contiguous() or
-                                  q_out.numel() != n * self.cfg.n_heads * hd):
-            raise ValueError(f"q_out: contiguous [{n}, {self.cfg.n_heads}, {hd}] {self.dtype}")
-        for w in (q_norm_w, k_norm_w):
-            if w is not None and (w.dtype != torch.float32 or w.numel() != hd or not w.is_contiguous()):
-                raise ValueError(f"norm weights: contiguous fp32 [{hd}]")
-        _same_device(dev, q=q, k=k, v=v, rope_cos=rope_cos, rope_sin=rope_sin, q_out=q_out, q_norm_w=q_norm_w,
-                     k_norm_w=k_norm_w)
-        st = _on_device(dev, abi.lib().picoattn_paged_append, self.cfg_ref, self.ref, layer, batch.ref, _dtype(k),
-                        abi.ptr(q), 0 if q is None else _heads(q, n, hd, "q"), k.data_ptr(), _heads(k, n, hd, "k"),
-                        v.data_ptr(), _heads(v, n, hd, "v"), abi.ptr(q_norm_w), abi.ptr(k_norm_w),
-                        rope_cos.data_ptr(), rope_sin.data_ptr(), 2 * half, abi.ptr(q_out), batch.ws_ptr,
-                        batch.ws_bytes, _launch_stream(dev, stream))
-        if st:
-            abi.check(st, "picoattn_paged_append")
+        n, dt = batch.n_tok, k.dtype
+        hq, hkv, hd, max_rows = self.shape
+        rot = _check_table(rope_cos, rope_sin, max_rows)
+        if v.dtype is not dt or (q is None) != (q_out is None):
+            raise ValueError("q, k, v of one type; q and q_out both or neither")
+        q_ptr = q_stride = out_ptr = 0
+        if q is not None:
+            if q.dtype is not dt or q_out.dtype is not self.dtype or not q_out.is_contiguous():
+                raise ValueError(f"q of k's type, q_out contiguous {self.dtype}, got {q.dtype}, {q_out.dtype}")
+            q_ptr, q_stride, out_ptr = q.data_ptr(), _heads(q, n, hq, hd, "q"), q_out.data_ptr()
+            _heads(q_out, n, hq, hd, "q_out")
+        qn = kn = 0
+        if q_norm_w is not None or k_norm_w is not None:
+            for w in (q_norm_w, k_norm_w):
+                if w is None or w.dtype is not torch.float32 or w.numel() != hd or not w.is_contiguous():
+                    raise ValueError(f"norm weights: both, contiguous fp32 [{hd}]")
+            qn, kn = q_norm_w.data_ptr(), k_norm_w.data_ptr()
+        _same_device(self.index, "append", q, k, v, rope_cos, rope_sin, q_out, q_norm_w, k_norm_w)
+        _launch(self.index, stream, "picoattn_paged_append", abi.lib().picoattn_paged_append, self.cfg_ref, self.ref,
+                layer, batch.ref,
+                abi.PAGED_APPEND_ARGS.pack(_dtype(k), rot, q_ptr, q_stride, k.data_ptr(), _heads(k, n, hkv, hd, "k"),
+                                           v.data_ptr(), _heads(v, n, hkv, hd, "v"), qn, kn, rope_cos.data_ptr(),
+                                           rope_sin.data_ptr(), out_ptr),
+                batch.ws_ptr, batch.ws_bytes)
 
     def attend(self, layer: int, batch: PagedBatch, q: torch.Tensor, out: torch.Tensor,
                stream: torch.cuda.Stream | None = None) -> None:
         """out [n_tok, n_heads, head_dim] (the cache's type or fp32) = causal attention
         of the rotated queries q (the cache's type) over their sequences' rows."""
-        n, hd, dev = batch.n_tok, self.cfg.head_dim, self.device
-        size = n * self.cfg.n_heads * hd
-        if q.dtype != self.dtype or q.numel() != size:
-            raise ValueError(f"q: [{n}, {self.cfg.n_heads}, {hd}] {self.dtype}, got {tuple(q.shape)} {q.dtype}")
-        if out.numel() != size or not out.is_contiguous():
-            raise ValueError(f"out: contiguous [{n}, {self.cfg.n_heads}, {hd}]")
-        _same_device(dev, q=q, out=out)
-        st = _on_device(dev, abi.lib().picoattn_paged_attn, self.cfg_ref, self.ref, layer, batch.ref, q.data_ptr(),
-                        _heads(q, n, hd, "q"), _dtype(out), out.data_ptr(), batch.ws_ptr, batch.ws_bytes,
-                        _launch_stream(dev, stream))
-        if st:
-            abi.check(st, "picoattn_paged_attn")
+        n = batch.n_tok
+        hq, _, hd, _ = self.shape
+        if q.dtype is not self.dtype or not out.is_contiguous():
+            raise ValueError(f"q: {self.dtype}, out: contiguous; got {q.dtype}, strides {out.stride()}")
+        _heads(out, n, hq, hd, "out")
+        _same_device(self.index, "attend", q, out)
+        _launch(self.index, stream, "picoattn_paged_attn", abi.lib().picoattn_paged_attn, self.cfg_ref, self.ref,
+                layer, batch.ref, q.data_ptr(), _heads(q, n, hq, hd, "q"), _dtype(out), out.data_ptr(), batch.ws_ptr,
+                batch.ws_bytes)
 
 
 class AttnState:

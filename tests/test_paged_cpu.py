@@ -46,17 +46,19 @@ def rope(dtype=abi.DTYPE_F16, mode=0, hd=64, rot=64, n=5, rows=100, q=None, k=No
     p = dict(pos=ADDR["pos"], cos=ADDR["cos"], sin=ADDR["sin"], ws=ADDR["ws"])
     p.update(over)
     q = q or abi.RopeRows(ADDR["q"], 8 * 64, ADDR["q_out"], 8 * 64, 8)
-    return L.picoattn_rope(dtype, mode, hd, rot, 0, n, p["pos"], rows, p["cos"], p["sin"], C.byref(q),
-                           C.byref(k) if k else None, p["ws"], ws_bytes, None)
+    args = abi.RopeArgs(dtype, mode, hd, rot, 0, n, rows, over.get("tensors", 2 if k else 1), p["pos"], p["cos"],
+                        p["sin"], q, k or abi.RopeRows())
+    return L.picoattn_rope(C.byref(args), p["ws"], ws_bytes, None)
 
 
 def append(c=None, ca=None, b=None, layer=0, dtype=abi.DTYPE_F16, rot=128, ws_bytes=1 << 30, **over):
     p = dict(q=ADDR["q"], qs=28 * 128, k=ADDR["k"], ks=512, v=ADDR["v"], vs=512, qn=None, kn=None, cos=ADDR["cos"],
              sin=ADDR["sin"], q_out=ADDR["q_out"], ws=ADDR["ws"])
     p.update(over)
-    return L.picoattn_paged_append(C.byref(c or cfg()), C.byref(ca or cache()), layer, C.byref(b or batch()), dtype,
-                                   p["q"], p["qs"], p["k"], p["ks"], p["v"], p["vs"], p["qn"], p["kn"], p["cos"],
-                                   p["sin"], rot, p["q_out"], p["ws"], ws_bytes, None)
+    args = abi.PagedAppendArgs(dtype, rot, p["q"], p["qs"], p["k"], p["ks"], p["v"], p["vs"], p["qn"], p["kn"],
+                               p["cos"], p["sin"], p["q_out"])
+    return L.picoattn_paged_append(C.byref(c or cfg()), C.byref(ca or cache()), layer, C.byref(b or batch()),
+                                   C.byref(args), p["ws"], ws_bytes, None)
 
 
 def attn(c=None, ca=None, b=None, layer=0, out_dtype=abi.DTYPE_F16, ws_bytes=1 << 30, **over):
@@ -93,6 +95,7 @@ INV, UNS, RNG, SPACE = abi.PICOATTN_EINVAL, abi.PICOATTN_EUNSUPPORTED, abi.PICOA
     (dict(q=abi.RopeRows(ADDR["q"], 512, ADDR["q"] + 64, 512, 8)), INV),         # overlaps, not in place
     (dict(q=abi.RopeRows(ADDR["q"], 512, ADDR["q"], 1024, 8)), INV),             # same start, other stride
     (dict(q=abi.RopeRows(ADDR["q"], 512, ADDR["q_out"], 512, 0)), INV),
+    (dict(tensors=3), INV), (dict(tensors=2), INV),
     (dict(k=abi.RopeRows(ADDR["k"], 512, ADDR["q_out"], 512, 8)), INV),          # both outputs at one place
     (dict(k=abi.RopeRows(ADDR["q_out"], 512, ADDR["k_out"], 512, 8)), INV),      # q's output over k
 ])
@@ -117,7 +120,7 @@ def test_rope_takes_interleaved_rows_of_one_projection_in_place():
     (dict(ca=cache(n_pages=0)), INV), (dict(ca=cache(k=None)), INV), (dict(ca=cache(v=ADDR["vp"] + 8)), INV),
     (dict(ca=cache(n_pages=1 << 26)), UNS),
     (dict(b=batch(n_seqs=0)), INV), (dict(b=batch(n_tok=0)), INV), (dict(b=batch(max_new=0)), INV),
-    (dict(b=batch(page_cols=0)), INV), (dict(b=batch(page_table=None)), INV), (dict(b=batch(q_start=None)), INV),
+    (dict(b=batch(page_cols=0)), INV), (dict(b=batch(n_tok=1 << 27)), UNS), (dict(b=batch(page_table=None)), INV), (dict(b=batch(q_start=None)), INV),
     (dict(b=batch(kv_len=ADDR["len"] + 2)), INV),
     (dict(b=batch(max_len=1025)), RNG), (dict(b=batch(max_len=0)), RNG), (dict(b=batch(max_new=2000)), RNG),
     (dict(b=batch(page_cols=63)), RNG),
@@ -146,6 +149,15 @@ def test_append_refuses(kw, want):
 ])
 def test_attn_refuses(kw, want):
     assert attn(**kw) == want
+
+
+def test_packed_arguments_have_the_structs_layout():
+    """abi.ROPE_ARGS / PAGED_APPEND_ARGS pack what the C structs (and their ctypes forms) hold."""
+    r = abi.RopeArgs(1, 0, 64, 32, 1, 7, 99, 2, 11, 12, 13, abi.RopeRows(21, 22, 23, 24, 25),
+                     abi.RopeRows(31, 32, 33, 34, 35))
+    assert bytes(r) == abi.ROPE_ARGS.pack(1, 0, 64, 32, 1, 7, 99, 2, 11, 12, 13, 21, 22, 23, 24, 25, 31, 32, 33, 34, 35)
+    a = abi.PagedAppendArgs(2, 48, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11)
+    assert bytes(a) == abi.PAGED_APPEND_ARGS.pack(2, 48, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11)
 
 
 def test_workspace_size():
