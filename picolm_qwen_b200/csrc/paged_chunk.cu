@@ -1,0 +1,929 @@
+// paged_chunk.cu -- paged attention of chunks of new tokens (and of single
+// tokens beside them) on the 5th-generation tensor cores.
+//
+// The g q heads of a KV head share its keys, so a 128-row tile of S = Q K^T holds
+// TQ = 128 / g tokens with all their g heads (row = token * g + head): 16 tokens
+// of 8 heads fill the tile that one head of 128 tokens would.  A block is one or
+// two such tiles of one KV head of one sequence; its keys come in tiles of 128
+// rows, gathered page by page by TMA.  Per CTA:
+//   warps 0-3, 4-7  softmax: thread = row = TMEM lane
+//   warp 8          work list and TMA;  warp 9  MMA issue, TMEM
+//   TMEM            S0, S1 (P over the columns it came from), O0, O1
+// Two-tile blocks: each softmax group has its own rows, K and V tiles serve
+// both, and one group's softmax runs while the other's products do.  One-tile
+// blocks (few new tokens): the groups take alternate key tiles of the same rows
+// and their (max, sum, O) are joined at the end.
+//
+// Compute-bound for two-tile blocks (per key tile and SM 2,048 cycles of tensor
+// work and as many of exponentials), HBM-bound for one-tile blocks.
+//
+// Work split: the blocks' costs (key tiles, twice for two-tile blocks) are known
+// to every CTA from the lengths.  Either whole blocks are handed out, longest
+// of each sequence first, by a counter; or, where blocks are too few or too
+// uneven, all their tiles are concatenated and cut into equal slices, the parts
+// of a cut block going to the workspace for a merge kernel.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+#include <type_traits>
+
+#include <cuda.h>
+
+#include "paged_common.cuh"
+#include "tcgen05.cuh"
+
+namespace picoattn {
+
+namespace {
+
+constexpr int BM = 128, BN = 128;
+constexpr int kThreads = 320;
+constexpr int kPlan = 64;          // threads that add up the sequences' costs
+constexpr int kMaxCtas = 160;
+constexpr int kMinCost = 4;        // least cost per CTA of a slice
+constexpr int kSliceOverhead = 12; // what cutting blocks costs, in the same unit (measured, see launch)
+constexpr int kPartRows = 2 * BM;
+constexpr float kNone = -1e30f;    // running maximum before any key
+constexpr float kStaleMaxP = 32768.0f;
+
+struct ChunkMeta {  // the cut block whose first part a CTA holds (nt 0: none)
+    int b, h, blk, nt, slices;
+    long long start, cost;  // its first cost unit; all blocks' units
+};
+
+struct ChunkArgs {
+    PagedAttnArgs a;
+    int tq;              // tokens per tile
+    int* counter;        // next whole block; zero between calls
+    ChunkMeta* meta;     // [grid]
+    float2* part_ml;     // [2 * grid][256]
+    float* part_o;       // [2 * grid][256][hd]
+};
+
+struct Item {
+    int b, h, tok0, ntok;  // first row of q and tokens of the block
+    int pos0;              // position of its first token
+    int j0, j1;            // key tiles
+    int slot;              // partial slot, -1: whole
+    int len;               // rows of the sequence
+    int poison;            // a page that does not exist was met
+};
+
+// ---- the work list --------------------------------------------------------------
+
+struct Blocks {
+    int n, len, t0, per, count;  // new tokens, rows, first token row, tokens per block, blocks
+    int tq;
+    __device__ __forceinline__ int ntok(int i) const { return min(per, n - i * per); }
+    __device__ __forceinline__ int tiles(int i) const { return (len - n + min(n, (i + 1) * per) + BN - 1) / BN; }
+    __device__ __forceinline__ int unit(int i) const { return ntok(i) > tq ? 2 : 1; }
+};
+
+__device__ __forceinline__ Blocks seq_blocks(const ChunkArgs& c, int b) {
+    const SeqSpan sp = seq_span(c.a.b, b);
+    Blocks x;
+    x.n = sp.ok ? sp.n : 0;
+    x.len = sp.len, x.t0 = sp.t0, x.tq = c.tq, x.per = 2 * c.tq;
+    x.count = (x.n + x.per - 1) / x.per;
+    return x;
+}
+
+__device__ __forceinline__ long long head_cost(const Blocks& x) {
+    long long s = 0;
+    for (int i = 0; i < x.count; i++) s += (long long)x.tiles(i) * x.unit(i);
+    return s;
+}
+
+struct Plan {
+    long long first_cost[kPlan + 1];  // of each plan thread's sequences
+    int first_item[kPlan + 1];
+    int most[kPlan / 32];             // the longest block's cost
+    int slices;                       // CTAs that share the cut-up list, 0: whole blocks
+};
+
+__device__ __forceinline__ long long slice_first(long long i, long long cost, int n) { return i * cost / n; }
+
+// A part's first (or end) tile for a slice that begins (ends) at cost unit x of a block from `start`.
+__device__ __forceinline__ int tile_at(long long x, long long start, int unit, int nt) {
+    return x <= start ? 0 : (int)min((long long)nt, (x - start + unit - 1) / unit);
+}
+
+// Walks a slice's parts (slices) or fetches whole blocks (list).
+struct Walk {
+    int b, h, blk;
+    long long at, end, base;  // cost units; base: of sequence b
+    Blocks x;
+    long long per_head, blk_start;
+    bool open;
+};
+
+// ---- one key tile of the online softmax ------------------------------------------
+
+template <class T>
+struct Pair16;
+template <>
+struct Pair16<__half> {
+    using V = __half2;
+    static __device__ __forceinline__ V cvt(float a, float b) { return __floats2half2_rn(a, b); }
+    static __device__ __forceinline__ float2 up(V v) { return __half22float2(v); }
+};
+template <>
+struct Pair16<__nv_bfloat16> {
+    using V = __nv_bfloat162;
+    static __device__ __forceinline__ V cvt(float a, float b) { return __floats2bfloat162_rn(a, b); }
+    static __device__ __forceinline__ float2 up(V v) { return __bfloat1622float2(v); }
+};
+
+// S (128 fp32 columns at tS, unscaled) -> P = 2^(scale S - m) in 16 bits over its
+// first 64 columns; m (log2 units) and the row sum l updated, O (HD columns at tO)
+// rescaled when m grows.  lim: keys visible to the row counted from the tile's
+// first; mask: some row of the warp does not see all 128.  The maximum is stale
+// by design: p is taken against the running one in the same pass that reads S, and
+// kept unless some p passes 2^15 (exact in 16 bits' range and harmless in the fp32
+// sums); then the tile is done again with its own maximum.
+template <class T, int HD, class WaitPrevPV>
+__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, bool first, int lim, bool mask, float scale,
+                                             float& m, float& l, WaitPrevPV wait_prev_pv) {
+    using P2 = Pair16<T>;
+    const uint64_t sc2 = f2_pack(scale, scale);
+    bool done = false;
+    {
+        uint32_t pk[BN / 2];
+        uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+        typename P2::V top[4] = {P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f)};
+        uint32_t sbuf[2][32];
+        tmem_ld32(tS, sbuf[0]);
+        if (first) {  // start from the maximum of the first 32 columns
+            tmem_ld_wait();
+            float m0 = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+                if (!mask || e < lim) m0 = fmaxf(m0, __uint_as_float(sbuf[0][e]));
+            m = fmaxf(m0 * scale, kNone);
+        }
+        const uint64_t nm2 = f2_pack(-m, -m);
+#pragma unroll
+        for (int c = 0; c < BN / 32; c++) {
+            tmem_ld_wait();
+            uint32_t (&sr)[32] = sbuf[c & 1];
+            if (c + 1 < BN / 32) tmem_ld32(tS + (c + 1) * 32, sbuf[(c + 1) & 1]);
+            if (mask) {
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                    if (c * 32 + e >= lim) sr[e] = __float_as_uint(-INFINITY);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                float d0, d1;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), sc2, nm2), d0, d1);
+                const float p0 = ex2(d0), p1 = ex2(d1);
+                sum[e & 3] = f2_add(sum[e & 3], f2_pack(p0, p1));
+                const typename P2::V h = P2::cvt(p0, p1);
+                top[e & 3] = __hmax2(top[e & 3], h);
+                pk[c * 16 + e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        const float2 t2 = P2::up(__hmax2(__hmax2(top[0], top[1]), __hmax2(top[2], top[3])));
+        if (!__any_sync(0xffffffffu, !(fmaxf(t2.x, t2.y) <= kStaleMaxP))) {
+            tmem_st32(tS, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
+            tmem_st32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
+            float a0, a1;
+            f2_unpack(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])), a0, a1);
+            l += a0 + a1;
+            done = true;
+        }
+    }
+    if (!done) {
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; c++) {
+            uint32_t sr[32];
+            tmem_ld32(tS + c * 32, sr);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+                if (!mask || c * 32 + e < lim) mx = fmaxf(mx, __uint_as_float(sr[e]));
+        }
+        const float m_new = fmaxf(mx * scale, first ? kNone : m);
+        if (!first) {
+            const float corr = ex2(m - m_new);
+            wait_prev_pv();
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; c++) {
+                uint32_t o[32];
+                tmem_ld32(tO + c * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                tmem_st32(tO + c * 32, o);
+            }
+            tmem_st_wait();
+            l *= corr;
+        }
+        m = m_new;
+        // 32 scores at a time; P of chunk c lands in columns [16c, 16c + 16), already read
+        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t sbuf[2][32];
+        tmem_ld32(tS, sbuf[0]);
+#pragma unroll
+        for (int c = 0; c < BN / 32; c++) {
+            tmem_ld_wait();
+            uint32_t (&sr)[32] = sbuf[c & 1];
+            if (c + 1 < BN / 32) tmem_ld32(tS + (c + 1) * 32, sbuf[(c + 1) & 1]);
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                float p[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const bool seen = !mask || c * 32 + 2 * e + i < lim;
+                    p[i] = seen ? ex2(__fmaf_rn(__uint_as_float(sr[2 * e + i]), scale, -m)) : 0.f;
+                }
+                s4[e & 3] += p[0] + p[1];
+                const typename P2::V h = P2::cvt(p[0], p[1]);
+                pk[e] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            tmem_st16(tS + c * 16, pk);
+        }
+        l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    }
+    tmem_st_wait();
+}
+
+// ---- output ------------------------------------------------------------------------
+
+// 128 bytes of every row of a warp (lane = row, 32 words w) to dst + off(row):
+// through a 4 KB shared stage, 16-byte unit u of row r at u ^ (r & 7), so that
+// eight lanes write a row's 128 bytes together.  off < 0: the row is not stored.
+__device__ __forceinline__ void store_rows(const uint32_t (&w)[32], uint4* stage, uint8_t* dst, long long off, int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+        stage[lane * 8 + (u ^ (lane & 7))] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int row = 4 * i + (lane >> 3), u = lane & 7;
+        const long long o = __shfl_sync(0xffffffffu, off, row);
+        if (o >= 0) *reinterpret_cast<uint4*>(dst + o + 16 * u) = stage[row * 8 + (u ^ (row & 7))];
+    }
+}
+
+// ---- the kernel --------------------------------------------------------------------
+
+template <int HD>
+struct Smem {
+    static constexpr int kBox = BM * 128;            // 128 rows x 64 columns of 16 bits
+    static constexpr int kTile = (HD / 64) * kBox;
+    static constexpr int NK = 2, NV = 2;
+    static constexpr int kQ = 0;
+    static constexpr int kK = 2 * kTile;
+    static constexpr int kV = kK + NK * kTile;
+    static constexpr int kStage = kV + NV * kTile;   // 4 KB per softmax warp
+    static constexpr int kPlanAt = kStage + 8 * 4096;
+    static constexpr int kBars = (kPlanAt + (int)sizeof(Plan) + 15) / 16 * 16;
+    static constexpr int kItems = kBars + 24 * 8;
+    static constexpr int kEnd = kItems + 2 * (int)sizeof(Item) + 16;
+    static constexpr int kDyn = kEnd + 1024;         // slack to align the base
+    static_assert(kDyn <= 227 * 1024, "one CTA per SM");
+};
+
+template <class T, int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const ChunkArgs c) {
+    using L = Smem<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const PagedAttnArgs& a = c.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+    uint64_t* item_full = bars + 0;     // [2]
+    uint64_t* item_empty = bars + 2;    // [2]
+    uint64_t* q_full = bars + 4;
+    uint64_t* q_empty = bars + 5;
+    uint64_t* k_full = bars + 6;        // [NK]
+    uint64_t* k_empty = bars + 8;
+    uint64_t* v_full = bars + 10;       // [NV]
+    uint64_t* v_empty = bars + 12;
+    uint64_t* s_full = bars + 14;       // [2] per softmax group
+    uint64_t* p_full = bars + 16;
+    uint64_t* pv_done = bars + 18;
+    uint64_t* o_free = bars + 20;
+    Plan* plan = reinterpret_cast<Plan*>(smem + L::kPlanAt);
+    Item* items = reinterpret_cast<Item*>(smem + L::kItems);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
+    unsigned int* status = a.b.status;
+
+    pdl_trigger();
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 3);
+            mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1), mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&pv_done[i], 1), mbar_init(&o_free[i], 4);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        fence_mbar_init();
+        prefetch_tmap(&tmQ);
+        prefetch_tmap(&tmK);
+        prefetch_tmap(&tmV);
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    if (c.tq * a.g < BM) {  // rows that no load of Q writes
+        for (int i = tid; i < 2 * L::kTile / 16; i += kThreads)
+            reinterpret_cast<uint4*>(smem + L::kQ)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_shared();
+    }
+    pdl_wait();
+    // ---------------- plan ----------------
+    const int per = (a.b.n_seqs + kPlan - 1) / kPlan;
+    long long my_cost = 0;
+    int my_items = 0, my_max = 0;
+    if (tid < kPlan) {
+        for (int b = tid * per; b < min((tid + 1) * per, a.b.n_seqs); b++) {
+            const Blocks x = seq_blocks(c, b);
+            my_cost += head_cost(x) * a.hkv;
+            my_items += x.count * a.hkv;
+            if (x.count) my_max = max(my_max, x.tiles(x.count - 1) * 2);
+        }
+        plan->first_cost[tid + 1] = my_cost;
+        plan->first_item[tid + 1] = my_items;
+    }
+    // rows of sequences outside the host's bounds
+    for (int b = blockIdx.x; b < a.b.n_seqs; b += gridDim.x) {
+        const SeqSpan sp = seq_span(a.b, b);
+        if (sp.ok) continue;
+        if (tid == 0) atomicOr(status, PICOATTN_DEV_BAD_POS);
+        const int t0 = max(sp.t0, 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
+        const long long words = t1 > t0 ? (long long)(t1 - t0) * a.hq * HD : 0;
+        for (long long i = tid; i < words; i += kThreads) {
+            const size_t at = (size_t)t0 * a.hq * HD + i;
+            if (a.out_dtype == PICOATTN_DTYPE_F32) static_cast<float*>(a.out)[at] = __int_as_float(0x7fc00000);
+            else static_cast<T*>(a.out)[at] = Elem<T>::round(__int_as_float(0x7fc00000));
+        }
+    }
+    if (tid < kPlan) {
+        for (int o = 16; o; o >>= 1) my_max = max(my_max, __shfl_xor_sync(0xffffffffu, my_max, o));
+        if (lane == 0) plan->most[warp] = my_max;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) {  // prefix sums, two entries a lane
+        const long long x0 = plan->first_cost[2 * lane + 1], x1 = plan->first_cost[2 * lane + 2];
+        const int y0 = plan->first_item[2 * lane + 1], y1 = plan->first_item[2 * lane + 2];
+        long long xs = x0 + x1;
+        int ys = y0 + y1;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long xo = __shfl_up_sync(0xffffffffu, xs, o);
+            const int yo = __shfl_up_sync(0xffffffffu, ys, o);
+            if (lane >= o) xs += xo, ys += yo;
+        }
+        plan->first_cost[2 * lane + 1] = xs - x1, plan->first_cost[2 * lane + 2] = xs;
+        plan->first_item[2 * lane + 1] = ys - y1, plan->first_item[2 * lane + 2] = ys;
+        if (lane == 31) {
+            plan->first_cost[0] = 0;
+            plan->first_item[0] = 0;
+            const int n = (int)min((long long)gridDim.x, (xs + kMinCost - 1) / kMinCost);
+            int most = 0;
+            for (int i = 0; i < kPlan / 32; i++) most = max(most, plan->most[i]);
+            // whole blocks end when the longest does, or, dealt out one by one, some 15% after the mean
+            const long long mean = n ? (xs + n - 1) / n : 0;
+            const long long whole = max((long long)most, ys <= (int)gridDim.x ? 0 : mean + mean / 7);
+            plan->slices = mean + kSliceOverhead < whole ? n : 0;
+            c.meta[blockIdx.x].nt = 0;
+        }
+    }
+    __syncthreads();
+    const uint32_t tmem = *tmem_slot;
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);
+    const int g = a.g, tq = c.tq;
+
+    if (warp == 8) {
+        // ---------------- work list and TMA ----------------
+        const int slices = plan->slices;
+        Walk wk{};
+        wk.open = false;
+        if (slices && (int)blockIdx.x < slices) {
+            const long long cost = plan->first_cost[kPlan];
+            wk.at = slice_first(blockIdx.x, cost, slices);
+            wk.end = slice_first(blockIdx.x + 1, cost, slices);
+            int lo = 0, hi = kPlan;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (plan->first_cost[mid] <= wk.at) lo = mid;
+                else hi = mid;
+            }
+            wk.b = lo * per;
+            wk.base = plan->first_cost[lo];
+        }
+        // next item of this CTA (lane 0); false: none
+        auto next = [&](Item& it) -> bool {
+            it.poison = 0;
+            if (!slices) {
+                const int idx = atomicAdd(c.counter, 1);
+                if (idx >= plan->first_item[kPlan]) return false;
+                int lo = 0, hi = kPlan;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (plan->first_item[mid] <= idx) lo = mid;
+                    else hi = mid;
+                }
+                int rest = idx - plan->first_item[lo], b = lo * per;
+                Blocks x = seq_blocks(c, b);
+                while (rest >= x.count * a.hkv) {
+                    rest -= x.count * a.hkv;
+                    x = seq_blocks(c, ++b);
+                }
+                const int i = x.count - 1 - rest / a.hkv;  // a sequence's longest first
+                it.b = b, it.h = rest % a.hkv;
+                it.tok0 = x.t0 + i * x.per, it.ntok = x.ntok(i), it.pos0 = x.len - x.n + i * x.per;
+                it.j0 = 0, it.j1 = x.tiles(i), it.slot = -1, it.len = x.len;
+                return true;
+            }
+            while (wk.at < wk.end) {
+                if (!wk.open) {  // find the block that holds cost unit `at`
+                    for (;; wk.b++) {
+                        wk.x = seq_blocks(c, wk.b);
+                        wk.per_head = head_cost(wk.x);
+                        if (wk.at < wk.base + wk.per_head * a.hkv) break;
+                        wk.base += wk.per_head * a.hkv;
+                    }
+                    wk.h = (int)((wk.at - wk.base) / wk.per_head);
+                    wk.blk = 0;
+                    wk.blk_start = wk.base + wk.h * wk.per_head;
+                    for (;;) {
+                        const int cost = wk.x.tiles(wk.blk) * wk.x.unit(wk.blk);
+                        if (wk.at < wk.blk_start + cost) break;
+                        wk.blk_start += cost;
+                        wk.blk++;
+                    }
+                    wk.open = true;
+                }
+                const int nt = wk.x.tiles(wk.blk), u = wk.x.unit(wk.blk);
+                const int j0 = tile_at(wk.at, wk.blk_start, u, nt), j1 = tile_at(wk.end, wk.blk_start, u, nt);
+                if (j0 < j1) {
+                    it.b = wk.b, it.h = wk.h;
+                    it.tok0 = wk.x.t0 + wk.blk * wk.x.per, it.ntok = wk.x.ntok(wk.blk);
+                    it.pos0 = wk.x.len - wk.x.n + wk.blk * wk.x.per;
+                    it.j0 = j0, it.j1 = j1, it.len = wk.x.len;
+                    it.slot = j0 == 0 && j1 == nt ? -1 : 2 * (int)blockIdx.x + (j0 == 0 ? 1 : 0);
+                    if (j0 == 0 && j1 < nt)
+                        c.meta[blockIdx.x] = {wk.b, wk.h, wk.blk, nt, slices, wk.blk_start, plan->first_cost[kPlan]};
+                }
+                // step to the next block
+                wk.at = wk.blk_start + nt * u;
+                if (wk.blk + 1 < wk.x.count) {
+                    wk.blk_start = wk.at;
+                    wk.blk++;
+                } else if (wk.h + 1 < a.hkv) {
+                    wk.h++;
+                    wk.blk = 0;
+                    wk.blk_start = wk.at;
+                } else {
+                    wk.base += wk.per_head * a.hkv;
+                    wk.b++;
+                    wk.open = false;
+                }
+                if (j0 < j1) return true;
+            }
+            return false;
+        };
+        const int box_rows = min(a.b.page_size, BN), boxes = BN / box_rows;
+        const int half = (lane / boxes) % (HD / 64), kv = lane / (boxes * (HD / 64)), box = lane % boxes;
+        int t = 0;
+        for (int k = 0;; k++) {
+            const int slot = k & 1;
+            if (k >= 2) mbar_wait(&item_empty[slot], (uint32_t)(((k >> 1) - 1) & 1), status);
+            if (lane == 0) {
+                Item it;
+                if (!next(it)) it.b = -1;
+                items[slot] = it;
+            }
+            __syncwarp();
+            const Item it = items[slot];
+            if (lane == 0) mbar_arrive(&item_full[slot]);
+            if (it.b < 0) break;
+            const bool two = it.ntok > tq;
+            if (lane == 0) {
+                if (k >= 1) mbar_wait(q_empty, (uint32_t)((k - 1) & 1), status);
+                mbar_arrive_expect_tx(q_full, (two ? 2u : 1u) * (HD / 64) * (uint32_t)(tq * g) * 128u);
+                for (int w = 0; w < (two ? 2 : 1); w++)
+                    for (int x = 0; x < HD / 64; x++)
+                        tma_load_3d(smem + L::kQ + w * L::kTile + x * L::kBox, &tmQ, 64 * x, it.h * g, it.tok0 + w * tq,
+                                    q_full);
+            }
+            const int* table = a.b.page_table + (size_t)it.b * a.b.page_cols;
+            auto page_of = [&](int j) {  // this lane's box of tile j: its page, -1: none, -2: no such page
+                const int r = j * BN + box * box_rows;
+                if (kv > 1 || j >= it.j1 || r >= it.len) return -1;
+                const int p = table[r >> a.b.page_shift];
+                return p < 0 || p >= a.b.n_pages ? -2 : p;
+            };
+            int page = page_of(it.j0);
+            for (int j = it.j0; j < it.j1; j++, t++) {
+                const int next_page = page_of(j + 1);
+                const int r = j * BN + box * box_rows;
+                const int y = ((max(page, 0) * a.hkv + it.h) * a.b.page_size) + (r & (a.b.page_size - 1));
+                const bool any_bad = __any_sync(0xffffffffu, page == -2);
+                const uint32_t n_boxes = __popc(__ballot_sync(0xffffffffu, page != -1 && kv == 0));
+                if (any_bad && lane == 0) {
+                    atomicOr(status, PICOATTN_DEV_BAD_PAGE);
+                    items[slot].poison = 1;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int s = t % 2, use = t / 2;
+                    uint64_t* full = i ? &v_full[s] : &k_full[s];
+                    if (use > 0) mbar_wait(i ? &v_empty[s] : &k_empty[s], (uint32_t)((use - 1) & 1), status);
+                    if (lane == 0) mbar_arrive_expect_tx(full, n_boxes * (uint32_t)box_rows * 128u);
+                    __syncwarp();
+                    if (page != -1 && kv == i)
+                        tma_load_2d(smem + (i ? L::kV : L::kK) + s * L::kTile + half * L::kBox + box * box_rows * 128,
+                                    i ? &tmV : &tmK, 64 * half, y, full);
+                }
+                page = next_page;
+            }
+        }
+    } else if (warp == 9) {
+        // ---------------- MMA issue ----------------
+        if (lane == 0) {
+            constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+            constexpr uint32_t idesc_qk = idesc_f16_f32(BM, BN, false, false) | kBf16;
+            constexpr uint32_t idesc_pv = idesc_f16_f32(BM, HD, false, true) | kBf16;
+            const uint64_t dq = smem_desc_sw128(smem_u32(smem + L::kQ), 16, 1024);
+            const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kK), 16, 1024);
+            const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV), L::kBox, 1024);
+            // S of group w from Q tile qt and K stage s
+            auto qk = [&](int w, int qt, int s) {
+                const uint64_t qd = desc_advance(dq, qt * L::kTile), kd = desc_advance(dk, s * L::kTile);
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk++) {
+                    const uint32_t off = (kk >> 2) * L::kBox + (kk & 3) * 32;
+                    umma_ss(tmem + w * 128, desc_advance(qd, off), desc_advance(kd, off), idesc_qk, kk > 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[w]);
+            };
+            auto pv = [&](int w, int s, bool first) {
+                const uint64_t vd = desc_advance(dv, s * L::kTile);
+#pragma unroll
+                for (int kk = 0; kk < BN / 16; kk++)
+                    umma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, desc_advance(vd, kk * 16 * 128), idesc_pv,
+                            (!first || kk > 0) ? 1u : 0u);
+                umma_commit(&pv_done[w]);
+            };
+            auto wait = [&](uint64_t* bar, int phase) {
+                if (!mbar_test(bar, (uint32_t)(phase & 1))) mbar_wait(bar, (uint32_t)(phase & 1), status);
+            };
+            int t = 0, tiles[2] = {0, 0}, uses[2] = {0, 0};  // key tiles; each group's tiles and blocks so far
+            for (int k = 0;; k++) {
+                const int slot = k & 1;
+                mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
+                const Item it = items[slot];
+                mbar_arrive(&item_empty[slot]);
+                if (it.b < 0) break;
+                const int n = it.j1 - it.j0;
+                wait(q_full, k);
+                if (it.ntok > tq) {
+                    // two Q tiles; group 0's keys may end before the block's
+                    const int n0 = min(it.j1, (it.pos0 + tq + BN - 1) / BN) - it.j0;
+                    wait(&k_full[t % 2], t / 2);
+                    tc_fence_after();
+                    if (n0 > 0) qk(0, 0, t % 2);
+                    qk(1, 1, t % 2);
+                    umma_commit(&k_empty[t % 2]);
+                    if (n == 1) umma_commit(q_empty);
+                    for (int j = 0; j < n; j++, t++) {
+                        const bool more = j + 1 < n;
+#pragma unroll
+                        for (int w = 0; w < 2; w++) {
+                            const int nw = w ? n : n0;
+                            if (j < nw) {
+                                const bool need_o = j == 0 && uses[w] > 0, kw = j + 1 < nw;
+                                bool ok = mbar_test(&p_full[w], (uint32_t)(tiles[w] & 1)) &
+                                          mbar_test(&v_full[t % 2], (uint32_t)((t / 2) & 1));
+                                if (need_o) ok &= mbar_test(&o_free[w], (uint32_t)((uses[w] - 1) & 1));
+                                if (kw) ok &= mbar_test(&k_full[(t + 1) % 2], (uint32_t)(((t + 1) / 2) & 1));
+                                if (!ok) {
+                                    mbar_wait(&p_full[w], (uint32_t)(tiles[w] & 1), status);
+                                    mbar_wait(&v_full[t % 2], (uint32_t)((t / 2) & 1), status);
+                                    if (need_o) mbar_wait(&o_free[w], (uint32_t)((uses[w] - 1) & 1), status);
+                                    if (kw) mbar_wait(&k_full[(t + 1) % 2], (uint32_t)(((t + 1) / 2) & 1), status);
+                                }
+                                tc_fence_after();
+                                pv(w, t % 2, j == 0);
+                                if (kw) qk(w, w, (t + 1) % 2);
+                                tiles[w]++;
+                            }
+                        }
+                        umma_commit(&v_empty[t % 2]);
+                        if (more) {
+                            umma_commit(&k_empty[(t + 1) % 2]);
+                            if (j + 2 == n) umma_commit(q_empty);
+                        }
+                    }
+                    if (n0 > 0) uses[0]++;
+                    uses[1]++;
+                } else {
+                    // one Q tile: the groups take alternate key tiles
+                    for (int j = 0; j < min(n, 2); j++) {
+                        wait(&k_full[(t + j) % 2], (t + j) / 2);
+                        tc_fence_after();
+                        qk(j, 0, (t + j) % 2);
+                        umma_commit(&k_empty[(t + j) % 2]);
+                        if (j + 1 == n) umma_commit(q_empty);
+                    }
+                    for (int j = 0; j < n; j++, t++) {
+                        const int w = j & 1;
+                        const bool need_o = j < 2 && uses[w] > 0, more = j + 2 < n;
+                        wait(&p_full[w], tiles[w]);
+                        wait(&v_full[t % 2], t / 2);
+                        if (need_o) wait(&o_free[w], uses[w] - 1);
+                        tc_fence_after();
+                        pv(w, t % 2, j < 2);
+                        umma_commit(&v_empty[t % 2]);
+                        tiles[w]++;
+                        if (more) {
+                            wait(&k_full[t % 2], (t + 2) / 2);
+                            tc_fence_after();
+                            qk(w, 0, t % 2);
+                            umma_commit(&k_empty[t % 2]);
+                            if (j + 3 == n) umma_commit(q_empty);
+                        }
+                    }
+                    uses[0]++;
+                    if (n > 1) uses[1]++;
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax ----------------
+        const int w = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + w * 128 + lanes, tO = tmem + 256 + w * 128 + lanes;
+        uint4* stage = reinterpret_cast<uint4*>(smem + L::kStage + warp * 4096);
+        float2* xs = reinterpret_cast<float2*>(smem + L::kStage + 4 * 4096);  // group 1's (max, sum), one-tile blocks
+        const int rt = r / g, rh = r - rt * g;  // the row's token in its tile, and head
+        int t = 0, mine = 0;  // key tiles of the CTA, of this group
+        for (int k = 0;; k++) {
+            const int slot = k & 1;
+            mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
+            const Item it = items[slot];
+            if (it.b < 0) break;
+            const bool two = it.ntok > tq;
+            const int n = it.j1 - it.j0;
+            const int tok = (two ? w * tq : 0) + rt;
+            const bool valid = rt < tq && tok < it.ntok;
+            const int lim = valid ? it.pos0 + tok + 1 : 0;  // keys the row sees
+            // the fewest and most keys that valid rows of this warp see (rows are token-major)
+            const bool live = __any_sync(0xffffffffu, valid);
+            const int lim_lo = __reduce_min_sync(0xffffffffu, valid ? lim : 0x7fffffff);
+            const int n_own = !two ? (n + 1 - w) / 2
+                                   : (w ? n : max(0, min(it.j1, (it.pos0 + tq + BN - 1) / BN) - it.j0));
+            float m = kNone, l = 0.f;
+            for (int i = 0; i < n_own; i++, mine++) {
+                const int j = two ? i : 2 * i + w, base = (it.j0 + j) * BN;
+                mbar_wait(&s_full[w], (uint32_t)(mine & 1), status);
+                tc_fence_after();
+                if (live)
+                    softmax_tile<T, HD>(tS, tO, i == 0, lim - base, base + BN > lim_lo, scale, m, l,
+                                        [&] { mbar_wait(&pv_done[w], (uint32_t)((mine - 1) & 1), status); });
+                if (base + BN > it.len) {
+                    // rows past the sequence hold anything: their V must not meet the zero weights as a NaN
+                    const int s = (t + j) % 2;
+                    mbar_wait(&v_full[s], (uint32_t)(((t + j) / 2) & 1), status);
+                    for (int e = r; e < BN * 8 * (HD / 64); e += 128) {
+                        const int row = (e >> 3) & (BN - 1), x = e >> 10;
+                        if (base + row >= it.len)
+                            *reinterpret_cast<uint4*>(smem + L::kV + s * L::kTile + x * L::kBox + row * 128 + (e & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_shared();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[w]);
+            }
+            t += n;
+            // the items' last tile has been read: its poison flag is final
+            if (n_own > 0 && *reinterpret_cast<volatile int*>(&items[slot].poison)) l = __int_as_float(0x7fc00000);
+            named_bar_sync(1 + w, 128);  // every warp of the group has read the item
+            if (r == 0) mbar_arrive(&item_empty[slot]);
+            if (n_own > 0) {
+                mbar_wait(&pv_done[w], (uint32_t)((mine - 1) & 1), status);
+                tc_fence_after();
+            }
+            const bool join = !two && n > 1;
+            if (!two && w == 1) {  // hand over to group 0
+                if (join) {
+                    xs[r] = make_float2(m, l);
+                    tc_fence_before();
+                    named_bar_arrive(3, 256);
+                }
+                continue;
+            }
+            float w0 = 1.f, w1 = 0.f;
+            if (join) {
+                named_bar_sync(3, 256);
+                tc_fence_after();
+                const float2 o = xs[r];
+                const float M = fmaxf(m, o.x);
+                w0 = ex2(m - M), w1 = ex2(o.x - M);
+                l = l * w0 + o.y * w1;
+                m = M;
+            }
+            const bool part = it.slot >= 0;
+            if (!part) {
+                const float inv = 1.0f / l;
+                w0 *= inv, w1 *= inv;
+            }
+            // 32 columns of the row's O, weighted
+            auto load = [&](int col, float (&o)[32]) {
+                if (n_own == 0) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = 0.f;
+                    return;
+                }
+                uint32_t x[32];
+                tmem_ld32(tO + col, x);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = __uint_as_float(x[e]) * w0;
+                if (join) {
+                    tmem_ld32(tO + 128 + col, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __fmaf_rn(__uint_as_float(x[e]), w1, o[e]);
+                }
+            };
+            auto release = [&] {  // O is in registers: the next block's products may overwrite it
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (n_own > 0) mbar_arrive(&o_free[w]);
+                    if (join) mbar_arrive(&o_free[1]);
+                }
+            };
+            const int row = w * BM + r;  // of the block's two tiles (one-tile blocks: w is 0)
+            if (part && valid) c.part_ml[(size_t)it.slot * kPartRows + row] = make_float2(m, l);
+            const long long orow =
+                part ? ((long long)it.slot * kPartRows + row) * HD
+                     : ((long long)(it.tok0 + tok) * a.hq + it.h * g + rh) * HD;
+            const bool f32 = part || a.out_dtype == PICOATTN_DTYPE_F32;
+            uint8_t* dst = part ? reinterpret_cast<uint8_t*>(c.part_o) : static_cast<uint8_t*>(a.out);
+            if (!live) {
+                release();
+            } else if (f32) {
+#pragma unroll 1
+                for (int col = 0; col < HD; col += 32) {
+                    float o[32];
+                    load(col, o);
+                    if (col + 32 == HD) release();
+                    uint32_t x[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) x[e] = __float_as_uint(o[e]);
+                    store_rows(x, stage, dst + col * 4, valid ? orow * 4 : -1, lane);
+                }
+            } else {
+#pragma unroll 1
+                for (int col = 0; col < HD; col += 64) {
+                    uint32_t x[32];
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        float o[32];
+                        load(col + 32 * y, o);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[16 * y + e] = Elem<T>::pack2(o[2 * e], o[2 * e + 1]);
+                    }
+                    if (col + 64 == HD) release();
+                    store_rows(x, stage, dst + col * 2, valid ? orow * 2 : -1, lane);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the parts of the blocks that slices cut: block (CTA that holds a cut
+// block's first part, row group), thread (row, four columns).  Also sets the
+// work counter back.
+template <class T, int HD>
+__global__ void __launch_bounds__(256) paged_chunk_merge_kernel(ChunkArgs c) {
+    constexpr int C4 = HD / 4, RB = 256 / C4;
+    pdl_trigger();
+    pdl_wait();
+    const PagedAttnArgs& a = c.a;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *c.counter = 0;
+    const ChunkMeta mt = c.meta[blockIdx.x];
+    if (mt.nt == 0) return;
+    const Blocks x = seq_blocks(c, mt.b);
+    const int row = blockIdx.y * RB + threadIdx.x / C4, c4 = threadIdx.x % C4;
+    const int rt = (row % BM) / a.g, rh = row % BM - rt * a.g, tok = row / BM * c.tq + rt;
+    if (rt >= c.tq || tok >= x.ntok(mt.blk)) return;
+    const int unit = x.unit(mt.blk);
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    int j0 = 0;
+    for (int i = blockIdx.x; j0 < mt.nt; i++) {
+        const int j1 = tile_at(slice_first(i + 1, mt.cost, mt.slices), mt.start, unit, mt.nt);
+        if (j1 == j0) continue;
+        const size_t at = (size_t)(2 * i + (j0 == 0 ? 1 : 0)) * kPartRows + row;
+        const float2 ml = __ldcg(c.part_ml + at);
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(c.part_o + at * HD) + c4);
+        const float Mn = fmaxf(M, ml.x), keep = ex2(M - Mn), w = ex2(ml.x - Mn);
+        M = Mn;
+        L = L * keep + ml.y * w;
+        acc.x = acc.x * keep + o.x * w, acc.y = acc.y * keep + o.y * w;
+        acc.z = acc.z * keep + o.z * w, acc.w = acc.w * keep + o.w * w;
+        j0 = j1;
+    }
+    const float inv = 1.0f / L;
+    const size_t at = ((size_t)(x.t0 + mt.blk * x.per + tok) * a.hq + mt.h * a.g + rh) * HD + 4 * c4;
+    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+    if (a.out_dtype == PICOATTN_DTYPE_F32)
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = acc;
+    else
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
+            make_uint2(Elem<T>::pack2(acc.x, acc.y), Elem<T>::pack2(acc.z, acc.w));
+}
+
+// ---- host -----------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeTiled>(p) : nullptr;
+    }();
+    return fn;
+}
+
+// Boxes of 64 columns (128 bytes, 128-byte swizzle) x the other dimensions' box.
+bool make_map(CUtensorMap* m, const PagedAttnArgs& a, const void* base, int rank, const cuuint64_t* dims,
+              const cuuint64_t* strides, const cuuint32_t* box) {
+    const EncodeTiled fn = encoder();
+    const cuuint32_t one[3] = {1, 1, 1};
+    return fn && fn(m, a.dtype == PICOATTN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                    (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr size_t kMetaBytes = (kMaxCtas * sizeof(ChunkMeta) + 255) / 256 * 256;
+constexpr size_t kMlBytes = 2 * (size_t)kMaxCtas * kPartRows * 8;
+
+template <class T, int HD>
+cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
+    using L = Smem<HD>;
+    static PerDeviceOnce setup;
+    cudaError_t e = setup.run([] {
+        return cudaFuncSetAttribute(paged_chunk_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDyn);
+    });
+    if (e != cudaSuccess) return e;
+    ChunkArgs c{};
+    c.a = a;
+    c.tq = BM / a.g;
+    c.counter = reinterpret_cast<int*>(a.b.status) + 16;  // in the workspace header
+    c.meta = reinterpret_cast<ChunkMeta*>(a.ws);
+    c.part_ml = reinterpret_cast<float2*>(a.ws + kMetaBytes);
+    c.part_o = reinterpret_cast<float*>(a.ws + kMetaBytes + kMlBytes);
+    CUtensorMap mq, mk, mv;
+    const cuuint64_t qd[3] = {HD, (cuuint64_t)a.hq, (cuuint64_t)a.b.n_tok}, qs[2] = {HD * 2, (cuuint64_t)a.qs * 2};
+    const cuuint32_t qb[3] = {64, (cuuint32_t)a.g, (cuuint32_t)c.tq};
+    const cuuint64_t kd[2] = {HD, (cuuint64_t)a.b.n_pages * a.hkv * a.b.page_size}, ks[1] = {HD * 2};
+    const cuuint32_t kb[2] = {64, (cuuint32_t)std::min(a.b.page_size, BN)};
+    if (!make_map(&mq, a, a.q, 3, qd, qs, qb) || !make_map(&mk, a, a.k_pool, 2, kd, ks, kb) ||
+        !make_map(&mv, a, a.v_pool, 2, kd, ks, kb))
+        return cudaErrorInvalidValue;
+    const long long blocks = (long long)a.b.n_seqs * a.hkv * ((a.b.max_new + 2 * c.tq - 1) / (2 * c.tq));
+    const long long tiles = (a.b.max_len + BN - 1) / BN;  // a slice has at least kMinCost units, a whole block a CTA
+    const int grid = (int)std::min<long long>(std::min(device_sm_count(), kMaxCtas), blocks * tiles);
+    e = launch_pdl(paged_chunk_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)L::kDyn, stream, mq, mk, mv, c);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(paged_chunk_merge_kernel<T, HD>, dim3(grid, kPartRows / (256 / (HD / 4))), dim3(256), 0, stream, c);
+}
+
+}  // namespace
+
+size_t paged_chunk_bytes(int hd) { return kMetaBytes + kMlBytes + 2 * (size_t)kMaxCtas * kPartRows * 4 * hd; }
+
+cudaError_t launch_paged_chunk(const PagedAttnArgs& a, cudaStream_t stream) {
+    if (a.dtype == PICOATTN_DTYPE_F16)
+        return a.hd == 64 ? launch_types<__half, 64>(a, stream) : launch_types<__half, 128>(a, stream);
+    return a.hd == 64 ? launch_types<__nv_bfloat16, 64>(a, stream) : launch_types<__nv_bfloat16, 128>(a, stream);
+}
+
+}  // namespace picoattn

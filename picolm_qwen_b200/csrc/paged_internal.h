@@ -87,6 +87,9 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t stream);
 bool paged_few_fits(const PagedAttnArgs& a);
 size_t paged_few_bytes(int hd, int n_seqs);
 cudaError_t launch_paged_few(const PagedAttnArgs& a, cudaStream_t stream);
+// Any batch (paged_chunk.cu)
+size_t paged_chunk_bytes(int hd);
+cudaError_t launch_paged_chunk(const PagedAttnArgs& a, cudaStream_t stream);
 size_t paged_workspace_bytes(const picoattn_config_t& cfg, int n_seqs);
 
 }  // namespace picoattn

@@ -237,7 +237,8 @@ class PagedBatch:
         ws = abi.lib().picoattn_paged_workspace_size(C.byref(cache.cfg), n)
         if ws == 0:
             raise abi.PicoAttnError(abi.PICOATTN_EUNSUPPORTED, "paged_workspace_size")
-        self.workspace = torch.zeros(ws, dtype=torch.uint8, device=cache.device)
+        self.workspace = torch.empty(ws, dtype=torch.uint8, device=cache.device)
+        self.workspace[:256].zero_()  # its header
         self.ref, self.ws_ptr, self.ws_bytes = C.addressof(self.desc), self.workspace.data_ptr(), ws
 
     def status(self) -> int:
