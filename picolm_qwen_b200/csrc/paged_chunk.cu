@@ -7,8 +7,11 @@
 // two such tiles of one KV head of one sequence; its keys come in tiles of 128
 // rows, gathered page by page by TMA.  Per CTA:
 //   warps 0-3, 4-7  softmax: thread = row = TMEM lane
-//   warp 8          work list and TMA;  warp 9  MMA issue, TMEM
+//   warp 8          work list and TMA;  warps 9, 10  MMA issue for each group
 //   TMEM            S0, S1 (P over the columns it came from), O0, O1
+// Each group's S is two halves of 64 keys that go their own way: while the group
+// takes the softmax of one, the products of the other (P V, then the next tile's
+// Q K^T into the same columns) run, so neither waits out the other's latency.
 // Two-tile blocks: each softmax group has its own rows, K and V tiles serve
 // both, and one group's softmax runs while the other's products do.  One-tile
 // blocks (few new tokens): the groups take alternate key tiles of the same rows
@@ -36,8 +39,8 @@ namespace picoattn {
 
 namespace {
 
-constexpr int BM = 128, BN = 128;
-constexpr int kThreads = 320;
+constexpr int BM = 128, BN = 128, BH = BN / 2;
+constexpr int kThreads = 352;
 constexpr int kPlan = 64;          // threads that add up the sequences' costs
 constexpr int kMaxCtas = 160;
 constexpr int kMinCost = 4;        // least cost per CTA of a slice
@@ -68,6 +71,13 @@ struct Item {
     int len;               // rows of the sequence
     int poison;            // a page that does not exist was met
 };
+
+// The key tiles of an item that softmax group w works on: all of a two-tile
+// block's that its rows see, every other one of a one-tile block's.
+__device__ __forceinline__ int own_tiles(const Item& it, int w, int tq) {
+    if (it.ntok <= tq) return (it.j1 - it.j0 + 1 - w) / 2;
+    return w ? it.j1 - it.j0 : max(0, min(it.j1, (it.pos0 + tq + BN - 1) / BN) - it.j0);
+}
 
 // ---- the work list --------------------------------------------------------------
 
@@ -134,76 +144,73 @@ struct Pair16<__nv_bfloat16> {
     static __device__ __forceinline__ float2 up(V v) { return __bfloat1622float2(v); }
 };
 
-// S (128 fp32 columns at tS, unscaled) -> P = 2^(scale S - m) in 16 bits over its
-// first 64 columns; m (log2 units) and the row sum l updated, O (HD columns at tO)
-// rescaled when m grows.  lim: keys visible to the row counted from the tile's
-// first; mask: some row of the warp does not see all 128.  The maximum is stale
-// by design: p is taken against the running one in the same pass that reads S, and
-// kept unless some p passes 2^15 (exact in 16 bits' range and harmless in the fp32
-// sums); then the tile is done again with its own maximum.
+// S (64 fp32 columns at tS, unscaled) -> P = 2^(scale S - m) in 16 bits over its
+// first 32 columns; m (log2 units) and the row sum l updated, O (HD columns at tO)
+// rescaled when m grows.  lim: keys visible to the row counted from the first;
+// mask: some row of the warp does not see all 64.  The maximum is stale by
+// design: p is taken against the running one in the same pass that reads S, and
+// kept unless some p passes 2^15 (in range in 16 bits and harmless in the fp32
+// sums); then the keys are done again with their own maximum.  wait_prev_pv()
+// returns when the group's products so far are in O.
 template <class T, int HD, class WaitPrevPV>
-__device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, bool first, int lim, bool mask, float scale,
+__device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool first, int lim, bool mask, float scale,
                                              float& m, float& l, WaitPrevPV wait_prev_pv) {
     using P2 = Pair16<T>;
     const uint64_t sc2 = f2_pack(scale, scale);
-    bool done = false;
-    {
-        uint32_t pk[BN / 2];
-        uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
-        typename P2::V top[4] = {P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f)};
-        uint32_t sbuf[2][32];
-        tmem_ld32(tS, sbuf[0]);
-        if (first) {  // start from the maximum of the first 32 columns
-            tmem_ld_wait();
-            float m0 = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 32; e++)
-                if (!mask || e < lim) m0 = fmaxf(m0, __uint_as_float(sbuf[0][e]));
-            m = fmaxf(m0 * scale, kNone);
-        }
+    uint32_t pk[BH / 2], sr[2][32];
+    // p of the keys against m into pk; their sum, and the largest
+    auto p_pass = [&](float& sum, float& top) {
+        uint64_t s2[4] = {0ull, 0ull, 0ull, 0ull};
+        typename P2::V t2[2] = {P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f)};
         const uint64_t nm2 = f2_pack(-m, -m);
 #pragma unroll
-        for (int c = 0; c < BN / 32; c++) {
-            tmem_ld_wait();
-            uint32_t (&sr)[32] = sbuf[c & 1];
-            if (c + 1 < BN / 32) tmem_ld32(tS + (c + 1) * 32, sbuf[(c + 1) & 1]);
+        for (int c = 0; c < 2; c++) {
+            if (c == 1) tmem_ld_wait();
             if (mask) {
 #pragma unroll
                 for (int e = 0; e < 32; e++)
-                    if (c * 32 + e >= lim) sr[e] = __float_as_uint(-INFINITY);
+                    if (c * 32 + e >= lim) sr[c][e] = __float_as_uint(-INFINITY);
             }
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 float d0, d1;
-                f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), sc2, nm2), d0, d1);
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), sc2, nm2), d0,
+                          d1);
                 const float p0 = ex2(d0), p1 = ex2(d1);
-                sum[e & 3] = f2_add(sum[e & 3], f2_pack(p0, p1));
+                s2[e & 3] = f2_add(s2[e & 3], f2_pack(p0, p1));
                 const typename P2::V h = P2::cvt(p0, p1);
-                top[e & 3] = __hmax2(top[e & 3], h);
+                t2[e & 1] = __hmax2(t2[e & 1], h);
                 pk[c * 16 + e] = *reinterpret_cast<const uint32_t*>(&h);
             }
         }
-        const float2 t2 = P2::up(__hmax2(__hmax2(top[0], top[1]), __hmax2(top[2], top[3])));
-        if (!__any_sync(0xffffffffu, !(fmaxf(t2.x, t2.y) <= kStaleMaxP))) {
-            tmem_st32(tS, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
-            tmem_st32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
-            float a0, a1;
-            f2_unpack(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])), a0, a1);
-            l += a0 + a1;
-            done = true;
-        }
+        float a0, a1;
+        f2_unpack(f2_add(f2_add(s2[0], s2[1]), f2_add(s2[2], s2[3])), a0, a1);
+        sum = a0 + a1;
+        const float2 t = P2::up(__hmax2(t2[0], t2[1]));
+        top = fmaxf(t.x, t.y);
+    };
+    tmem_ld32(tS, sr[0]);
+    tmem_ld_wait();
+    tmem_ld32(tS + 32, sr[1]);
+    if (first) {  // start from the maximum of the first 32 keys
+        float m0 = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+            if (!mask || e < lim) m0 = fmaxf(m0, __uint_as_float(sr[0][e]));
+        m = fmaxf(m0 * scale, kNone);
     }
-    if (!done) {
+    float sum, top;
+    p_pass(sum, top);
+    if (__any_sync(0xffffffffu, !(top <= kStaleMaxP))) {
+        tmem_ld32(tS, sr[0]);
+        tmem_ld32(tS + 32, sr[1]);
+        tmem_ld_wait();
         float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < BN / 32; c++) {
-            uint32_t sr[32];
-            tmem_ld32(tS + c * 32, sr);
-            tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int e = 0; e < 32; e++)
-                if (!mask || c * 32 + e < lim) mx = fmaxf(mx, __uint_as_float(sr[e]));
-        }
+                if (!mask || c * 32 + e < lim) mx = fmaxf(mx, __uint_as_float(sr[c][e]));
         const float m_new = fmaxf(mx * scale, first ? kNone : m);
         if (!first) {
             const float corr = ex2(m - m_new);
@@ -222,32 +229,10 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, bool firs
             l *= corr;
         }
         m = m_new;
-        // 32 scores at a time; P of chunk c lands in columns [16c, 16c + 16), already read
-        float s4[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t sbuf[2][32];
-        tmem_ld32(tS, sbuf[0]);
-#pragma unroll
-        for (int c = 0; c < BN / 32; c++) {
-            tmem_ld_wait();
-            uint32_t (&sr)[32] = sbuf[c & 1];
-            if (c + 1 < BN / 32) tmem_ld32(tS + (c + 1) * 32, sbuf[(c + 1) & 1]);
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                float p[2];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const bool seen = !mask || c * 32 + 2 * e + i < lim;
-                    p[i] = seen ? ex2(__fmaf_rn(__uint_as_float(sr[2 * e + i]), scale, -m)) : 0.f;
-                }
-                s4[e & 3] += p[0] + p[1];
-                const typename P2::V h = P2::cvt(p[0], p[1]);
-                pk[e] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            tmem_st16(tS + c * 16, pk);
-        }
-        l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        p_pass(sum, top);
     }
+    tmem_st32(tS, pk);
+    l += sum;
     tmem_st_wait();
 }
 
@@ -283,7 +268,7 @@ struct Smem {
     static constexpr int kStage = kV + NV * kTile;   // 4 KB per softmax warp
     static constexpr int kPlanAt = kStage + 8 * 4096;
     static constexpr int kBars = (kPlanAt + (int)sizeof(Plan) + 15) / 16 * 16;
-    static constexpr int kItems = kBars + 24 * 8;
+    static constexpr int kItems = kBars + 26 * 8;
     static constexpr int kEnd = kItems + 2 * (int)sizeof(Item) + 16;
     static constexpr int kDyn = kEnd + 1024;         // slack to align the base
     static_assert(kDyn <= 227 * 1024, "one CTA per SM");
@@ -307,10 +292,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* k_empty = bars + 8;
     uint64_t* v_full = bars + 10;       // [NV]
     uint64_t* v_empty = bars + 12;
-    uint64_t* s_full = bars + 14;       // [2] per softmax group
-    uint64_t* p_full = bars + 16;
-    uint64_t* pv_done = bars + 18;
-    uint64_t* o_free = bars + 20;
+    uint64_t* s_full = bars + 14;       // [group][half]
+    uint64_t* p_full = bars + 18;       // [group][half]
+    uint64_t* pv_done = bars + 22;      // [2] per softmax group, a phase per half tile
+    uint64_t* o_free = bars + 24;       // [2]
     Plan* plan = reinterpret_cast<Plan*>(smem + L::kPlanAt);
     Item* items = reinterpret_cast<Item*>(smem + L::kItems);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
@@ -319,12 +304,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 3);
-            mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1), mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
-            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&pv_done[i], 1), mbar_init(&o_free[i], 4);
+            mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 4);
+            mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 2);
+            mbar_init(&pv_done[i], 1), mbar_init(&o_free[i], 4);
         }
+        for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
         mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
+        mbar_init(q_empty, 2);
         fence_mbar_init();
         prefetch_tmap(&tmQ);
         prefetch_tmap(&tmK);
@@ -547,118 +533,107 @@ __global__ void __launch_bounds__(kThreads, 1)
                 page = next_page;
             }
         }
-    } else if (warp == 9) {
-        // ---------------- MMA issue ----------------
-        if (lane == 0) {
-            constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
-            constexpr uint32_t idesc_qk = idesc_f16_f32(BM, BN, false, false) | kBf16;
-            constexpr uint32_t idesc_pv = idesc_f16_f32(BM, HD, false, true) | kBf16;
-            const uint64_t dq = smem_desc_sw128(smem_u32(smem + L::kQ), 16, 1024);
-            const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kK), 16, 1024);
-            const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV), L::kBox, 1024);
-            // S of group w from Q tile qt and K stage s
-            auto qk = [&](int w, int qt, int s) {
-                const uint64_t qd = desc_advance(dq, qt * L::kTile), kd = desc_advance(dk, s * L::kTile);
+    } else if (warp >= 9) {
+        // ---------------- MMA issue: one warp per softmax group ----------------
+        // Each waits for what is ready early (V, the next K) while its group is still
+        // busy, so that only P stands between a softmax and its products.
+        const int w = warp - 9;
+        constexpr uint32_t kBf16 = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+        constexpr uint32_t idesc_qk = idesc_f16_f32(BM, BH, false, false) | kBf16;
+        constexpr uint32_t idesc_pv = idesc_f16_f32(BM, HD, false, true) | kBf16;
+        const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
+        const uint64_t dq = smem_desc_sw128(smem_u32(smem + L::kQ), 16, 1024);
+        const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kK), 16, 1024);
+        const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV), L::kBox, 1024);
+        // half y of S from Q tile qt and the K stage of tile t; `last`: the block's last tile of this group
+        auto qk = [&](int qt, int t, int y, bool last) {
+            if (elect_one()) {
+                const uint64_t qd = desc_advance(dq, qt * L::kTile), kd = desc_advance(dk, (t % 2) * L::kTile + y * BH * 128);
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; kk++) {
                     const uint32_t off = (kk >> 2) * L::kBox + (kk & 3) * 32;
-                    umma_ss(tmem + w * 128, desc_advance(qd, off), desc_advance(kd, off), idesc_qk, kk > 0 ? 1u : 0u);
+                    umma_ss(tS + y * BH, desc_advance(qd, off), desc_advance(kd, off), idesc_qk, kk > 0 ? 1u : 0u);
                 }
-                umma_commit(&s_full[w]);
-            };
-            auto pv = [&](int w, int s, bool first) {
-                const uint64_t vd = desc_advance(dv, s * L::kTile);
-#pragma unroll
-                for (int kk = 0; kk < BN / 16; kk++)
-                    umma_ts(tmem + 256 + w * 128, tmem + w * 128 + kk * 8, desc_advance(vd, kk * 16 * 128), idesc_pv,
-                            (!first || kk > 0) ? 1u : 0u);
-                umma_commit(&pv_done[w]);
-            };
-            auto wait = [&](uint64_t* bar, int phase) {
-                if (!mbar_test(bar, (uint32_t)(phase & 1))) mbar_wait(bar, (uint32_t)(phase & 1), status);
-            };
-            int t = 0, tiles[2] = {0, 0}, uses[2] = {0, 0};  // key tiles; each group's tiles and blocks so far
-            for (int k = 0;; k++) {
-                const int slot = k & 1;
-                mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
-                const Item it = items[slot];
-                mbar_arrive(&item_empty[slot]);
-                if (it.b < 0) break;
-                const int n = it.j1 - it.j0;
-                wait(q_full, k);
-                if (it.ntok > tq) {
-                    // two Q tiles; group 0's keys may end before the block's
-                    const int n0 = min(it.j1, (it.pos0 + tq + BN - 1) / BN) - it.j0;
-                    wait(&k_full[t % 2], t / 2);
-                    tc_fence_after();
-                    if (n0 > 0) qk(0, 0, t % 2);
-                    qk(1, 1, t % 2);
+                umma_commit(&s_full[2 * w + y]);
+                if (y) {
                     umma_commit(&k_empty[t % 2]);
-                    if (n == 1) umma_commit(q_empty);
-                    for (int j = 0; j < n; j++, t++) {
-                        const bool more = j + 1 < n;
-#pragma unroll
-                        for (int w = 0; w < 2; w++) {
-                            const int nw = w ? n : n0;
-                            if (j < nw) {
-                                const bool need_o = j == 0 && uses[w] > 0, kw = j + 1 < nw;
-                                bool ok = mbar_test(&p_full[w], (uint32_t)(tiles[w] & 1)) &
-                                          mbar_test(&v_full[t % 2], (uint32_t)((t / 2) & 1));
-                                if (need_o) ok &= mbar_test(&o_free[w], (uint32_t)((uses[w] - 1) & 1));
-                                if (kw) ok &= mbar_test(&k_full[(t + 1) % 2], (uint32_t)(((t + 1) / 2) & 1));
-                                if (!ok) {
-                                    mbar_wait(&p_full[w], (uint32_t)(tiles[w] & 1), status);
-                                    mbar_wait(&v_full[t % 2], (uint32_t)((t / 2) & 1), status);
-                                    if (need_o) mbar_wait(&o_free[w], (uint32_t)((uses[w] - 1) & 1), status);
-                                    if (kw) mbar_wait(&k_full[(t + 1) % 2], (uint32_t)(((t + 1) / 2) & 1), status);
-                                }
-                                tc_fence_after();
-                                pv(w, t % 2, j == 0);
-                                if (kw) qk(w, w, (t + 1) % 2);
-                                tiles[w]++;
-                            }
-                        }
-                        umma_commit(&v_empty[t % 2]);
-                        if (more) {
-                            umma_commit(&k_empty[(t + 1) % 2]);
-                            if (j + 2 == n) umma_commit(q_empty);
-                        }
-                    }
-                    if (n0 > 0) uses[0]++;
-                    uses[1]++;
-                } else {
-                    // one Q tile: the groups take alternate key tiles
-                    for (int j = 0; j < min(n, 2); j++) {
-                        wait(&k_full[(t + j) % 2], (t + j) / 2);
-                        tc_fence_after();
-                        qk(j, 0, (t + j) % 2);
-                        umma_commit(&k_empty[(t + j) % 2]);
-                        if (j + 1 == n) umma_commit(q_empty);
-                    }
-                    for (int j = 0; j < n; j++, t++) {
-                        const int w = j & 1;
-                        const bool need_o = j < 2 && uses[w] > 0, more = j + 2 < n;
-                        wait(&p_full[w], tiles[w]);
-                        wait(&v_full[t % 2], t / 2);
-                        if (need_o) wait(&o_free[w], uses[w] - 1);
-                        tc_fence_after();
-                        pv(w, t % 2, j < 2);
-                        umma_commit(&v_empty[t % 2]);
-                        tiles[w]++;
-                        if (more) {
-                            wait(&k_full[t % 2], (t + 2) / 2);
-                            tc_fence_after();
-                            qk(w, 0, t % 2);
-                            umma_commit(&k_empty[t % 2]);
-                            if (j + 3 == n) umma_commit(q_empty);
-                        }
-                    }
-                    uses[0]++;
-                    if (n > 1) uses[1]++;
+                    if (last) umma_commit(q_empty);
                 }
             }
+            __syncwarp();
+        };
+        auto pv = [&](int t, int y, bool first) {
+            if (elect_one()) {
+                const uint64_t vd = desc_advance(dv, (t % 2) * L::kTile + y * BH * 128);
+#pragma unroll
+                for (int kk = 0; kk < BH / 16; kk++)
+                    umma_ts(tO, tS + y * BH + kk * 8, desc_advance(vd, kk * 16 * 128), idesc_pv,
+                            (!first || kk > 0) ? 1u : 0u);
+                umma_commit(&pv_done[w]);
+                if (y) umma_commit(&v_empty[t % 2]);
+            }
+            __syncwarp();
+        };
+        auto wait = [&](uint64_t* bar, int phase) { mbar_wait(bar, (uint32_t)(phase & 1), status); };
+        int t = 0, mine = 0, uses = 0;  // key tiles of the CTA, of this group; blocks this group worked on
+        for (int k = 0;; k++) {
+            const int slot = k & 1;
+            wait(&item_full[slot], k >> 1);
+            const Item it = items[slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[slot]);
+            if (it.b < 0) break;
+            const int n = it.j1 - it.j0;
+            const bool two = it.ntok > tq;
+            // this group's tiles: first, step, count (group 0's keys may end before a two-tile block's)
+            const int step = two ? 1 : 2, j0 = two ? 0 : w;
+            const int own = own_tiles(it, w, tq);
+            wait(q_full, k);
+            if (own > 0) {
+                wait(&k_full[(t + j0) % 2], (t + j0) / 2);
+                tc_fence_after();
+                for (int y = 0; y < 2; y++) qk(two ? w : 0, t + j0, y, own == 1);
+            } else if (lane == 0) {
+                mbar_arrive(q_empty);
+            }
+            // tiles of the other group alone are none of this one's business
+            auto pass = [&](int j, bool of_k) {
+                if (lane == 0) mbar_arrive(of_k ? &k_empty[(t + j) % 2] : &v_empty[(t + j) % 2]);
+            };
+            int i = 0;
+            for (int j = 0; j < n; j++) {
+                const bool use = i < own && j == j0 + i * step;
+                if (!use) {
+                    // released once the tile is there, so that its stage's phases go round one by one
+                    wait(&k_full[(t + j) % 2], (t + j) / 2);
+                    pass(j, true);
+                    wait(&v_full[(t + j) % 2], (t + j) / 2);
+                    pass(j, false);
+                    continue;
+                }
+                wait(&v_full[(t + j) % 2], (t + j) / 2);
+                const bool more = i + 1 < own;
+                if (more && step == 1) wait(&k_full[(t + j + 1) % 2], (t + j + 1) / 2);
+                if (i == 0 && uses > 0) wait(&o_free[w], uses - 1);
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    wait(&p_full[2 * w + y], mine);
+                    tc_fence_after();
+                    pv(t + j, y, i == 0 && y == 0);
+                    if (more) {
+                        if (step == 2 && y == 0) {
+                            wait(&k_full[(t + j + 2) % 2], (t + j + 2) / 2);
+                            tc_fence_after();
+                        }
+                        qk(two ? w : 0, t + j + step, y, i + 2 == own);
+                    }
+                }
+                mine++;
+                i++;
+            }
+            t += n;
+            if (own > 0) uses++;
         }
-        __syncwarp();
     } else {
         // ---------------- softmax ----------------
         const int w = warp >> 2, r = tid & 127;
@@ -681,31 +656,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the fewest and most keys that valid rows of this warp see (rows are token-major)
             const bool live = __any_sync(0xffffffffu, valid);
             const int lim_lo = __reduce_min_sync(0xffffffffu, valid ? lim : 0x7fffffff);
-            const int n_own = !two ? (n + 1 - w) / 2
-                                   : (w ? n : max(0, min(it.j1, (it.pos0 + tq + BN - 1) / BN) - it.j0));
+            const int n_own = own_tiles(it, w, tq);
             float m = kNone, l = 0.f;
             for (int i = 0; i < n_own; i++, mine++) {
                 const int j = two ? i : 2 * i + w, base = (it.j0 + j) * BN;
-                mbar_wait(&s_full[w], (uint32_t)(mine & 1), status);
-                tc_fence_after();
-                if (live)
-                    softmax_tile<T, HD>(tS, tO, i == 0, lim - base, base + BN > lim_lo, scale, m, l,
-                                        [&] { mbar_wait(&pv_done[w], (uint32_t)((mine - 1) & 1), status); });
-                if (base + BN > it.len) {
-                    // rows past the sequence hold anything: their V must not meet the zero weights as a NaN
-                    const int s = (t + j) % 2;
-                    mbar_wait(&v_full[s], (uint32_t)(((t + j) / 2) & 1), status);
-                    for (int e = r; e < BN * 8 * (HD / 64); e += 128) {
-                        const int row = (e >> 3) & (BN - 1), x = e >> 10;
-                        if (base + row >= it.len)
-                            *reinterpret_cast<uint4*>(smem + L::kV + s * L::kTile + x * L::kBox + row * 128 + (e & 7) * 16) =
-                                make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+                for (int y = 0; y < 2; y++) {
+                    mbar_wait(&s_full[2 * w + y], (uint32_t)(mine & 1), status);
+                    tc_fence_after();
+                    const int hb = base + y * BH;
+                    // phase of the products before this half's: 2 mine + y - 1
+                    if (live)
+                        softmax_half<T, HD>(tS + y * BH, tO, i == 0 && y == 0, lim - hb, hb + BH > lim_lo, scale, m, l,
+                                            [&] { mbar_wait(&pv_done[w], (uint32_t)((y + 1) & 1), status); });
+                    if (y == 0 && base + BN > it.len) {
+                        // rows past the sequence hold anything: their V must not meet the zero weights as a NaN
+                        const int s = (t + j) % 2;
+                        mbar_wait(&v_full[s], (uint32_t)(((t + j) / 2) & 1), status);
+                        for (int e = r; e < BN * 8 * (HD / 64); e += 128) {
+                            const int row = (e >> 3) & (BN - 1), x = e >> 10;
+                            if (base + row >= it.len)
+                                *reinterpret_cast<uint4*>(smem + L::kV + s * L::kTile + x * L::kBox + row * 128 +
+                                                          (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_shared();
                     }
-                    fence_proxy_async_shared();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * w + y]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[w]);
             }
             t += n;
             // the items' last tile has been read: its poison flag is final
@@ -713,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             named_bar_sync(1 + w, 128);  // every warp of the group has read the item
             if (r == 0) mbar_arrive(&item_empty[slot]);
             if (n_own > 0) {
-                mbar_wait(&pv_done[w], (uint32_t)((mine - 1) & 1), status);
+                mbar_wait(&pv_done[w], 1u, status);  // an odd phase: a tile's second half
                 tc_fence_after();
             }
             const bool join = !two && n > 1;

@@ -16,6 +16,16 @@
 
 namespace picoattn {
 
+// One lane of a converged warp, the same at every call: a warp that takes its
+// decisions together and lets this lane issue keeps descriptors in uniform
+// registers (measured per tcgen05.mma: 30 cycles to issue so, 50 to 60 from a
+// branch that one lane runs alone; the tensor core takes 64).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // ---- tiled TMA ---------------------------------------------------------------
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
