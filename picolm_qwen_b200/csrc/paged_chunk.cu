@@ -7,7 +7,8 @@
 // two such tiles of one KV head of one sequence; its keys come in tiles of 128
 // rows, gathered page by page by TMA.  Per CTA:
 //   warps 0-3, 4-7  softmax: thread = row = TMEM lane
-//   warp 8          work list and TMA;  warps 9, 10  MMA issue for each group
+//   warp 8          work list, TMA of Q and K;  warp 11  TMA of V
+//   warps 9, 10     MMA issue for each group
 //   TMEM            S0, S1 (P over the columns it came from), O0, O1
 // Each group's S is two halves of 64 keys that go their own way: while the group
 // takes the softmax of one, the products of the other (P V, then the next tile's
@@ -40,14 +41,15 @@ namespace picoattn {
 namespace {
 
 constexpr int BM = 128, BN = 128, BH = BN / 2;
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;
 constexpr int kPlan = 64;          // threads that add up the sequences' costs
 constexpr int kMaxCtas = 160;
-constexpr int kMinCost = 4;        // least cost per CTA of a slice
-constexpr int kSliceOverhead = 12; // what cutting blocks costs, in the same unit (measured, see launch)
+constexpr int kMinCost = 12;       // least cost per CTA of a slice
+constexpr int kSliceOverhead = 24; // what cutting blocks costs, in the same unit (measured, see launch)
 constexpr int kPartRows = 2 * BM;
+constexpr int kRing = 4;           // stages of 64 keys, K and V each
 constexpr float kNone = -1e30f;    // running maximum before any key
-constexpr float kStaleMaxP = 32768.0f;
+constexpr float kStaleSum = 32768.0f;
 
 struct ChunkMeta {  // the cut block whose first part a CTA holds (nt 0: none)
     int b, h, blk, nt, slices;
@@ -86,7 +88,8 @@ struct Blocks {
     int tq;
     __device__ __forceinline__ int ntok(int i) const { return min(per, n - i * per); }
     __device__ __forceinline__ int tiles(int i) const { return (len - n + min(n, (i + 1) * per) + BN - 1) / BN; }
-    __device__ __forceinline__ int unit(int i) const { return ntok(i) > tq ? 2 : 1; }
+    // cost of a key tile: a two-tile block's takes some 3,500 cycles, a one-tile block's 2,600
+    __device__ __forceinline__ int unit(int i) const { return ntok(i) > tq ? 4 : 3; }
 };
 
 __device__ __forceinline__ Blocks seq_blocks(const ChunkArgs& c, int b) {
@@ -135,13 +138,11 @@ template <>
 struct Pair16<__half> {
     using V = __half2;
     static __device__ __forceinline__ V cvt(float a, float b) { return __floats2half2_rn(a, b); }
-    static __device__ __forceinline__ float2 up(V v) { return __half22float2(v); }
 };
 template <>
 struct Pair16<__nv_bfloat16> {
     using V = __nv_bfloat162;
     static __device__ __forceinline__ V cvt(float a, float b) { return __floats2bfloat162_rn(a, b); }
-    static __device__ __forceinline__ float2 up(V v) { return __bfloat1622float2(v); }
 };
 
 // S (64 fp32 columns at tS, unscaled) -> P = 2^(scale S - m) in 16 bits over its
@@ -149,8 +150,8 @@ struct Pair16<__nv_bfloat16> {
 // rescaled when m grows.  lim: keys visible to the row counted from the first;
 // mask: some row of the warp does not see all 64.  The maximum is stale by
 // design: p is taken against the running one in the same pass that reads S, and
-// kept unless some p passes 2^15 (in range in 16 bits and harmless in the fp32
-// sums); then the keys are done again with their own maximum.  wait_prev_pv()
+// kept unless the sum passes 2^15 (so that every p is in range in 16 bits); then
+// the keys are done again with their own maximum.  wait_prev_pv()
 // returns when the group's products so far are in O.
 template <class T, int HD, class WaitPrevPV>
 __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool first, int lim, bool mask, float scale,
@@ -158,10 +159,9 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool firs
     using P2 = Pair16<T>;
     const uint64_t sc2 = f2_pack(scale, scale);
     uint32_t pk[BH / 2], sr[2][32];
-    // p of the keys against m into pk; their sum, and the largest
-    auto p_pass = [&](float& sum, float& top) {
+    // p of the keys against m into pk; returns their sum
+    auto p_pass = [&] {
         uint64_t s2[4] = {0ull, 0ull, 0ull, 0ull};
-        typename P2::V t2[2] = {P2::cvt(0.f, 0.f), P2::cvt(0.f, 0.f)};
         const uint64_t nm2 = f2_pack(-m, -m);
 #pragma unroll
         for (int c = 0; c < 2; c++) {
@@ -179,15 +179,12 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool firs
                 const float p0 = ex2(d0), p1 = ex2(d1);
                 s2[e & 3] = f2_add(s2[e & 3], f2_pack(p0, p1));
                 const typename P2::V h = P2::cvt(p0, p1);
-                t2[e & 1] = __hmax2(t2[e & 1], h);
                 pk[c * 16 + e] = *reinterpret_cast<const uint32_t*>(&h);
             }
         }
         float a0, a1;
         f2_unpack(f2_add(f2_add(s2[0], s2[1]), f2_add(s2[2], s2[3])), a0, a1);
-        sum = a0 + a1;
-        const float2 t = P2::up(__hmax2(t2[0], t2[1]));
-        top = fmaxf(t.x, t.y);
+        return a0 + a1;
     };
     tmem_ld32(tS, sr[0]);
     tmem_ld_wait();
@@ -199,9 +196,8 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool firs
             if (!mask || e < lim) m0 = fmaxf(m0, __uint_as_float(sr[0][e]));
         m = fmaxf(m0 * scale, kNone);
     }
-    float sum, top;
-    p_pass(sum, top);
-    if (__any_sync(0xffffffffu, !(top <= kStaleMaxP))) {
+    float sum = p_pass();
+    if (__any_sync(0xffffffffu, !(sum <= kStaleSum))) {
         tmem_ld32(tS, sr[0]);
         tmem_ld32(tS + 32, sr[1]);
         tmem_ld_wait();
@@ -229,11 +225,66 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool firs
             l *= corr;
         }
         m = m_new;
-        p_pass(sum, top);
+        sum = p_pass();
     }
     tmem_st32(tS, pk);
     l += sum;
     tmem_st_wait();
+}
+
+template <int HD>
+struct Smem {
+    static constexpr int kBox = BM * 128;            // 128 rows x 64 columns of 16 bits
+    static constexpr int kTile = (HD / 64) * kBox;
+    static constexpr int kHalf = (HD / 64) * BH * 128;  // a ring stage: 64 keys, HD / 64 boxes of 8 KB
+    static constexpr int kHBox = BH * 128;
+    static constexpr int kQ = 0;
+    static constexpr int kK = 2 * kTile;
+    static constexpr int kV = kK + kRing * kHalf;
+    static constexpr int kStage = kV + kRing * kHalf;   // 4 KB per softmax warp
+    static constexpr int kPlanAt = kStage + 8 * 4096;
+    static constexpr int kBars = (kPlanAt + (int)sizeof(Plan) + 15) / 16 * 16;
+    static constexpr int kItems = kBars + 36 * 8;
+    static constexpr int kEnd = kItems + 2 * (int)sizeof(Item) + 16;
+    static constexpr int kDyn = kEnd + 1024;         // slack to align the base
+    static_assert(kDyn <= 227 * 1024, "one CTA per SM");
+};
+
+// The pages of an item's key tiles into a ring of half tiles (64 rows x HD as
+// HD / 64 boxes of 128-byte rows), by one warp: a lane per box and page.  t: half
+// tiles that the ring has seen.
+template <int HD>
+__device__ __forceinline__ void load_tiles(const PagedAttnArgs& a, const CUtensorMap& map, Item& item, uint8_t* ring,
+                                           uint64_t* full, uint64_t* empty, int t, unsigned int* status, int lane) {
+    using L = Smem<HD>;
+    const int rows = min(a.b.page_size, BH), boxes = BH / rows;  // rows of a box, boxes of a half's column group
+    const int col = lane / boxes, box = lane % boxes;
+    const bool mine = col < HD / 64;
+    const int b = item.b, h = item.h, len = item.len, last = 2 * item.j1;
+    const int* table = a.b.page_table + (size_t)b * a.b.page_cols;
+    auto page_of = [&](int y) {  // of this lane's box of half tile y; -1: none, -2: no such page
+        const int r = y * BH + box * rows;
+        if (!mine || y >= last || r >= len) return -1;
+        const int p = table[r >> a.b.page_shift];
+        return p < 0 || p >= a.b.n_pages ? -2 : p;
+    };
+    int page = page_of(2 * item.j0);
+    for (int y = 2 * item.j0; y < last; y++, t++) {
+        const int next = page_of(y + 1), s = t % kRing, use = t / kRing;
+        const int r = y * BH + box * rows;
+        const int at = (max(page, 0) * a.hkv + h) * a.b.page_size + (r & (a.b.page_size - 1));
+        if (__any_sync(0xffffffffu, page == -2) && lane == 0) {
+            atomicOr(status, PICOATTN_DEV_BAD_PAGE);
+            item.poison = 1;
+        }
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, page != -1));
+        if (use > 0) mbar_wait(&empty[s], (uint32_t)((use - 1) & 1), status);
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], n * (uint32_t)rows * 128u);
+        __syncwarp();
+        if (page != -1)
+            tma_load_2d(ring + s * L::kHalf + col * L::kHBox + box * rows * 128, &map, 64 * col, at, &full[s]);
+        page = next;
+    }
 }
 
 // ---- output ------------------------------------------------------------------------
@@ -257,23 +308,6 @@ __device__ __forceinline__ void store_rows(const uint32_t (&w)[32], uint4* stage
 
 // ---- the kernel --------------------------------------------------------------------
 
-template <int HD>
-struct Smem {
-    static constexpr int kBox = BM * 128;            // 128 rows x 64 columns of 16 bits
-    static constexpr int kTile = (HD / 64) * kBox;
-    static constexpr int NK = 2, NV = 2;
-    static constexpr int kQ = 0;
-    static constexpr int kK = 2 * kTile;
-    static constexpr int kV = kK + NK * kTile;
-    static constexpr int kStage = kV + NV * kTile;   // 4 KB per softmax warp
-    static constexpr int kPlanAt = kStage + 8 * 4096;
-    static constexpr int kBars = (kPlanAt + (int)sizeof(Plan) + 15) / 16 * 16;
-    static constexpr int kItems = kBars + 26 * 8;
-    static constexpr int kEnd = kItems + 2 * (int)sizeof(Item) + 16;
-    static constexpr int kDyn = kEnd + 1024;         // slack to align the base
-    static_assert(kDyn <= 227 * 1024, "one CTA per SM");
-};
-
 template <class T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -288,14 +322,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* item_empty = bars + 2;    // [2]
     uint64_t* q_full = bars + 4;
     uint64_t* q_empty = bars + 5;
-    uint64_t* k_full = bars + 6;        // [NK]
-    uint64_t* k_empty = bars + 8;
-    uint64_t* v_full = bars + 10;       // [NV]
-    uint64_t* v_empty = bars + 12;
-    uint64_t* s_full = bars + 14;       // [group][half]
-    uint64_t* p_full = bars + 18;       // [group][half]
-    uint64_t* pv_done = bars + 22;      // [2] per softmax group, a phase per half tile
-    uint64_t* o_free = bars + 24;       // [2]
+    uint64_t* s_full = bars + 6;        // [group][half]
+    uint64_t* p_full = bars + 10;       // [group][half]
+    uint64_t* pv_done = bars + 14;      // [2] per softmax group, a phase per half tile
+    uint64_t* o_free = bars + 16;       // [2]
+    uint64_t* k_full = bars + 18;       // [kRing], each
+    uint64_t* k_empty = k_full + kRing;
+    uint64_t* v_full = k_empty + kRing;
+    uint64_t* v_empty = v_full + kRing;
     Plan* plan = reinterpret_cast<Plan*>(smem + L::kPlanAt);
     Item* items = reinterpret_cast<Item*>(smem + L::kItems);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
@@ -304,11 +338,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 4);
-            mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 2), mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 2);
+            mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 5);
             mbar_init(&pv_done[i], 1), mbar_init(&o_free[i], 4);
         }
         for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+        for (int i = 0; i < kRing; i++) {
+            mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 2);
+            mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 2);
+        }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 2);
         fence_mbar_init();
@@ -332,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const Blocks x = seq_blocks(c, b);
             my_cost += head_cost(x) * a.hkv;
             my_items += x.count * a.hkv;
-            if (x.count) my_max = max(my_max, x.tiles(x.count - 1) * 2);
+            if (x.count) my_max = max(my_max, x.tiles(x.count - 1) * 4);
         }
         plan->first_cost[tid + 1] = my_cost;
         plan->first_item[tid + 1] = my_items;
@@ -388,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = a.g, tq = c.tq;
 
     if (warp == 8) {
-        // ---------------- work list and TMA ----------------
+        // ---------------- work list, TMA of Q and K ----------------
         const int slices = plan->slices;
         Walk wk{};
         wk.open = false;
@@ -477,8 +514,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             return false;
         };
-        const int box_rows = min(a.b.page_size, BN), boxes = BN / box_rows;
-        const int half = (lane / boxes) % (HD / 64), kv = lane / (boxes * (HD / 64)), box = lane % boxes;
         int t = 0;
         for (int k = 0;; k++) {
             const int slot = k & 1;
@@ -501,39 +536,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tma_load_3d(smem + L::kQ + w * L::kTile + x * L::kBox, &tmQ, 64 * x, it.h * g, it.tok0 + w * tq,
                                     q_full);
             }
-            const int* table = a.b.page_table + (size_t)it.b * a.b.page_cols;
-            auto page_of = [&](int j) {  // this lane's box of tile j: its page, -1: none, -2: no such page
-                const int r = j * BN + box * box_rows;
-                if (kv > 1 || j >= it.j1 || r >= it.len) return -1;
-                const int p = table[r >> a.b.page_shift];
-                return p < 0 || p >= a.b.n_pages ? -2 : p;
-            };
-            int page = page_of(it.j0);
-            for (int j = it.j0; j < it.j1; j++, t++) {
-                const int next_page = page_of(j + 1);
-                const int r = j * BN + box * box_rows;
-                const int y = ((max(page, 0) * a.hkv + it.h) * a.b.page_size) + (r & (a.b.page_size - 1));
-                const bool any_bad = __any_sync(0xffffffffu, page == -2);
-                const uint32_t n_boxes = __popc(__ballot_sync(0xffffffffu, page != -1 && kv == 0));
-                if (any_bad && lane == 0) {
-                    atomicOr(status, PICOATTN_DEV_BAD_PAGE);
-                    items[slot].poison = 1;
-                }
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int s = t % 2, use = t / 2;
-                    uint64_t* full = i ? &v_full[s] : &k_full[s];
-                    if (use > 0) mbar_wait(i ? &v_empty[s] : &k_empty[s], (uint32_t)((use - 1) & 1), status);
-                    if (lane == 0) mbar_arrive_expect_tx(full, n_boxes * (uint32_t)box_rows * 128u);
-                    __syncwarp();
-                    if (page != -1 && kv == i)
-                        tma_load_2d(smem + (i ? L::kV : L::kK) + s * L::kTile + half * L::kBox + box * box_rows * 128,
-                                    i ? &tmV : &tmK, 64 * half, y, full);
-                }
-                page = next_page;
-            }
+            load_tiles<HD>(a, tmK, items[slot], smem + L::kK, k_full, k_empty, t, status, lane);
+            t += 2 * (it.j1 - it.j0);
         }
-    } else if (warp >= 9) {
+    } else if (warp == 11) {
+        // ---------------- TMA of V ----------------
+        int t = 0;
+        for (int k = 0;; k++) {
+            const int slot = k & 1;
+            mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
+            const int b = items[slot].b, n = items[slot].j1 - items[slot].j0;
+            if (b >= 0) load_tiles<HD>(a, tmV, items[slot], smem + L::kV, v_full, v_empty, t, status, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[slot]);
+            if (b < 0) break;
+            t += 2 * n;
+        }
+    } else if (warp >= 8) {
         // ---------------- MMA issue: one warp per softmax group ----------------
         // Each waits for what is ready early (V, the next K) while its group is still
         // busy, so that only P stands between a softmax and its products.
@@ -544,38 +563,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tS = tmem + w * 128, tO = tmem + 256 + w * 128;
         const uint64_t dq = smem_desc_sw128(smem_u32(smem + L::kQ), 16, 1024);
         const uint64_t dk = smem_desc_sw128(smem_u32(smem + L::kK), 16, 1024);
-        const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV), L::kBox, 1024);
-        // half y of S from Q tile qt and the K stage of tile t; `last`: the block's last tile of this group
-        auto qk = [&](int qt, int t, int y, bool last) {
+        const uint64_t dv = smem_desc_sw128(smem_u32(smem + L::kV), L::kHBox, 1024);
+        // half y of S from Q tile qt and half tile c of the ring; `last`: the block's last of this
+        // group.  A ring stage is free after two arrivals: one of each group, or both of the only
+        // group that uses it (`alone`)
+        auto qk = [&](int qt, int c, int y, bool alone, bool last) {
             if (elect_one()) {
-                const uint64_t qd = desc_advance(dq, qt * L::kTile), kd = desc_advance(dk, (t % 2) * L::kTile + y * BH * 128);
+                const uint64_t qd = desc_advance(dq, qt * L::kTile), kd = desc_advance(dk, (c % kRing) * L::kHalf);
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; kk++) {
-                    const uint32_t off = (kk >> 2) * L::kBox + (kk & 3) * 32;
-                    umma_ss(tS + y * BH, desc_advance(qd, off), desc_advance(kd, off), idesc_qk, kk > 0 ? 1u : 0u);
-                }
+                for (int kk = 0; kk < HD / 16; kk++)
+                    umma_ss(tS + y * BH, desc_advance(qd, (kk >> 2) * L::kBox + (kk & 3) * 32),
+                            desc_advance(kd, (kk >> 2) * L::kHBox + (kk & 3) * 32), idesc_qk, kk > 0 ? 1u : 0u);
                 umma_commit(&s_full[2 * w + y]);
-                if (y) {
-                    umma_commit(&k_empty[t % 2]);
-                    if (last) umma_commit(q_empty);
-                }
+                umma_commit(&k_empty[c % kRing]);
+                if (alone) umma_commit(&k_empty[c % kRing]);
+                if (last) umma_commit(q_empty);
             }
             __syncwarp();
         };
-        auto pv = [&](int t, int y, bool first) {
+        auto pv = [&](int c, int y, bool alone, bool first) {
             if (elect_one()) {
-                const uint64_t vd = desc_advance(dv, (t % 2) * L::kTile + y * BH * 128);
+                const uint64_t vd = desc_advance(dv, (c % kRing) * L::kHalf);
 #pragma unroll
                 for (int kk = 0; kk < BH / 16; kk++)
                     umma_ts(tO, tS + y * BH + kk * 8, desc_advance(vd, kk * 16 * 128), idesc_pv,
                             (!first || kk > 0) ? 1u : 0u);
                 umma_commit(&pv_done[w]);
-                if (y) umma_commit(&v_empty[t % 2]);
+                umma_commit(&v_empty[c % kRing]);
+                if (alone) umma_commit(&v_empty[c % kRing]);
             }
             __syncwarp();
         };
         auto wait = [&](uint64_t* bar, int phase) { mbar_wait(bar, (uint32_t)(phase & 1), status); };
-        int t = 0, mine = 0, uses = 0;  // key tiles of the CTA, of this group; blocks this group worked on
+        int t = 0, mine = 0, uses = 0;  // half tiles of the CTA; tiles of this group; blocks this group worked on
         for (int k = 0;; k++) {
             const int slot = k & 1;
             wait(&item_full[slot], k >> 1);
@@ -585,53 +605,51 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (it.b < 0) break;
             const int n = it.j1 - it.j0;
             const bool two = it.ntok > tq;
-            // this group's tiles: first, step, count (group 0's keys may end before a two-tile block's)
-            const int step = two ? 1 : 2, j0 = two ? 0 : w;
-            const int own = own_tiles(it, w, tq);
+            // this group's tiles j0 + i step, i < own, and from which tile on they are its alone
+            // (group 0's keys may end before a two-tile block's)
+            const int qt = two ? w : 0, step = two ? 1 : 2, j0 = two ? 0 : w;
+            const int own = own_tiles(it, w, tq), solo = two ? (w ? own_tiles(it, 0, tq) : n) : 0;
             wait(q_full, k);
             if (own > 0) {
-                wait(&k_full[(t + j0) % 2], (t + j0) / 2);
-                tc_fence_after();
-                for (int y = 0; y < 2; y++) qk(two ? w : 0, t + j0, y, own == 1);
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const int c = t + 2 * j0 + y;
+                    wait(&k_full[c % kRing], c / kRing);
+                    tc_fence_after();
+                    qk(qt, c, y, j0 >= solo, own == 1 && y == 1);
+                }
             } else if (lane == 0) {
                 mbar_arrive(q_empty);
             }
-            // tiles of the other group alone are none of this one's business
-            auto pass = [&](int j, bool of_k) {
-                if (lane == 0) mbar_arrive(of_k ? &k_empty[(t + j) % 2] : &v_empty[(t + j) % 2]);
-            };
-            int i = 0;
-            for (int j = 0; j < n; j++) {
-                const bool use = i < own && j == j0 + i * step;
-                if (!use) {
-                    // released once the tile is there, so that its stage's phases go round one by one
-                    wait(&k_full[(t + j) % 2], (t + j) / 2);
-                    pass(j, true);
-                    wait(&v_full[(t + j) % 2], (t + j) / 2);
-                    pass(j, false);
-                    continue;
-                }
-                wait(&v_full[(t + j) % 2], (t + j) / 2);
+            for (int i = 0; i < own; i++, mine++) {
+                const int j = j0 + i * step;
                 const bool more = i + 1 < own;
-                if (more && step == 1) wait(&k_full[(t + j + 1) % 2], (t + j + 1) / 2);
-                if (i == 0 && uses > 0) wait(&o_free[w], uses - 1);
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
-                    wait(&p_full[2 * w + y], mine);
+                    const int c = t + 2 * j + y, cn = c + 2 * step;
+                    if (i == 0 && y == 0 && uses > 0) wait(&o_free[w], uses - 1);
+                    // all at once: a probe of a finished phase costs some 110 cycles, and the tensor
+                    // pipe may stand still meanwhile
+                    const bool now = mbar_test(&v_full[c % kRing], (uint32_t)((c / kRing) & 1)) &
+                                     (!(more && two) || mbar_test(&k_full[cn % kRing], (uint32_t)((cn / kRing) & 1))) &
+                                     mbar_test(&p_full[2 * w + y], (uint32_t)(mine & 1));
+                    if (!now) {
+                        wait(&v_full[c % kRing], c / kRing);
+                        if (more && two) wait(&k_full[cn % kRing], cn / kRing);
+                        wait(&p_full[2 * w + y], mine);
+                    }
                     tc_fence_after();
-                    pv(t + j, y, i == 0 && y == 0);
+                    pv(c, y, j >= solo, i == 0 && y == 0);
                     if (more) {
-                        if (step == 2 && y == 0) {
-                            wait(&k_full[(t + j + 2) % 2], (t + j + 2) / 2);
+                        if (!two) {
+                            wait(&k_full[cn % kRing], cn / kRing);
                             tc_fence_after();
                         }
-                        qk(two ? w : 0, t + j + step, y, i + 2 == own);
+                        qk(qt, cn, y, j + step >= solo, i + 2 == own && y == 1);
                     }
                 }
-                mine++;
-                i++;
             }
-            t += n;
+            t += 2 * n;
             if (own > 0) uses++;
         }
     } else {
@@ -642,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint4* stage = reinterpret_cast<uint4*>(smem + L::kStage + warp * 4096);
         float2* xs = reinterpret_cast<float2*>(smem + L::kStage + 4 * 4096);  // group 1's (max, sum), one-tile blocks
         const int rt = r / g, rh = r - rt * g;  // the row's token in its tile, and head
-        int t = 0, mine = 0;  // key tiles of the CTA, of this group
+        int t = 0, mine = 0;  // half tiles of the CTA, key tiles of this group
         for (int k = 0;; k++) {
             const int slot = k & 1;
             mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
@@ -669,14 +687,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (live)
                         softmax_half<T, HD>(tS + y * BH, tO, i == 0 && y == 0, lim - hb, hb + BH > lim_lo, scale, m, l,
                                             [&] { mbar_wait(&pv_done[w], (uint32_t)((y + 1) & 1), status); });
-                    if (y == 0 && base + BN > it.len) {
+                    if (hb + BH > it.len) {
                         // rows past the sequence hold anything: their V must not meet the zero weights as a NaN
-                        const int s = (t + j) % 2;
-                        mbar_wait(&v_full[s], (uint32_t)(((t + j) / 2) & 1), status);
-                        for (int e = r; e < BN * 8 * (HD / 64); e += 128) {
-                            const int row = (e >> 3) & (BN - 1), x = e >> 10;
-                            if (base + row >= it.len)
-                                *reinterpret_cast<uint4*>(smem + L::kV + s * L::kTile + x * L::kBox + row * 128 +
+                        const int cc = t + 2 * j + y, s = cc % kRing;
+                        mbar_wait(&v_full[s], (uint32_t)((cc / kRing) & 1), status);
+                        for (int e = r; e < BH * 8 * (HD / 64); e += 128) {
+                            const int row = (e >> 3) & (BH - 1), x = e >> 9;
+                            if (hb + row >= it.len)
+                                *reinterpret_cast<uint4*>(smem + L::kV + s * L::kHalf + x * L::kHBox + row * 128 +
                                                           (e & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
                         fence_proxy_async_shared();
@@ -686,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) mbar_arrive(&p_full[2 * w + y]);
                 }
             }
-            t += n;
+            t += 2 * n;
             // the items' last tile has been read: its poison flag is final
             if (n_own > 0 && *reinterpret_cast<volatile int*>(&items[slot].poison)) l = __int_as_float(0x7fc00000);
             named_bar_sync(1 + w, 128);  // every warp of the group has read the item
@@ -803,34 +821,35 @@ __global__ void __launch_bounds__(256) paged_chunk_merge_kernel(ChunkArgs c) {
     const ChunkMeta mt = c.meta[blockIdx.x];
     if (mt.nt == 0) return;
     const Blocks x = seq_blocks(c, mt.b);
-    const int row = blockIdx.y * RB + threadIdx.x / C4, c4 = threadIdx.x % C4;
-    const int rt = (row % BM) / a.g, rh = row % BM - rt * a.g, tok = row / BM * c.tq + rt;
-    if (rt >= c.tq || tok >= x.ntok(mt.blk)) return;
-    const int unit = x.unit(mt.blk);
-    float M = -INFINITY, L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    int j0 = 0;
-    for (int i = blockIdx.x; j0 < mt.nt; i++) {
-        const int j1 = tile_at(slice_first(i + 1, mt.cost, mt.slices), mt.start, unit, mt.nt);
-        if (j1 == j0) continue;
-        const size_t at = (size_t)(2 * i + (j0 == 0 ? 1 : 0)) * kPartRows + row;
-        const float2 ml = __ldcg(c.part_ml + at);
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(c.part_o + at * HD) + c4);
-        const float Mn = fmaxf(M, ml.x), keep = ex2(M - Mn), w = ex2(ml.x - Mn);
-        M = Mn;
-        L = L * keep + ml.y * w;
-        acc.x = acc.x * keep + o.x * w, acc.y = acc.y * keep + o.y * w;
-        acc.z = acc.z * keep + o.z * w, acc.w = acc.w * keep + o.w * w;
-        j0 = j1;
+    const int c4 = threadIdx.x % C4, unit = x.unit(mt.blk);
+    for (int row = blockIdx.y * RB + threadIdx.x / C4; row < kPartRows; row += gridDim.y * RB) {
+        const int rt = (row % BM) / a.g, rh = row % BM - rt * a.g, tok = row / BM * c.tq + rt;
+        if (rt >= c.tq || tok >= x.ntok(mt.blk)) continue;
+        float M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        int j0 = 0;
+        for (int i = blockIdx.x; j0 < mt.nt; i++) {
+            const int j1 = tile_at(slice_first(i + 1, mt.cost, mt.slices), mt.start, unit, mt.nt);
+            if (j1 == j0) continue;
+            const size_t at = (size_t)(2 * i + (j0 == 0 ? 1 : 0)) * kPartRows + row;
+            const float2 ml = __ldcg(c.part_ml + at);
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(c.part_o + at * HD) + c4);
+            const float Mn = fmaxf(M, ml.x), keep = ex2(M - Mn), w = ex2(ml.x - Mn);
+            M = Mn;
+            L = L * keep + ml.y * w;
+            acc.x = acc.x * keep + o.x * w, acc.y = acc.y * keep + o.y * w;
+            acc.z = acc.z * keep + o.z * w, acc.w = acc.w * keep + o.w * w;
+            j0 = j1;
+        }
+        const float inv = 1.0f / L;
+        const size_t at = ((size_t)(x.t0 + mt.blk * x.per + tok) * a.hq + mt.h * a.g + rh) * HD + 4 * c4;
+        acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+        if (a.out_dtype == PICOATTN_DTYPE_F32)
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = acc;
+        else
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
+                make_uint2(Elem<T>::pack2(acc.x, acc.y), Elem<T>::pack2(acc.z, acc.w));
     }
-    const float inv = 1.0f / L;
-    const size_t at = ((size_t)(x.t0 + mt.blk * x.per + tok) * a.hq + mt.h * a.g + rh) * HD + 4 * c4;
-    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-    if (a.out_dtype == PICOATTN_DTYPE_F32)
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = acc;
-    else
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
-            make_uint2(Elem<T>::pack2(acc.x, acc.y), Elem<T>::pack2(acc.z, acc.w));
 }
 
 // ---- host -----------------------------------------------------------------------------
@@ -883,7 +902,7 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     const cuuint64_t qd[3] = {HD, (cuuint64_t)a.hq, (cuuint64_t)a.b.n_tok}, qs[2] = {HD * 2, (cuuint64_t)a.qs * 2};
     const cuuint32_t qb[3] = {64, (cuuint32_t)a.g, (cuuint32_t)c.tq};
     const cuuint64_t kd[2] = {HD, (cuuint64_t)a.b.n_pages * a.hkv * a.b.page_size}, ks[1] = {HD * 2};
-    const cuuint32_t kb[2] = {64, (cuuint32_t)std::min(a.b.page_size, BN)};
+    const cuuint32_t kb[2] = {64, (cuuint32_t)std::min(a.b.page_size, BH)};
     if (!make_map(&mq, a, a.q, 3, qd, qs, qb) || !make_map(&mk, a, a.k_pool, 2, kd, ks, kb) ||
         !make_map(&mv, a, a.v_pool, 2, kd, ks, kb))
         return cudaErrorInvalidValue;
@@ -892,7 +911,7 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     const int grid = (int)std::min<long long>(std::min(device_sm_count(), kMaxCtas), blocks * tiles);
     e = launch_pdl(paged_chunk_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)L::kDyn, stream, mq, mk, mv, c);
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_chunk_merge_kernel<T, HD>, dim3(grid, kPartRows / (256 / (HD / 4))), dim3(256), 0, stream, c);
+    return launch_pdl(paged_chunk_merge_kernel<T, HD>, dim3(grid, 8), dim3(256), 0, stream, c);
 }
 
 }  // namespace
