@@ -42,10 +42,10 @@ namespace {
 
 constexpr int BM = 128, BN = 128, BH = BN / 2;
 constexpr int kThreads = 384;
-constexpr int kPlan = 64;          // threads that add up the sequences' costs
+constexpr int kPlan = 32;          // runs of sequences whose costs are added up, a lane each
 constexpr int kMaxCtas = 160;
 constexpr int kMinCost = 12;       // least cost per CTA of a slice
-constexpr int kSliceOverhead = 24; // what cutting blocks costs, in the same unit (measured, see launch)
+constexpr int kSliceOverhead = 32; // what cutting blocks costs, in the same unit (measured, see launch)
 constexpr int kPartRows = 2 * BM;
 constexpr int kRing = 4;           // stages of 64 keys, K and V each
 constexpr float kNone = -1e30f;    // running maximum before any key
@@ -101,34 +101,192 @@ __device__ __forceinline__ Blocks seq_blocks(const ChunkArgs& c, int b) {
     return x;
 }
 
-__device__ __forceinline__ long long head_cost(const Blocks& x) {
-    long long s = 0;
-    for (int i = 0; i < x.count; i++) s += (long long)x.tiles(i) * x.unit(i);
+// One head's cost: 4 * tiles * blocks, in 32 bits for 10^6 tokens of a sequence and more.
+__device__ __forceinline__ int head_cost(const Blocks& x) {
+    int s = 0;
+    for (int i = 0; i < x.count; i++) s += x.tiles(i) * x.unit(i);
     return s;
+}
+// The same by a whole warp.
+__device__ __forceinline__ int head_cost_warp(const Blocks& x, int lane) {
+    int s = 0;
+    for (int i = lane; i < x.count; i += 32) s += x.tiles(i) * x.unit(i);
+    return __reduce_add_sync(0xffffffffu, s);
+}
+
+// a / b for non-negative a and positive b, in 32 bits where they fit (a tenth of the instructions)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    if (((unsigned long long)(a | b) >> 32) == 0) return (unsigned)a / (unsigned)b;
+    return a / b;
 }
 
 struct Plan {
-    long long first_cost[kPlan + 1];  // of each plan thread's sequences
+    long long first_cost[kPlan + 1];  // of each run of sequences
     int first_item[kPlan + 1];
-    int most[kPlan / 32];             // the longest block's cost
-    int slices;                       // CTAs that share the cut-up list, 0: whole blocks
 };
 
-__device__ __forceinline__ long long slice_first(long long i, long long cost, int n) { return i * cost / n; }
+// The plan, by one warp: a run of `per` sequences a lane, or, for a few
+// sequences, one a lane with its blocks spread over the lanes.  Returns the CTAs
+// that share the cut-up list, 0: whole blocks (whose list needs no costs).
+// Every CTA makes it for itself and comes to the same result.  This is the first
+// thing a call does, from cold instruction caches, so it is kept short.
+__device__ __forceinline__ int make_plan(const ChunkArgs& c, Plan* plan, int per, int grid, int lane) {
+    long long cost = 0;
+    int items = 0, most = 0;
+    if (c.a.b.n_seqs <= 4) {
+        for (int b = 0; b < c.a.b.n_seqs; b++) {
+            const Blocks x = seq_blocks(c, b);
+            const int s = head_cost_warp(x, lane);
+            if (lane == b) {
+                cost = (long long)s * c.a.hkv;
+                items = x.count * c.a.hkv;
+                most = x.count ? x.tiles(x.count - 1) * 4 : 0;
+            }
+        }
+    } else {
+        for (int b = lane * per; b < min((lane + 1) * per, c.a.b.n_seqs); b++) {
+            const Blocks x = seq_blocks(c, b);
+            cost += (long long)head_cost(x) * c.a.hkv;
+            items += x.count * c.a.hkv;
+            if (x.count) most = max(most, x.tiles(x.count - 1) * 4);
+        }
+    }
+    float all = (float)cost;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        const int io = __shfl_up_sync(0xffffffffu, items, o);
+        if (lane >= o) items += io;
+    }
+    if (lane == 0) plan->first_item[0] = 0;
+    plan->first_item[lane + 1] = items;
+    most = __reduce_max_sync(0xffffffffu, most);
+    items = __shfl_sync(0xffffffffu, items, 31);
+    // whole blocks end when the longest does, or, dealt out one by one, some 15% after the mean
+    const float n = fminf((float)grid, all * (1.0f / kMinCost)), mean = all / fmaxf(n, 1.0f);
+    const float whole = fmaxf((float)most, items <= grid ? 0.f : 1.15f * mean);
+    __syncwarp();
+    if (mean + kSliceOverhead >= whole) return 0;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long co = __shfl_up_sync(0xffffffffu, cost, o);
+        if (lane >= o) cost += co;
+    }
+    if (lane == 0) plan->first_cost[0] = 0;
+    plan->first_cost[lane + 1] = cost;
+    cost = __shfl_sync(0xffffffffu, cost, 31);
+    __syncwarp();
+    return (int)min((long long)grid, (cost + kMinCost - 1) / kMinCost);
+}
+
+__device__ __forceinline__ long long slice_first(long long i, long long cost, int n) {
+    return quotient(i * cost, n);
+}
 
 // A part's first (or end) tile for a slice that begins (ends) at cost unit x of a block from `start`.
 __device__ __forceinline__ int tile_at(long long x, long long start, int unit, int nt) {
-    return x <= start ? 0 : (int)min((long long)nt, (x - start + unit - 1) / unit);
+    return x <= start ? 0 : (int)min((long long)nt, quotient(x - start + unit - 1, unit));
 }
 
-// Walks a slice's parts (slices) or fetches whole blocks (list).
+// Where a CTA is in its work (the producer warp, the same in every lane).
 struct Walk {
-    int b, h, blk;
-    long long at, end, base;  // cost units; base: of sequence b
+    int b, h, blk, per_head;  // sequence, head and block; one head's cost
+    long long at, end;        // cost units of the slice still to do
+    long long base, start;    // first unit of the sequence, of the block
     Blocks x;
-    long long per_head, blk_start;
-    bool open;
+    bool open;                // b .. start are set
+    int taken;                // whole blocks so far
 };
+
+// The slice's first cost unit -> its sequence, head and block.
+__device__ __forceinline__ void walk_find(const ChunkArgs& c, Walk& wk, int lane) {
+    const int hkv = c.a.hkv;
+    for (;; wk.b++) {
+        wk.x = seq_blocks(c, wk.b);
+        wk.per_head = head_cost_warp(wk.x, lane);
+        if (wk.at < wk.base + (long long)wk.per_head * hkv) break;
+        wk.base += (long long)wk.per_head * hkv;
+    }
+    wk.h = (int)quotient(wk.at - wk.base, wk.per_head);
+    wk.start = wk.base + (long long)wk.h * wk.per_head;
+    const int rest = (int)(wk.at - wk.start);
+    int before = 0;  // cost of the head's blocks before the 32 looked at
+    for (int i0 = 0;; i0 += 32) {
+        const int i = i0 + lane, cost = i < wk.x.count ? wk.x.tiles(i) * wk.x.unit(i) : 0;
+        int upto = cost;
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, rest < before + upto);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            wk.blk = i0 + l;
+            wk.start += before + __shfl_sync(0xffffffffu, upto - cost, l);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    wk.open = true;
+}
+
+// The next item of a CTA; false: none.
+__device__ __forceinline__ bool next_item(const ChunkArgs& c, const Plan* plan, Walk& wk, int slices, int per, Item& it,
+                                          int lane) {
+    const int hkv = c.a.hkv;
+    it.poison = 0;
+    if (!slices) {  // whole blocks: the CTA's own first one, then by the counter
+        int idx = blockIdx.x;
+        if (wk.taken++) {
+            if (lane == 0) idx = (int)gridDim.x + atomicAdd(c.counter, 1);
+            idx = __shfl_sync(0xffffffffu, idx, 0);
+        }
+        if (idx >= plan->first_item[kPlan]) return false;
+        const int run = __popc(__ballot_sync(0xffffffffu, plan->first_item[lane + 1] <= idx));
+        int rest = idx - plan->first_item[run], b = run * per;
+        Blocks x = seq_blocks(c, b);
+        while (rest >= x.count * hkv) {
+            rest -= x.count * hkv;
+            x = seq_blocks(c, ++b);
+        }
+        const int r = (int)((unsigned)rest / (unsigned)hkv), i = x.count - 1 - r;  // a sequence's longest first
+        it.b = b, it.h = rest - r * hkv;
+        it.tok0 = x.t0 + i * x.per, it.ntok = x.ntok(i), it.pos0 = x.len - x.n + i * x.per;
+        it.j0 = 0, it.j1 = x.tiles(i), it.slot = -1, it.len = x.len;
+        return true;
+    }
+    while (wk.at < wk.end) {
+        if (!wk.open) walk_find(c, wk, lane);
+        const int nt = wk.x.tiles(wk.blk), u = wk.x.unit(wk.blk);
+        const int j0 = tile_at(wk.at, wk.start, u, nt), j1 = tile_at(wk.end, wk.start, u, nt);
+        if (j0 < j1) {
+            it.b = wk.b, it.h = wk.h;
+            it.tok0 = wk.x.t0 + wk.blk * wk.x.per, it.ntok = wk.x.ntok(wk.blk);
+            it.pos0 = wk.x.len - wk.x.n + wk.blk * wk.x.per;
+            it.j0 = j0, it.j1 = j1, it.len = wk.x.len;
+            it.slot = j0 == 0 && j1 == nt ? -1 : 2 * (int)blockIdx.x + (j0 == 0 ? 1 : 0);
+            if (j0 == 0 && j1 < nt && lane == 0)
+                c.meta[blockIdx.x] = {wk.b, wk.h, wk.blk, nt, slices, wk.start, plan->first_cost[kPlan]};
+        }
+        // step to the next block
+        wk.at = wk.start + nt * u;
+        if (wk.blk + 1 < wk.x.count) {
+            wk.start = wk.at;
+            wk.blk++;
+        } else if (wk.h + 1 < hkv) {
+            wk.h++;
+            wk.blk = 0;
+            wk.start = wk.at;
+        } else {
+            wk.base += (long long)wk.per_head * hkv;
+            wk.b++;
+            wk.open = false;
+        }
+        if (j0 < j1) return true;
+    }
+    return false;
+}
 
 // ---- one key tile of the online softmax ------------------------------------------
 
@@ -360,172 +518,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_proxy_async_shared();
     }
     pdl_wait();
-    // ---------------- plan ----------------
-    const int per = (a.b.n_seqs + kPlan - 1) / kPlan;
-    long long my_cost = 0;
-    int my_items = 0, my_max = 0;
-    if (tid < kPlan) {
-        for (int b = tid * per; b < min((tid + 1) * per, a.b.n_seqs); b++) {
-            const Blocks x = seq_blocks(c, b);
-            my_cost += head_cost(x) * a.hkv;
-            my_items += x.count * a.hkv;
-            if (x.count) my_max = max(my_max, x.tiles(x.count - 1) * 4);
-        }
-        plan->first_cost[tid + 1] = my_cost;
-        plan->first_item[tid + 1] = my_items;
-    }
-    // rows of sequences outside the host's bounds
-    for (int b = blockIdx.x; b < a.b.n_seqs; b += gridDim.x) {
-        const SeqSpan sp = seq_span(a.b, b);
-        if (sp.ok) continue;
-        if (tid == 0) atomicOr(status, PICOATTN_DEV_BAD_POS);
-        const int t0 = max(sp.t0, 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
-        const long long words = t1 > t0 ? (long long)(t1 - t0) * a.hq * HD : 0;
-        for (long long i = tid; i < words; i += kThreads) {
-            const size_t at = (size_t)t0 * a.hq * HD + i;
-            if (a.out_dtype == PICOATTN_DTYPE_F32) static_cast<float*>(a.out)[at] = __int_as_float(0x7fc00000);
-            else static_cast<T*>(a.out)[at] = Elem<T>::round(__int_as_float(0x7fc00000));
-        }
-    }
-    if (tid < kPlan) {
-        for (int o = 16; o; o >>= 1) my_max = max(my_max, __shfl_xor_sync(0xffffffffu, my_max, o));
-        if (lane == 0) plan->most[warp] = my_max;
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 0) {  // prefix sums, two entries a lane
-        const long long x0 = plan->first_cost[2 * lane + 1], x1 = plan->first_cost[2 * lane + 2];
-        const int y0 = plan->first_item[2 * lane + 1], y1 = plan->first_item[2 * lane + 2];
-        long long xs = x0 + x1;
-        int ys = y0 + y1;
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long xo = __shfl_up_sync(0xffffffffu, xs, o);
-            const int yo = __shfl_up_sync(0xffffffffu, ys, o);
-            if (lane >= o) xs += xo, ys += yo;
-        }
-        plan->first_cost[2 * lane + 1] = xs - x1, plan->first_cost[2 * lane + 2] = xs;
-        plan->first_item[2 * lane + 1] = ys - y1, plan->first_item[2 * lane + 2] = ys;
-        if (lane == 31) {
-            plan->first_cost[0] = 0;
-            plan->first_item[0] = 0;
-            const int n = (int)min((long long)gridDim.x, (xs + kMinCost - 1) / kMinCost);
-            int most = 0;
-            for (int i = 0; i < kPlan / 32; i++) most = max(most, plan->most[i]);
-            // whole blocks end when the longest does, or, dealt out one by one, some 15% after the mean
-            const long long mean = n ? (xs + n - 1) / n : 0;
-            const long long whole = max((long long)most, ys <= (int)gridDim.x ? 0 : mean + mean / 7);
-            plan->slices = mean + kSliceOverhead < whole ? n : 0;
-            c.meta[blockIdx.x].nt = 0;
-        }
-    }
-    __syncthreads();
     const uint32_t tmem = *tmem_slot;
     const float scale = 1.4426950408889634f / sqrtf((float)HD);
     const int g = a.g, tq = c.tq;
 
     if (warp == 8) {
         // ---------------- work list, TMA of Q and K ----------------
-        const int slices = plan->slices;
+        const int per = (a.b.n_seqs + kPlan - 1) / kPlan;
+        const int slices = make_plan(c, plan, per, gridDim.x, lane);
+        if (lane == 0) c.meta[blockIdx.x].nt = 0;
         Walk wk{};
-        wk.open = false;
-        if (slices && (int)blockIdx.x < slices) {
+        if ((int)blockIdx.x < slices) {
             const long long cost = plan->first_cost[kPlan];
             wk.at = slice_first(blockIdx.x, cost, slices);
             wk.end = slice_first(blockIdx.x + 1, cost, slices);
-            int lo = 0, hi = kPlan;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (plan->first_cost[mid] <= wk.at) lo = mid;
-                else hi = mid;
-            }
-            wk.b = lo * per;
-            wk.base = plan->first_cost[lo];
+            const int run = __popc(__ballot_sync(0xffffffffu, plan->first_cost[lane + 1] <= wk.at));
+            wk.b = run * per;
+            wk.base = plan->first_cost[run];
         }
-        // next item of this CTA (lane 0); false: none
-        auto next = [&](Item& it) -> bool {
-            it.poison = 0;
-            if (!slices) {
-                const int idx = atomicAdd(c.counter, 1);
-                if (idx >= plan->first_item[kPlan]) return false;
-                int lo = 0, hi = kPlan;
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (plan->first_item[mid] <= idx) lo = mid;
-                    else hi = mid;
-                }
-                int rest = idx - plan->first_item[lo], b = lo * per;
-                Blocks x = seq_blocks(c, b);
-                while (rest >= x.count * a.hkv) {
-                    rest -= x.count * a.hkv;
-                    x = seq_blocks(c, ++b);
-                }
-                const int i = x.count - 1 - rest / a.hkv;  // a sequence's longest first
-                it.b = b, it.h = rest % a.hkv;
-                it.tok0 = x.t0 + i * x.per, it.ntok = x.ntok(i), it.pos0 = x.len - x.n + i * x.per;
-                it.j0 = 0, it.j1 = x.tiles(i), it.slot = -1, it.len = x.len;
-                return true;
-            }
-            while (wk.at < wk.end) {
-                if (!wk.open) {  // find the block that holds cost unit `at`
-                    for (;; wk.b++) {
-                        wk.x = seq_blocks(c, wk.b);
-                        wk.per_head = head_cost(wk.x);
-                        if (wk.at < wk.base + wk.per_head * a.hkv) break;
-                        wk.base += wk.per_head * a.hkv;
-                    }
-                    wk.h = (int)((wk.at - wk.base) / wk.per_head);
-                    wk.blk = 0;
-                    wk.blk_start = wk.base + wk.h * wk.per_head;
-                    for (;;) {
-                        const int cost = wk.x.tiles(wk.blk) * wk.x.unit(wk.blk);
-                        if (wk.at < wk.blk_start + cost) break;
-                        wk.blk_start += cost;
-                        wk.blk++;
-                    }
-                    wk.open = true;
-                }
-                const int nt = wk.x.tiles(wk.blk), u = wk.x.unit(wk.blk);
-                const int j0 = tile_at(wk.at, wk.blk_start, u, nt), j1 = tile_at(wk.end, wk.blk_start, u, nt);
-                if (j0 < j1) {
-                    it.b = wk.b, it.h = wk.h;
-                    it.tok0 = wk.x.t0 + wk.blk * wk.x.per, it.ntok = wk.x.ntok(wk.blk);
-                    it.pos0 = wk.x.len - wk.x.n + wk.blk * wk.x.per;
-                    it.j0 = j0, it.j1 = j1, it.len = wk.x.len;
-                    it.slot = j0 == 0 && j1 == nt ? -1 : 2 * (int)blockIdx.x + (j0 == 0 ? 1 : 0);
-                    if (j0 == 0 && j1 < nt)
-                        c.meta[blockIdx.x] = {wk.b, wk.h, wk.blk, nt, slices, wk.blk_start, plan->first_cost[kPlan]};
-                }
-                // step to the next block
-                wk.at = wk.blk_start + nt * u;
-                if (wk.blk + 1 < wk.x.count) {
-                    wk.blk_start = wk.at;
-                    wk.blk++;
-                } else if (wk.h + 1 < a.hkv) {
-                    wk.h++;
-                    wk.blk = 0;
-                    wk.blk_start = wk.at;
-                } else {
-                    wk.base += wk.per_head * a.hkv;
-                    wk.b++;
-                    wk.open = false;
-                }
-                if (j0 < j1) return true;
-            }
-            return false;
-        };
         int t = 0;
         for (int k = 0;; k++) {
             const int slot = k & 1;
             if (k >= 2) mbar_wait(&item_empty[slot], (uint32_t)(((k >> 1) - 1) & 1), status);
+            Item it;
+            if (!next_item(c, plan, wk, slices, per, it, lane)) it.b = -1;
             if (lane == 0) {
-                Item it;
-                if (!next(it)) it.b = -1;
                 items[slot] = it;
+                mbar_arrive(&item_full[slot]);
             }
-            __syncwarp();
-            const Item it = items[slot];
-            if (lane == 0) mbar_arrive(&item_full[slot]);
             if (it.b < 0) break;
             const bool two = it.ntok > tq;
             if (lane == 0) {
@@ -654,6 +677,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ---------------- softmax ----------------
+        // rows of sequences outside the host's bounds
+        for (int b = blockIdx.x; b < a.b.n_seqs; b += gridDim.x) {
+            const SeqSpan sp = seq_span(a.b, b);
+            if (sp.ok) continue;
+            if (tid == 0) atomicOr(status, PICOATTN_DEV_BAD_POS);
+            const int t0 = max(sp.t0, 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
+            const long long n = t1 > t0 ? (long long)(t1 - t0) * a.hq * HD : 0;
+            for (long long i = tid; i < n; i += 256) {
+                const size_t at = (size_t)t0 * a.hq * HD + i;
+                if (a.out_dtype == PICOATTN_DTYPE_F32) static_cast<float*>(a.out)[at] = __int_as_float(0x7fc00000);
+                else static_cast<T*>(a.out)[at] = Elem<T>::round(__int_as_float(0x7fc00000));
+            }
+        }
         const int w = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + w * 128 + lanes, tO = tmem + 256 + w * 128 + lanes;
@@ -737,23 +773,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float inv = 1.0f / l;
                 w0 *= inv, w1 *= inv;
             }
-            // 32 columns of the row's O, weighted
-            auto load = [&](int col, float (&o)[32]) {
+            // 64 columns of the row's O, weighted
+            auto load = [&](int col, float (&o)[64]) {
                 if (n_own == 0) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = 0.f;
+                    for (int e = 0; e < 64; e++) o[e] = 0.f;
                     return;
                 }
-                uint32_t x[32];
-                tmem_ld32(tO + col, x);
+                uint32_t (&x)[64] = reinterpret_cast<uint32_t (&)[64]>(o);
+                tmem_ld32(tO + col, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+                tmem_ld32(tO + col + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = __uint_as_float(x[e]) * w0;
+                for (int e = 0; e < 64; e++) o[e] *= w0;
                 if (join) {
-                    tmem_ld32(tO + 128 + col, x);
-                    tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = __fmaf_rn(__uint_as_float(x[e]), w1, o[e]);
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t y[32];
+                        tmem_ld32(tO + 128 + col + 32 * h, y);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[32 * h + e] = __fmaf_rn(__uint_as_float(y[e]), w1, o[32 * h + e]);
+                    }
                 }
             };
             auto release = [&] {  // O is in registers: the next block's products may overwrite it
@@ -773,30 +814,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint8_t* dst = part ? reinterpret_cast<uint8_t*>(c.part_o) : static_cast<uint8_t*>(a.out);
             if (!live) {
                 release();
-            } else if (f32) {
-#pragma unroll 1
-                for (int col = 0; col < HD; col += 32) {
-                    float o[32];
-                    load(col, o);
-                    if (col + 32 == HD) release();
-                    uint32_t x[32];
-#pragma unroll
-                    for (int e = 0; e < 32; e++) x[e] = __float_as_uint(o[e]);
-                    store_rows(x, stage, dst + col * 4, valid ? orow * 4 : -1, lane);
-                }
             } else {
 #pragma unroll 1
                 for (int col = 0; col < HD; col += 64) {
-                    uint32_t x[32];
-#pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        float o[32];
-                        load(col + 32 * y, o);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) x[16 * y + e] = Elem<T>::pack2(o[2 * e], o[2 * e + 1]);
-                    }
+                    float o[64];
+                    load(col, o);
                     if (col + 64 == HD) release();
-                    store_rows(x, stage, dst + col * 2, valid ? orow * 2 : -1, lane);
+                    uint32_t x[32];
+                    if (f32) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+#pragma unroll
+                            for (int e = 0; e < 32; e++) x[e] = __float_as_uint(o[32 * h + e]);
+                            store_rows(x, stage, dst + (col + 32 * h) * 4, valid ? orow * 4 : -1, lane);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) x[e] = Elem<T>::pack2(o[2 * e], o[2 * e + 1]);
+                        store_rows(x, stage, dst + col * 2, valid ? orow * 2 : -1, lane);
+                    }
                 }
             }
         }
