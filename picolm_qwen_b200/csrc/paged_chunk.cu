@@ -44,7 +44,8 @@ constexpr int BM = 128, BN = 128, BH = BN / 2;
 constexpr int kThreads = 384;
 constexpr int kPlan = 32;          // runs of sequences whose costs are added up, a lane each
 constexpr int kMaxCtas = 160;
-constexpr int kMinCost = 12;       // least cost per CTA of a slice
+constexpr int kItemCost = 4;       // of a block, whatever its tiles
+constexpr int kMinCost = 16;       // least cost per CTA of a slice
 constexpr int kSliceOverhead = 32; // what cutting blocks costs, in the same unit (measured, see launch)
 constexpr int kPartRows = 2 * BM;
 constexpr int kRing = 4;           // stages of 64 keys, K and V each
@@ -89,6 +90,7 @@ struct Blocks {
     __device__ __forceinline__ int ntok(int i) const { return min(per, n - i * per); }
     __device__ __forceinline__ int tiles(int i) const { return (len - n + min(n, (i + 1) * per) + BN - 1) / BN; }
     // cost of a key tile: a two-tile block's takes some 3,500 cycles, a one-tile block's 2,600
+    __device__ __forceinline__ int cost(int i) const { return tiles(i) * unit(i) + kItemCost; }
     __device__ __forceinline__ int unit(int i) const { return ntok(i) > tq ? 4 : 3; }
 };
 
@@ -104,20 +106,14 @@ __device__ __forceinline__ Blocks seq_blocks(const ChunkArgs& c, int b) {
 // One head's cost: 4 * tiles * blocks, in 32 bits for 10^6 tokens of a sequence and more.
 __device__ __forceinline__ int head_cost(const Blocks& x) {
     int s = 0;
-    for (int i = 0; i < x.count; i++) s += x.tiles(i) * x.unit(i);
+    for (int i = 0; i < x.count; i++) s += x.cost(i);
     return s;
 }
 // The same by a whole warp.
 __device__ __forceinline__ int head_cost_warp(const Blocks& x, int lane) {
     int s = 0;
-    for (int i = lane; i < x.count; i += 32) s += x.tiles(i) * x.unit(i);
+    for (int i = lane; i < x.count; i += 32) s += x.cost(i);
     return __reduce_add_sync(0xffffffffu, s);
-}
-
-// a / b for non-negative a and positive b, in 32 bits where they fit (a tenth of the instructions)
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    if (((unsigned long long)(a | b) >> 32) == 0) return (unsigned)a / (unsigned)b;
-    return a / b;
 }
 
 struct Plan {
@@ -140,7 +136,7 @@ __device__ __forceinline__ int make_plan(const ChunkArgs& c, Plan* plan, int per
             if (lane == b) {
                 cost = (long long)s * c.a.hkv;
                 items = x.count * c.a.hkv;
-                most = x.count ? x.tiles(x.count - 1) * 4 : 0;
+                most = x.count ? x.tiles(x.count - 1) * 4 + kItemCost : 0;
             }
         }
     } else {
@@ -148,7 +144,7 @@ __device__ __forceinline__ int make_plan(const ChunkArgs& c, Plan* plan, int per
             const Blocks x = seq_blocks(c, b);
             cost += (long long)head_cost(x) * c.a.hkv;
             items += x.count * c.a.hkv;
-            if (x.count) most = max(most, x.tiles(x.count - 1) * 4);
+            if (x.count) most = max(most, x.tiles(x.count - 1) * 4 + kItemCost);
         }
     }
     float all = (float)cost;
@@ -185,6 +181,7 @@ __device__ __forceinline__ long long slice_first(long long i, long long cost, in
 
 // A part's first (or end) tile for a slice that begins (ends) at cost unit x of a block from `start`.
 __device__ __forceinline__ int tile_at(long long x, long long start, int unit, int nt) {
+    start += kItemCost;
     return x <= start ? 0 : (int)min((long long)nt, quotient(x - start + unit - 1, unit));
 }
 
@@ -212,7 +209,7 @@ __device__ __forceinline__ void walk_find(const ChunkArgs& c, Walk& wk, int lane
     const int rest = (int)(wk.at - wk.start);
     int before = 0;  // cost of the head's blocks before the 32 looked at
     for (int i0 = 0;; i0 += 32) {
-        const int i = i0 + lane, cost = i < wk.x.count ? wk.x.tiles(i) * wk.x.unit(i) : 0;
+        const int i = i0 + lane, cost = i < wk.x.count ? wk.x.cost(i) : 0;
         int upto = cost;
 #pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
@@ -270,7 +267,7 @@ __device__ __forceinline__ bool next_item(const ChunkArgs& c, const Plan* plan, 
                 c.meta[blockIdx.x] = {wk.b, wk.h, wk.blk, nt, slices, wk.start, plan->first_cost[kPlan]};
         }
         // step to the next block
-        wk.at = wk.start + nt * u;
+        wk.at = wk.start + nt * u + kItemCost;
         if (wk.blk + 1 < wk.x.count) {
             wk.start = wk.at;
             wk.blk++;
@@ -399,7 +396,7 @@ struct Smem {
     static constexpr int kQ = 0;
     static constexpr int kK = 2 * kTile;
     static constexpr int kV = kK + kRing * kHalf;
-    static constexpr int kStage = kV + kRing * kHalf;   // 4 KB per softmax warp
+    static constexpr int kStage = kV + kRing * kHalf;   // 16 KB per softmax group
     static constexpr int kPlanAt = kStage + 8 * 4096;
     static constexpr int kBars = (kPlanAt + (int)sizeof(Plan) + 15) / 16 * 16;
     static constexpr int kItems = kBars + 36 * 8;
@@ -456,12 +453,18 @@ __device__ __forceinline__ void store_rows(const uint32_t (&w)[32], uint4* stage
     for (int u = 0; u < 8; u++)
         stage[lane * 8 + (u ^ (lane & 7))] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
     __syncwarp();
+    // all reads before the first store: the compiler cannot tell the two apart
+    uint4 v[8];
+    long long o[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int row = 4 * i + (lane >> 3), u = lane & 7;
-        const long long o = __shfl_sync(0xffffffffu, off, row);
-        if (o >= 0) *reinterpret_cast<uint4*>(dst + o + 16 * u) = stage[row * 8 + (u ^ (row & 7))];
+        v[i] = stage[row * 8 + (u ^ (row & 7))];
+        o[i] = __shfl_sync(0xffffffffu, off, row);
     }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (o[i] >= 0) *reinterpret_cast<uint4*>(dst + o[i] + 16 * (lane & 7)) = v[i];
 }
 
 // ---- the kernel --------------------------------------------------------------------
@@ -469,7 +472,8 @@ __device__ __forceinline__ void store_rows(const uint32_t (&w)[32], uint4* stage
 template <class T, int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                       const __grid_constant__ CUtensorMap tmV, const ChunkArgs c) {
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                       const __grid_constant__ CUtensorMap tmP, const ChunkArgs c) {
     using L = Smem<HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int w = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + w * 128 + lanes, tO = tmem + 256 + w * 128 + lanes;
-        uint4* stage = reinterpret_cast<uint4*>(smem + L::kStage + warp * 4096);
+        uint4* gstage = reinterpret_cast<uint4*>(smem + L::kStage + w * 4 * 4096);  // 128 rows of 128 bytes
         float2* xs = reinterpret_cast<float2*>(smem + L::kStage + 4 * 4096);  // group 1's (max, sum), one-tile blocks
         const int rt = r / g, rh = r - rt * g;  // the row's token in its tile, and head
         int t = 0, mine = 0;  // half tiles of the CTA, key tiles of this group
@@ -752,6 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool join = !two && n > 1;
             if (!two && w == 1) {  // hand over to group 0
                 if (join) {
+                    if (r == 0) bulk_wait_read_all();
+                    named_bar_sync(2, 128);  // the stage, where xs lies, has been read
                     xs[r] = make_float2(m, l);
                     tc_fence_before();
                     named_bar_arrive(3, 256);
@@ -773,28 +779,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float inv = 1.0f / l;
                 w0 *= inv, w1 *= inv;
             }
-            // 64 columns of the row's O, weighted
-            auto load = [&](int col, float (&o)[64]) {
+            // 32 columns of the row's O, weighted
+            auto load = [&](int col, float (&o)[32]) {
                 if (n_own == 0) {
 #pragma unroll
-                    for (int e = 0; e < 64; e++) o[e] = 0.f;
+                    for (int e = 0; e < 32; e++) o[e] = 0.f;
                     return;
                 }
-                uint32_t (&x)[64] = reinterpret_cast<uint32_t (&)[64]>(o);
-                tmem_ld32(tO + col, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-                tmem_ld32(tO + col + 32, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
+                tmem_ld32(tO + col, reinterpret_cast<uint32_t (&)[32]>(o));
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 64; e++) o[e] *= w0;
+                for (int e = 0; e < 32; e++) o[e] *= w0;
                 if (join) {
+                    uint32_t y[32];
+                    tmem_ld32(tO + 128 + col, y);
+                    tmem_ld_wait();
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t y[32];
-                        tmem_ld32(tO + 128 + col + 32 * h, y);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[32 * h + e] = __fmaf_rn(__uint_as_float(y[e]), w1, o[32 * h + e]);
-                    }
+                    for (int e = 0; e < 32; e++) o[e] = __fmaf_rn(__uint_as_float(y[e]), w1, o[e]);
                 }
             };
             auto release = [&] {  // O is in registers: the next block's products may overwrite it
@@ -807,35 +808,54 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             const int row = w * BM + r;  // of the block's two tiles (one-tile blocks: w is 0)
             if (part && valid) c.part_ml[(size_t)it.slot * kPartRows + row] = make_float2(m, l);
-            const long long orow =
-                part ? ((long long)it.slot * kPartRows + row) * HD
-                     : ((long long)(it.tok0 + tok) * a.hq + it.h * g + rh) * HD;
             const bool f32 = part || a.out_dtype == PICOATTN_DTYPE_F32;
-            uint8_t* dst = part ? reinterpret_cast<uint8_t*>(c.part_o) : static_cast<uint8_t*>(a.out);
-            if (!live) {
-                release();
-            } else {
+            // A tile whose rows are all valid, or any part (its other rows are scratch), leaves by
+            // one TMA store per 128 bytes of its rows, from a swizzled stage of the group; the rows
+            // of a ragged tile by per-row stores.  (The SM's store path takes some 2,000 cycles
+            // for 64 columns of a tile by per-row stores.)
+            const bool bulk = part || it.ntok >= (w + 1) * tq;
+            const long long orow = ((long long)(it.tok0 + tok) * a.hq + it.h * g + rh) * HD;
+            const int step = f32 ? 32 : 64;
+            if (r == 0) bulk_wait_read_all();  // the stage's last store
 #pragma unroll 1
-                for (int col = 0; col < HD; col += 64) {
-                    float o[64];
+            for (int col = 0; col < HD; col += step) {
+                uint32_t x[32];
+                if (f32) {
+                    float o[32];
                     load(col, o);
-                    if (col + 64 == HD) release();
-                    uint32_t x[32];
-                    if (f32) {
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
+                    for (int e = 0; e < 32; e++) x[e] = __float_as_uint(o[e]);
+                } else {
 #pragma unroll
-                            for (int e = 0; e < 32; e++) x[e] = __float_as_uint(o[32 * h + e]);
-                            store_rows(x, stage, dst + (col + 32 * h) * 4, valid ? orow * 4 : -1, lane);
-                        }
-                    } else {
+                    for (int h = 0; h < 2; h++) {
+                        float o[32];
+                        load(col + 32 * h, o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) x[e] = Elem<T>::pack2(o[2 * e], o[2 * e + 1]);
-                        store_rows(x, stage, dst + col * 2, valid ? orow * 2 : -1, lane);
+                        for (int e = 0; e < 16; e++) x[16 * h + e] = Elem<T>::pack2(o[2 * e], o[2 * e + 1]);
                     }
+                }
+                if (col + step == HD) release();
+                if (bulk) {
+                    named_bar_sync(1 + w, 128);  // the stage is free
+#pragma unroll
+                    for (int u = 0; u < 8; u++)
+                        gstage[r * 8 + (u ^ (r & 7))] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+                    fence_proxy_async_shared();
+                    named_bar_sync(1 + w, 128);
+                    if (r == 0) {
+                        if (part) tma_store_2d(&tmP, gstage, col, it.slot * kPartRows + w * BM);
+                        else tma_store_3d(&tmO, gstage, col, it.h * g, it.tok0 + w * tq);
+                        bulk_commit_group();
+                        if (col + step < HD) bulk_wait_read_all();
+                    }
+                } else {
+                    if (col == 0) named_bar_sync(1 + w, 128);
+                    store_rows(x, gstage + (warp & 3) * 256, static_cast<uint8_t*>(a.out) + col * (f32 ? 4 : 2),
+                               valid ? orow * (f32 ? 4 : 2) : -1, lane);
                 }
             }
         }
+        if (r == 0) bulk_wait_all();
     }
     __syncthreads();
     if (warp == 9) {
@@ -847,9 +867,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the parts of the blocks that slices cut: block (CTA that holds a cut
 // block's first part, row group), thread (row, four columns).  Also sets the
 // work counter back.
+constexpr int kMergeBlocks = 8;  // per cut block
+
 template <class T, int HD>
 __global__ void __launch_bounds__(256) paged_chunk_merge_kernel(ChunkArgs c) {
     constexpr int C4 = HD / 4, RB = 256 / C4;
+    static_assert(kMaxCtas <= 256, "a thread per part");
     pdl_trigger();
     pdl_wait();
     const PagedAttnArgs& a = c.a;
@@ -857,25 +880,29 @@ __global__ void __launch_bounds__(256) paged_chunk_merge_kernel(ChunkArgs c) {
     const ChunkMeta mt = c.meta[blockIdx.x];
     if (mt.nt == 0) return;
     const Blocks x = seq_blocks(c, mt.b);
-    const int c4 = threadIdx.x % C4, unit = x.unit(mt.blk);
-    for (int row = blockIdx.y * RB + threadIdx.x / C4; row < kPartRows; row += gridDim.y * RB) {
+    const int unit = x.unit(mt.blk);
+    // the parts are those of this CTA and the ones after it, as the attention kernel cut them
+    const int i = blockIdx.x + threadIdx.x;
+    const bool has = i < mt.slices && tile_at(slice_first(i, mt.cost, mt.slices), mt.start, unit, mt.nt) <
+                                          tile_at(slice_first(i + 1, mt.cost, mt.slices), mt.start, unit, mt.nt);
+    const int parts = __syncthreads_count(has);
+    auto slot = [&](int p) { return (size_t)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * kPartRows; };
+    const int c4 = threadIdx.x % C4, ntok = x.ntok(mt.blk);
+    for (int row = blockIdx.y * RB + threadIdx.x / C4; row < kPartRows; row += kMergeBlocks * RB) {
         const int rt = (row % BM) / a.g, rh = row % BM - rt * a.g, tok = row / BM * c.tq + rt;
-        if (rt >= c.tq || tok >= x.ntok(mt.blk)) continue;
-        float M = -INFINITY, L = 0.f;
+        if (rt >= c.tq || tok >= ntok) continue;
+        float M = -INFINITY;
+#pragma unroll 4
+        for (int p = 0; p < parts; p++) M = fmaxf(M, __ldcg(c.part_ml + slot(p) + row).x);
+        float L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        int j0 = 0;
-        for (int i = blockIdx.x; j0 < mt.nt; i++) {
-            const int j1 = tile_at(slice_first(i + 1, mt.cost, mt.slices), mt.start, unit, mt.nt);
-            if (j1 == j0) continue;
-            const size_t at = (size_t)(2 * i + (j0 == 0 ? 1 : 0)) * kPartRows + row;
-            const float2 ml = __ldcg(c.part_ml + at);
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(c.part_o + at * HD) + c4);
-            const float Mn = fmaxf(M, ml.x), keep = ex2(M - Mn), w = ex2(ml.x - Mn);
-            M = Mn;
-            L = L * keep + ml.y * w;
-            acc.x = acc.x * keep + o.x * w, acc.y = acc.y * keep + o.y * w;
-            acc.z = acc.z * keep + o.z * w, acc.w = acc.w * keep + o.w * w;
-            j0 = j1;
+#pragma unroll 4
+        for (int p = 0; p < parts; p++) {
+            const float2 ml = __ldcg(c.part_ml + slot(p) + row);
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(c.part_o + (slot(p) + row) * HD) + c4);
+            const float w = ex2(ml.x - M);
+            L += ml.y * w;
+            acc.x += o.x * w, acc.y += o.y * w, acc.z += o.z * w, acc.w += o.w * w;
         }
         const float inv = 1.0f / L;
         const size_t at = ((size_t)(x.t0 + mt.blk * x.per + tok) * a.hq + mt.h * a.g + rh) * HD + 4 * c4;
@@ -905,13 +932,15 @@ EncodeTiled encoder() {
     return fn;
 }
 
-// Boxes of 64 columns (128 bytes, 128-byte swizzle) x the other dimensions' box.
-bool make_map(CUtensorMap* m, const PagedAttnArgs& a, const void* base, int rank, const cuuint64_t* dims,
-              const cuuint64_t* strides, const cuuint32_t* box) {
+// Boxes of 128-byte rows, 128-byte swizzle.
+bool make_map(CUtensorMap* m, int dtype, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+              const cuuint32_t* box) {
     const EncodeTiled fn = encoder();
     const cuuint32_t one[3] = {1, 1, 1};
-    return fn && fn(m, a.dtype == PICOATTN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                    (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUtensorMapDataType t = dtype == PICOATTN_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : dtype == PICOATTN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return fn && fn(m, t, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -934,20 +963,26 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     c.meta = reinterpret_cast<ChunkMeta*>(a.ws);
     c.part_ml = reinterpret_cast<float2*>(a.ws + kMetaBytes);
     c.part_o = reinterpret_cast<float*>(a.ws + kMetaBytes + kMlBytes);
-    CUtensorMap mq, mk, mv;
+    CUtensorMap mq, mk, mv, mo, mp;
     const cuuint64_t qd[3] = {HD, (cuuint64_t)a.hq, (cuuint64_t)a.b.n_tok}, qs[2] = {HD * 2, (cuuint64_t)a.qs * 2};
     const cuuint32_t qb[3] = {64, (cuuint32_t)a.g, (cuuint32_t)c.tq};
     const cuuint64_t kd[2] = {HD, (cuuint64_t)a.b.n_pages * a.hkv * a.b.page_size}, ks[1] = {HD * 2};
     const cuuint32_t kb[2] = {64, (cuuint32_t)std::min(a.b.page_size, BH)};
-    if (!make_map(&mq, a, a.q, 3, qd, qs, qb) || !make_map(&mk, a, a.k_pool, 2, kd, ks, kb) ||
-        !make_map(&mv, a, a.v_pool, 2, kd, ks, kb))
+    const size_t es = a.out_dtype == PICOATTN_DTYPE_F32 ? 4 : 2;
+    const cuuint64_t os[2] = {HD * es, (cuuint64_t)a.hq * HD * es};
+    const cuuint32_t ob[3] = {(cuuint32_t)(128 / es), (cuuint32_t)a.g, (cuuint32_t)c.tq};
+    const cuuint64_t pd[2] = {HD, 2 * (cuuint64_t)kMaxCtas * kPartRows}, ps[1] = {HD * 4};
+    const cuuint32_t pb[2] = {32, BM};
+    if (!make_map(&mq, a.dtype, a.q, 3, qd, qs, qb) || !make_map(&mk, a.dtype, a.k_pool, 2, kd, ks, kb) ||
+        !make_map(&mv, a.dtype, a.v_pool, 2, kd, ks, kb) || !make_map(&mo, a.out_dtype, a.out, 3, qd, os, ob) ||
+        !make_map(&mp, PICOATTN_DTYPE_F32, c.part_o, 2, pd, ps, pb))
         return cudaErrorInvalidValue;
     const long long blocks = (long long)a.b.n_seqs * a.hkv * ((a.b.max_new + 2 * c.tq - 1) / (2 * c.tq));
     const long long tiles = (a.b.max_len + BN - 1) / BN;  // a slice has at least kMinCost units, a whole block a CTA
     const int grid = (int)std::min<long long>(std::min(device_sm_count(), kMaxCtas), blocks * tiles);
-    e = launch_pdl(paged_chunk_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)L::kDyn, stream, mq, mk, mv, c);
+    e = launch_pdl(paged_chunk_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)L::kDyn, stream, mq, mk, mv, mo, mp, c);
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_chunk_merge_kernel<T, HD>, dim3(grid, 8), dim3(256), 0, stream, c);
+    return launch_pdl(paged_chunk_merge_kernel<T, HD>, dim3(grid, kMergeBlocks), dim3(256), 0, stream, c);
 }
 
 }  // namespace

@@ -158,6 +158,12 @@ __device__ __forceinline__ void fence_proxy_async_shared() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// a / b for non-negative a and positive b, in 32 bits where they fit (a tenth of the instructions).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    if (((unsigned long long)(a | b) >> 32) == 0) return (unsigned)a / (unsigned)b;
+    return a / b;
+}
+
 // ---- the ragged batch ---------------------------------------------------------
 
 struct SeqSpan {

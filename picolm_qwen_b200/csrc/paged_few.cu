@@ -26,6 +26,7 @@ constexpr int kUnit = 16;      // cache rows per unit
 constexpr int kWarps = 4;      // compute warps
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kStages = 3;
+constexpr int kWholeBytes = 256 << 10;
 constexpr int kMinUnits = 4;   // least units per CTA: a slice shorter than a tile gains nothing
 
 template <int HD>
@@ -50,6 +51,7 @@ struct FewArgs {
     long long* prefix;  // [n_seqs + 1] first unit of each sequence
     float2* part_ml;    // [2 * grid][16]
     float* part_o;      // [2 * grid][16][hd]
+    int whole;          // a stream per CTA: nothing is cut, nothing merged
 };
 
 __device__ __forceinline__ long long seq_units(const SeqSpan& s, int hkv) {
@@ -57,11 +59,12 @@ __device__ __forceinline__ long long seq_units(const SeqSpan& s, int hkv) {
 }
 // CTAs in use, and the units [first(i), first(i + 1)) of CTA i
 __device__ __forceinline__ int ctas_used(long long units, int grid) {
-    return (int)min((long long)grid, (units + kMinUnits - 1) / kMinUnits);
+    return (int)min((long long)grid, (units + kMinUnits - 1) >> 2);
+    static_assert(kMinUnits == 4, "a shift");
 }
-__device__ __forceinline__ long long first_unit(long long i, long long units, int ctas) { return i * units / ctas; }
+__device__ __forceinline__ long long first_unit(long long i, long long units, int ctas) { return quotient(i * units, ctas); }
 __device__ __forceinline__ int cta_of(long long unit, long long units, int ctas) {
-    int i = (int)(unit * ctas / units);
+    int i = (int)quotient(unit * ctas, units);
     while (i + 1 < ctas && first_unit(i + 1, units, ctas) <= unit) i++;
     while (i > 0 && first_unit(i, units, ctas) > unit) i--;
     return i;
@@ -91,18 +94,12 @@ __device__ __forceinline__ void store_out4(const PagedAttnArgs& a, size_t at, co
 }
 
 // Calls fn(b, span, head, u0, u1, units of the stream) for each part of the
-// units [c0, c1), in order.  chunk: first units of each thread's `per` sequences.
+// units [c0, c1), in order; b0: a sequence at or before the first, whose units
+// begin at `base`.
 template <class F>
-__device__ __forceinline__ void for_each_part(const PagedAttnArgs& a, const long long* chunk, int per, long long c0,
-                                              long long c1, F&& fn) {
-    int lo = 0, hi = kThreads;  // the last thread whose first unit is <= c0
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (chunk[mid] <= c0) lo = mid;
-        else hi = mid;
-    }
-    long long base = chunk[lo];
-    for (int b = lo * per; b < a.b.n_seqs && base < c1; b++) {
+__device__ __forceinline__ void for_each_part(const PagedAttnArgs& a, int b0, long long base, long long c0, long long c1,
+                                              F&& fn) {
+    for (int b = b0; b < a.b.n_seqs && base < c1; b++) {
         const SeqSpan sp = seq_span(a.b, b);
         const long long n = seq_units(sp, a.hkv);
         if (base + n > c0) {
@@ -110,7 +107,7 @@ __device__ __forceinline__ void for_each_part(const PagedAttnArgs& a, const long
             long long at = max(base, c0);
             const long long end = min(base + n, c1);
             while (at < end) {
-                const int h = (int)((at - base) / per_head);
+                const int h = (int)quotient(at - base, per_head);
                 const int u0 = (int)(at - base - (long long)h * per_head);
                 const int u1 = (int)min((long long)per_head, u0 + (end - at));
                 fn(b, sp, h, u0, u1, per_head);
@@ -119,6 +116,19 @@ __device__ __forceinline__ void for_each_part(const PagedAttnArgs& a, const long
         }
         base += n;
     }
+}
+
+// NaN into the rows of a sequence outside the host's bounds, those of KV head h
+// that are i, i + n, ... (as far as they lie in out).
+template <class T, int HD>
+__device__ __forceinline__ void nan_rows(const PagedAttnArgs& a, int b, int h, int i, int n, int tid, int threads) {
+    constexpr int C4 = HD / 4;
+    const int t0 = max(a.b.q_start[b], 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
+    const float nan = __int_as_float(0x7fc00000);
+    for (long long x = i; x < (long long)(t1 - t0) * a.g; x += n)
+        for (int c = tid; c < C4; c += threads)
+            store_out4<T>(a, ((size_t)(t0 + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * c,
+                          make_float4(nan, nan, nan, nan));
 }
 
 template <class T, int HD>
@@ -142,45 +152,69 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
         fence_mbar_init();
     }
     pdl_wait();
-    // first units of every thread's sequences
-    const int per = (a.b.n_seqs + kThreads - 1) / kThreads;
-    const int b0 = min(tid * per, a.b.n_seqs), b1 = min(b0 + per, a.b.n_seqs);
-    long long mine = 0;
-    for (int b = b0; b < b1; b++) {
-        const SeqSpan sp = seq_span(a.b, b);
-        if (!sp.ok && blockIdx.x == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
-        mine += seq_units(sp, a.hkv);
-    }
-    long long incl = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-    }
-    if (lane == 31) warp_tot[warp] = incl;
-    __syncthreads();
-    long long first = incl - mine;
-    for (int w = 0; w < warp; w++) first += warp_tot[w];
-    chunk[tid] = first;
-    if (tid == kThreads - 1) chunk[kThreads] = first + mine;
-    if (blockIdx.x == 0) {  // for the merge kernel
-        long long run = first;
-        for (int b = b0; b < b1; b++) {
-            fa.prefix[b] = run;
-            run += seq_units(seq_span(a.b, b), a.hkv);
+    int b0;
+    long long base, c0, c1;
+    if (fa.whole) {  // a stream per CTA
+        b0 = (int)(blockIdx.x / (unsigned)a.hkv);
+        const int h = (int)blockIdx.x - b0 * a.hkv;
+        const SeqSpan sp = seq_span(a.b, b0);
+        if (!sp.ok) {
+            if (h == 0 && tid == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+            nan_rows<T, HD>(a, b0, h, 0, 1, tid, kThreads);
         }
-        if (tid == kThreads - 1) fa.prefix[a.b.n_seqs] = first + mine;
+        if (!sp.ok || sp.n == 0) return;
+        const int per_head = (sp.len + kUnit - 1) / kUnit;
+        base = 0, c0 = (long long)h * per_head, c1 = c0 + per_head;
+        __syncthreads();  // the barriers
+    } else {
+        // first units of every thread's sequences
+        const int per = (a.b.n_seqs + kThreads - 1) / kThreads;
+        const int lo = min(tid * per, a.b.n_seqs), hi = min(lo + per, a.b.n_seqs);
+        long long mine = 0;
+        for (int b = lo; b < hi; b++) {
+            const SeqSpan sp = seq_span(a.b, b);
+            if (!sp.ok && blockIdx.x == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+            mine += seq_units(sp, a.hkv);
+        }
+        long long incl = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) warp_tot[warp] = incl;
+        __syncthreads();
+        long long first = incl - mine;
+        for (int w = 0; w < warp; w++) first += warp_tot[w];
+        chunk[tid] = first;
+        if (tid == kThreads - 1) chunk[kThreads] = first + mine;
+        if (blockIdx.x == 0) {  // for the merge kernel
+            long long run = first;
+            for (int b = lo; b < hi; b++) {
+                fa.prefix[b] = run;
+                run += seq_units(seq_span(a.b, b), a.hkv);
+            }
+            if (tid == kThreads - 1) fa.prefix[a.b.n_seqs] = first + mine;
+        }
+        __syncthreads();
+        const long long units = chunk[kThreads];
+        const int ctas = ctas_used(units, gridDim.x);
+        if ((int)blockIdx.x >= ctas) return;
+        c0 = first_unit(blockIdx.x, units, ctas), c1 = first_unit(blockIdx.x + 1, units, ctas);
+        int l = 0, h = kThreads;  // the last thread whose first unit is <= c0
+        while (h - l > 1) {
+            const int mid = (l + h) >> 1;
+            if (chunk[mid] <= c0) l = mid;
+            else h = mid;
+        }
+        b0 = l * per;
+        base = chunk[l];
     }
-    __syncthreads();
-    const long long units = chunk[kThreads];
-    const int ctas = ctas_used(units, gridDim.x);
-    if ((int)blockIdx.x >= ctas) return;
-    const long long c0 = first_unit(blockIdx.x, units, ctas), c1 = first_unit(blockIdx.x + 1, units, ctas);
 
     if (warp == kWarps) {
         // ---------------- producer: lanes 0-7 the K groups, 8-15 the V groups ----------------
         int t = 0;
         const uint8_t* pool = static_cast<const uint8_t*>(lane & 8 ? a.v_pool : a.k_pool);
-        for_each_part(a, chunk, per, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int) {
+        for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int) {
             const int r1 = min(u1 * kUnit, sp.len);
             const int* table = a.b.page_table + (size_t)b * a.b.page_cols;
             for (int row0 = u0 * kUnit; row0 < r1; row0 += F::T, t++) {
@@ -218,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
     const uint32_t tiles_u32 = smem_u32(tiles);
     const float scale = 1.4426950408889634f / sqrtf((float)HD);
     int t = 0;
-    for_each_part(a, chunk, per, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
+    for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
         const int rows = sp.n * a.g;  // <= kRows
         uint32_t qa[HD / 16][4];
         int lim[2];  // keys below it are visible to the lane's rows gid, gid + 8
@@ -398,12 +432,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     const int b = (int)(blockIdx.y / a.hkv), h = (int)(blockIdx.y % a.hkv), r = blockIdx.x;
     const SeqSpan sp = seq_span(a.b, b);
     if (!sp.ok) {
-        const int t0 = max(sp.t0, 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
-        const float nan = __int_as_float(0x7fc00000);
-        for (long long x = r; x < (long long)(t1 - t0) * a.g; x += gridDim.x)
-            for (int c = tid; c < C4; c += kMergeThreads)
-                store_out4<T>(a, ((size_t)(t0 + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * c,
-                              make_float4(nan, nan, nan, nan));
+        nan_rows<T, HD>(a, b, h, r, gridDim.x, tid, kMergeThreads);
         return;
     }
     if (r >= sp.n * a.g) return;
@@ -482,10 +511,17 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
         return cudaFuncSetAttribute(paged_few_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::bytes);
     });
     if (e != cudaSuccess) return e;
-    const long long units = (long long)a.b.n_seqs * a.hkv * ((a.b.max_len + kUnit - 1) / kUnit);
-    const int grid = (int)std::min<long long>(std::min(2 * device_sm_count(), kMaxParts), (units + kMinUnits - 1) / kMinUnits);
     FewArgs fa{};
     fa.a = a;
+    // Short sequences: a stream per CTA.  An SM takes in 65 KB a microsecond, so up
+    // to kWholeBytes a stream takes less time than cutting it saves, as the merge
+    // kernel is then not launched at all (one token over 512 rows of 4 KV heads of
+    // 64: 8.0 us cut, 6.2 whole).
+    fa.whole = (long long)a.b.max_len * HD * 4 <= kWholeBytes;
+    if (fa.whole)
+        return launch_pdl(paged_few_kernel<T, HD>, dim3(a.b.n_seqs * a.hkv), dim3(kThreads), (size_t)F::bytes, stream, fa);
+    const long long units = (long long)a.b.n_seqs * a.hkv * ((a.b.max_len + kUnit - 1) / kUnit);
+    const int grid = (int)std::min<long long>(std::min(2 * device_sm_count(), kMaxParts), (units + kMinUnits - 1) / kMinUnits);
     fa.part_ml = reinterpret_cast<float2*>(a.ws);
     fa.part_o = reinterpret_cast<float*>(a.ws + (size_t)2 * kMaxParts * kRows * 8);
     fa.prefix = reinterpret_cast<long long*>(a.ws + (size_t)2 * kMaxParts * kRows * (8 + 4 * HD));
