@@ -41,7 +41,11 @@ __device__ __forceinline__ void store_pieces(const float (&x)[16], TC* head, con
 // instruction issue as much as by memory (about 130 instructions per step of
 // 512 elements): the loads of a unit are issued first, its token's sequence,
 // position, page and table entries are found while they travel, and units are
-// numbered kind by kind, so that the warps of an SM run the same code.
+// numbered kind by kind, so that the warps of an SM run the same code.  Measured:
+// 2,048 tokens of 32/8 heads of 128 with QK-norm in fp16 14.3 us (51 MB: 3.6 TB/s,
+// 0.55 of the copy rate, as the contiguous prefill's prep kernel takes; a ring of
+// cp.async copies of the next units took 20.5, the shared memory it needs being
+// taken from the cache that the lookups live in); 64 tokens 3.3 us.
 constexpr int kSteps = 2;
 
 struct AppendSplit {
@@ -168,7 +172,7 @@ cudaError_t launch_hd(const PagedAppendArgs& a, cudaStream_t stream) {
     const long long units = (long long)a.b.n_tok * (sp.q_per + 2 * sp.kv_per);
     sp.q_units = (unsigned)a.b.n_tok * sp.q_per;
     sp.kv_units = (unsigned)a.b.n_tok * sp.kv_per;
-    const unsigned grid = (unsigned)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, 32LL * device_sm_count());
+    const unsigned grid = (unsigned)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, 6LL * device_sm_count());
     return launch_pdl(paged_append_kernel<TI, TC, HD>, dim3(grid), dim3(kAppendWarps * 32), 0, stream, a, sp);
 }
 
