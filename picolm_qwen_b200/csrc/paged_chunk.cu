@@ -399,7 +399,7 @@ struct Smem {
     static constexpr int kStage = kV + kRing * kHalf;   // 16 KB per softmax group
     static constexpr int kPlanAt = kStage + 8 * 4096;
     static constexpr int kBars = (kPlanAt + (int)sizeof(Plan) + 15) / 16 * 16;
-    static constexpr int kItems = kBars + 36 * 8;
+    static constexpr int kItems = kBars + 40 * 8;
     static constexpr int kEnd = kItems + 2 * (int)sizeof(Item) + 16;
     static constexpr int kDyn = kEnd + 1024;         // slack to align the base
     static_assert(kDyn <= 227 * 1024, "one CTA per SM");
@@ -407,10 +407,10 @@ struct Smem {
 
 // The pages of an item's key tiles into a ring of half tiles (64 rows x HD as
 // HD / 64 boxes of 128-byte rows), by one warp: a lane per box and page.  t: half
-// tiles that the ring has seen.
+// tiles that the ring has seen, counted up.  False: a wait ran out.
 template <int HD>
-__device__ __forceinline__ void load_tiles(const PagedAttnArgs& a, const CUtensorMap& map, Item& item, uint8_t* ring,
-                                           uint64_t* full, uint64_t* empty, int t, unsigned int* status, int lane) {
+__device__ __forceinline__ bool load_tiles(const PagedAttnArgs& a, const CUtensorMap& map, const Item& item, int* poison,
+                                           uint8_t* ring, uint64_t* full, uint64_t* empty, int& t, unsigned int* status, int lane) {
     using L = Smem<HD>;
     const int rows = min(a.b.page_size, BH), boxes = BH / rows;  // rows of a box, boxes of a half's column group
     const int col = lane / boxes, box = lane % boxes;
@@ -430,16 +430,22 @@ __device__ __forceinline__ void load_tiles(const PagedAttnArgs& a, const CUtenso
         const int at = (max(page, 0) * a.hkv + h) * a.b.page_size + (r & (a.b.page_size - 1));
         if (__any_sync(0xffffffffu, page == -2) && lane == 0) {
             atomicOr(status, PICOATTN_DEV_BAD_PAGE);
-            item.poison = 1;
+            *poison = 1;
         }
         const uint32_t n = __popc(__ballot_sync(0xffffffffu, page != -1));
-        if (use > 0) mbar_wait(&empty[s], (uint32_t)((use - 1) & 1), status);
+        if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)((use - 1) & 1), status))) return false;
         if (lane == 0) mbar_arrive_expect_tx(&full[s], n * (uint32_t)rows * 128u);
         __syncwarp();
         if (page != -1)
             tma_load_2d(ring + s * L::kHalf + col * L::kHBox + box * rows * 128, &map, 64 * col, at, &full[s]);
         page = next;
     }
+    return true;
+}
+
+// Giving up: the copies still on their way into the ring.
+__device__ __forceinline__ void settle_ring(uint64_t* full, int t) {
+    for (int c = max(0, t - kRing); c < t; c++) mbar_settle(&full[c % kRing], (uint32_t)((c / kRing) & 1));
 }
 
 // ---- output ------------------------------------------------------------------------
@@ -486,12 +492,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* q_empty = bars + 5;
     uint64_t* s_full = bars + 6;        // [group][half]
     uint64_t* p_full = bars + 10;       // [group][half]
-    uint64_t* pv_done = bars + 14;      // [2] per softmax group, a phase per half tile
-    uint64_t* o_free = bars + 16;       // [2]
-    uint64_t* k_full = bars + 18;       // [kRing], each
+    uint64_t* pv_done = bars + 14;      // [group][half]
+    uint64_t* o_free = bars + 18;       // [2] per group
+    uint64_t* k_full = bars + 20;       // [kRing], each
     uint64_t* k_empty = k_full + kRing;
     uint64_t* v_full = k_empty + kRing;
     uint64_t* v_empty = v_full + kRing;
+    uint64_t* mma_item = v_empty + kRing;  // both issuing warps are through with an item
+    uint64_t* joined = mma_item + 1;       // group 1's (max, sum) of a one-tile block is there
+    uint64_t* settle = joined + 1;         // [2] giving up: an issuing warp's products
     Plan* plan = reinterpret_cast<Plan*>(smem + L::kPlanAt);
     Item* items = reinterpret_cast<Item*>(smem + L::kItems);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
@@ -501,13 +510,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 5);
-            mbar_init(&pv_done[i], 1), mbar_init(&o_free[i], 4);
+            mbar_init(&o_free[i], 4);
         }
-        for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+        for (int i = 0; i < 4; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&pv_done[i], 1);
         for (int i = 0; i < kRing; i++) {
             mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 2);
             mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 2);
         }
+        mbar_init(mma_item, 2);
+        mbar_init(joined, 4);
+        mbar_init(&settle[0], 1), mbar_init(&settle[1], 1);
         mbar_init(q_full, 1);
         mbar_init(q_empty, 2);
         fence_mbar_init();
@@ -544,41 +556,47 @@ __global__ void __launch_bounds__(kThreads, 1)
             wk.base = plan->first_cost[run];
         }
         int t = 0;
-        for (int k = 0;; k++) {
+        bool ok = true;
+        for (int k = 0; ok; k++) {
             const int slot = k & 1;
-            if (k >= 2) mbar_wait(&item_empty[slot], (uint32_t)(((k >> 1) - 1) & 1), status);
+            if (k >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[slot], (uint32_t)(((k >> 1) - 1) & 1), status));
+            if (!ok) break;
             Item it;
             if (!next_item(c, plan, wk, slices, per, it, lane)) it.b = -1;
             if (lane == 0) {
-                items[slot] = it;
+                items[slot] = it;  // the other lanes go by their own copy
                 mbar_arrive(&item_full[slot]);
             }
             if (it.b < 0) break;
             const bool two = it.ntok > tq;
+            if (k >= 1) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (uint32_t)((k - 1) & 1), status));
+            if (!ok) break;
             if (lane == 0) {
-                if (k >= 1) mbar_wait(q_empty, (uint32_t)((k - 1) & 1), status);
                 mbar_arrive_expect_tx(q_full, (two ? 2u : 1u) * (HD / 64) * (uint32_t)(tq * g) * 128u);
                 for (int w = 0; w < (two ? 2 : 1); w++)
                     for (int x = 0; x < HD / 64; x++)
                         tma_load_3d(smem + L::kQ + w * L::kTile + x * L::kBox, &tmQ, 64 * x, it.h * g, it.tok0 + w * tq,
                                     q_full);
             }
-            load_tiles<HD>(a, tmK, items[slot], smem + L::kK, k_full, k_empty, t, status, lane);
-            t += 2 * (it.j1 - it.j0);
+            ok = load_tiles<HD>(a, tmK, it, &items[slot].poison, smem + L::kK, k_full, k_empty, t, status, lane);
+            if (!ok) mbar_settle(q_full, (uint32_t)(k & 1));
         }
+        if (!ok) settle_ring(k_full, t);
     } else if (warp == 11) {
         // ---------------- TMA of V ----------------
         int t = 0;
-        for (int k = 0;; k++) {
+        bool ok = true;
+        for (int k = 0; ok; k++) {
             const int slot = k & 1;
-            mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
-            const int b = items[slot].b, n = items[slot].j1 - items[slot].j0;
-            if (b >= 0) load_tiles<HD>(a, tmV, items[slot], smem + L::kV, v_full, v_empty, t, status, lane);
+            ok = __all_sync(0xffffffffu, mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status));
+            if (!ok) break;
+            const Item it = items[slot];
+            if (it.b >= 0) ok = load_tiles<HD>(a, tmV, it, &items[slot].poison, smem + L::kV, v_full, v_empty, t, status, lane);
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[slot]);
-            if (b < 0) break;
-            t += 2 * n;
+            if (it.b < 0) break;
         }
+        if (!ok) settle_ring(v_full, t);
     } else if (warp >= 8) {
         // ---------------- MMA issue: one warp per softmax group ----------------
         // Each waits for what is ready early (V, the next K) while its group is still
@@ -615,17 +633,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int kk = 0; kk < BH / 16; kk++)
                     umma_ts(tO, tS + y * BH + kk * 8, desc_advance(vd, kk * 16 * 128), idesc_pv,
                             (!first || kk > 0) ? 1u : 0u);
-                umma_commit(&pv_done[w]);
+                umma_commit(&pv_done[2 * w + y]);
                 umma_commit(&v_empty[c % kRing]);
                 if (alone) umma_commit(&v_empty[c % kRing]);
             }
             __syncwarp();
         };
-        auto wait = [&](uint64_t* bar, int phase) { mbar_wait(bar, (uint32_t)(phase & 1), status); };
+        bool ok = true;  // no wait has run out; the same in every lane
+        auto wait = [&](uint64_t* bar, int phase) {
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)(phase & 1), status));
+        };
         int t = 0, mine = 0, uses = 0;  // half tiles of the CTA; tiles of this group; blocks this group worked on
-        for (int k = 0;; k++) {
+        for (int k = 0; ok; k++) {
             const int slot = k & 1;
             wait(&item_full[slot], k >> 1);
+            if (!ok) break;
             const Item it = items[slot];
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[slot]);
@@ -642,13 +664,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int y = 0; y < 2; y++) {
                     const int c = t + 2 * j0 + y;
                     wait(&k_full[c % kRing], c / kRing);
+                    if (!ok) break;
                     tc_fence_after();
                     qk(qt, c, y, j0 >= solo, own == 1 && y == 1);
                 }
             } else if (lane == 0) {
                 mbar_arrive(q_empty);
             }
-            for (int i = 0; i < own; i++, mine++) {
+            for (int i = 0; i < own && ok; i++, mine++) {
                 const int j = j0 + i * step;
                 const bool more = i + 1 < own;
 #pragma unroll
@@ -660,16 +683,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool now = mbar_test(&v_full[c % kRing], (uint32_t)((c / kRing) & 1)) &
                                      (!(more && two) || mbar_test(&k_full[cn % kRing], (uint32_t)((cn / kRing) & 1))) &
                                      mbar_test(&p_full[2 * w + y], (uint32_t)(mine & 1));
-                    if (!now) {
+                    if (!__all_sync(0xffffffffu, now)) {
                         wait(&v_full[c % kRing], c / kRing);
                         if (more && two) wait(&k_full[cn % kRing], cn / kRing);
                         wait(&p_full[2 * w + y], mine);
                     }
+                    if (!ok) break;
                     tc_fence_after();
                     pv(c, y, j >= solo, i == 0 && y == 0);
                     if (more) {
                         if (!two) {
                             wait(&k_full[cn % kRing], cn / kRing);
+                            if (!ok) break;
                             tc_fence_after();
                         }
                         qk(qt, cn, y, j + step >= solo, i + 2 == own && y == 1);
@@ -678,6 +703,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             t += 2 * n;
             if (own > 0) uses++;
+            // The two go on to the next item together.  A wait by parity must find its phase or
+            // the one before it current, and a group has not looked at the stages that the other
+            // one used alone: here the other has seen all of them full, and none of the next
+            // item's can be given back before both have been here.
+            if (lane == 0) mbar_arrive(mma_item);
+            wait(mma_item, k);
+        }
+        if (!ok) {  // products in flight end before the TMEM and the stages they read are given up
+            if (elect_one()) umma_commit(&settle[w]);
+            __syncwarp();
+            mbar_settle(&settle[w], 0);
         }
     } else {
         // ---------------- softmax ----------------
@@ -700,10 +736,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint4* gstage = reinterpret_cast<uint4*>(smem + L::kStage + w * 4 * 4096);  // 128 rows of 128 bytes
         float2* xs = reinterpret_cast<float2*>(smem + L::kStage + 4 * 4096);  // group 1's (max, sum), one-tile blocks
         const int rt = r / g, rh = r - rt * g;  // the row's token in its tile, and head
-        int t = 0, mine = 0;  // half tiles of the CTA, key tiles of this group
+        int t = 0, mine = 0, joins = 0;  // half tiles of the CTA, key tiles of this group, one-tile blocks joined
+        bool ok = true;                  // no wait of this thread has run out: then nothing more is stored
         for (int k = 0;; k++) {
             const int slot = k & 1;
-            mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
+            if (ok) ok = mbar_wait(&item_full[slot], (uint32_t)((k >> 1) & 1), status);
+            // the group goes on together, with an item that all of it has, or not at all
+            if (!named_bar_all(1 + w, 128, ok)) break;
             const Item it = items[slot];
             if (it.b < 0) break;
             const bool two = it.ntok > tq;
@@ -720,17 +759,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int j = two ? i : 2 * i + w, base = (it.j0 + j) * BN;
 #pragma unroll 1
                 for (int y = 0; y < 2; y++) {
-                    mbar_wait(&s_full[2 * w + y], (uint32_t)(mine & 1), status);
+                    if (ok) ok = mbar_wait(&s_full[2 * w + y], (uint32_t)(mine & 1), status);
                     tc_fence_after();
                     const int hb = base + y * BH;
-                    // phase of the products before this half's: 2 mine + y - 1
+                    // the products before this half's: the other half's of this tile, or of the one before
                     if (live)
                         softmax_half<T, HD>(tS + y * BH, tO, i == 0 && y == 0, lim - hb, hb + BH > lim_lo, scale, m, l,
-                                            [&] { mbar_wait(&pv_done[w], (uint32_t)((y + 1) & 1), status); });
+                                            [&] { if (ok) ok = mbar_wait(&pv_done[2 * w + (y ^ 1)], (uint32_t)((mine + y + 1) & 1), status); });
                     if (hb + BH > it.len) {
                         // rows past the sequence hold anything: their V must not meet the zero weights as a NaN
                         const int cc = t + 2 * j + y, s = cc % kRing;
-                        mbar_wait(&v_full[s], (uint32_t)((cc / kRing) & 1), status);
+                        if (ok) ok = mbar_wait(&v_full[s], (uint32_t)((cc / kRing) & 1), status);
                         for (int e = r; e < BH * 8 * (HD / 64); e += 128) {
                             const int row = (e >> 3) & (BH - 1), x = e >> 9;
                             if (hb + row >= it.len)
@@ -750,7 +789,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             named_bar_sync(1 + w, 128);  // every warp of the group has read the item
             if (r == 0) mbar_arrive(&item_empty[slot]);
             if (n_own > 0) {
-                mbar_wait(&pv_done[w], 1u, status);  // an odd phase: a tile's second half
+                for (int y = 0; y < 2; y++)
+                    if (ok) ok = mbar_wait(&pv_done[2 * w + y], (uint32_t)((mine - 1) & 1), status);
                 tc_fence_after();
             }
             const bool join = !two && n > 1;
@@ -760,13 +800,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     named_bar_sync(2, 128);  // the stage, where xs lies, has been read
                     xs[r] = make_float2(m, l);
                     tc_fence_before();
-                    named_bar_arrive(3, 256);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(joined);
                 }
                 continue;
             }
             float w0 = 1.f, w1 = 0.f;
             if (join) {
-                named_bar_sync(3, 256);
+                if (ok) ok = mbar_wait(joined, (uint32_t)(joins & 1), status);
+                joins++;
                 tc_fence_after();
                 const float2 o = xs[r];
                 const float M = fmaxf(m, o.x);
@@ -807,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             };
             const int row = w * BM + r;  // of the block's two tiles (one-tile blocks: w is 0)
-            if (part && valid) c.part_ml[(size_t)it.slot * kPartRows + row] = make_float2(m, l);
+            if (part && valid && ok) c.part_ml[(size_t)it.slot * kPartRows + row] = make_float2(m, l);
             const bool f32 = part || a.out_dtype == PICOATTN_DTYPE_F32;
             // A tile whose rows are all valid, or any part (its other rows are scratch), leaves by
             // one TMA store per 128 bytes of its rows, from a swizzled stage of the group; the rows
@@ -842,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         gstage[r * 8 + (u ^ (r & 7))] = make_uint4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
                     fence_proxy_async_shared();
                     named_bar_sync(1 + w, 128);
-                    if (r == 0) {
+                    if (r == 0 && ok) {
                         if (part) tma_store_2d(&tmP, gstage, col, it.slot * kPartRows + w * BM);
                         else tma_store_3d(&tmO, gstage, col, it.h * g, it.tok0 + w * tq);
                         bulk_commit_group();
@@ -851,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else {
                     if (col == 0) named_bar_sync(1 + w, 128);
                     store_rows(x, gstage + (warp & 3) * 256, static_cast<uint8_t*>(a.out) + col * (f32 ? 4 : 2),
-                               valid ? orow * (f32 ? 4 : 2) : -1, lane);
+                               valid && ok ? orow * (f32 ? 4 : 2) : -1, lane);
                 }
             }
         }

@@ -446,6 +446,64 @@ def test_attention_of_no_new_tokens(rt):
     assert (y == 7).all() and B.batch.status() == 0
 
 
+def gpu_attn(B, layer, q):
+    """The 64-bit form on the GPU, for batches too large for want_attn, with its error bound's main terms: the weights'
+    rounding (u |v| weighted), and a score error of hd 2^-23 sum|q k|; 2^-16 for the fp32 sums of up to 16,384 rows
+    (n / 8 additions of 2^-23, twice) and the exponential."""
+    out = torch.zeros((B.n_tok, B.hq, B.hd), dtype=torch.float64, device="cuda")
+    err = torch.zeros_like(out)
+    g = B.hq // B.hkv
+    for b, (n, t) in enumerate(zip(B.new, B.total)):
+        if n == 0:
+            continue
+        k, v = (B.rows(p, layer, b, t).double() for p in (B.cache.k_pool, B.cache.v_pool))
+        x = q[B.start[b]:B.start[b] + n].double()
+        hidden = torch.arange(t, device="cuda") > (t - n + torch.arange(n, device="cuda"))[:, None]
+        for h in range(B.hq):
+            s = (x[:, h] @ k[:, h // g].T) * B.hd ** -0.5
+            mag = (x[:, h].abs() @ k[:, h // g].abs().T).amax(-1, keepdim=True) * B.hd ** -0.5
+            p = s.masked_fill(hidden, -np.inf).softmax(-1)
+            out[B.start[b]:B.start[b] + n, h] = p @ v[:, h // g]
+            w, most = p @ v[:, h // g].abs(), v[:, h // g].abs().max()
+            # weights below the type's normal range are off by TINY each, of a sum of at least 1
+            err[B.start[b]:B.start[b] + n, h] = (HALF[B.dt] + 2 * B.hd * 2.0 ** -23 * mag + 2.0 ** -16) * w + \
+                t * TINY[B.dt] * most
+    return out, err
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_random_batches_one_after_the_other(rt, seed):
+    """Two ragged batches of other shapes, run in turn without waiting: every call's outputs against the 64-bit form."""
+    import random
+    rng = random.Random(seed)
+    two = []
+    for i in range(2):
+        hq, hkv, hd = rng.choice([(32, 4, 64), (14, 2, 64), (28, 4, 128), (32, 8, 128), (40, 8, 128), (6, 3, 64)])
+        ones, chunks = (rng.randrange(0, 30), rng.randrange(1, 4)) if (seed + i) % 4 else (rng.randrange(1, 40), 0)
+        new = [1] * ones + [rng.randrange(2, 400) for _ in range(chunks)]
+        rng.shuffle(new)
+        past = [rng.randrange(0, 2000) for _ in new]
+        B = Batch(rt, new, past, hq, hkv, hd, rng.choice([16, 32, 64, 128, 256]), rng.choice(["f16", "bf16"]), layers=1,
+                  pad=rng.randrange(3), seed=seed)
+        B.fill(0)
+        B.q = B.rand(B.n_tok, hq, hd).to(B.dt)
+        B.outs = [torch.full((B.n_tok, hq, hd), float("nan"), device="cuda", dtype=B.dt) for _ in range(6)]
+        two.append(B)
+    torch.cuda.synchronize()
+    for r in range(6):
+        for B in two:
+            B.cache.attend(0, B.batch, B.q, B.outs[r])
+    for B in two:
+        assert B.batch.status() == 0
+        want, err = gpu_attn(B, 0, B.q)
+        tol = err + HALF[B.dt] * (want.abs() + err) + TINY[B.dt]
+        for r, y in enumerate(B.outs):
+            d = (y.double() - want).abs()[:B.start[-1]]
+            bad = ~(d <= tol[:B.start[-1]])
+            assert not bad.any(), (f"run {r}: {int(bad.sum())} off, worst {float((d / tol[:B.start[-1]]).max()):.3g} of the "
+                                   f"tolerance, first at {bad.nonzero()[0].tolist()}")
+
+
 def test_many_sequences(rt):
     """More sequences than a block has threads, some of them empty."""
     n = 1500
