@@ -1,15 +1,15 @@
-// paged_few.cu -- paged attention of sequences with few query rows: at most 16
-// rows (new tokens x q heads of a KV head) per KV head, single tokens and drafts.
+// paged_few.cu -- paged attention of sequences with few query rows (new tokens x q
+// heads of a KV head): single tokens and drafts, up to 32 rows.
 //
 // Bound by HBM: each K and V row is read once for all the q heads and new tokens
-// that share it, ~4 * 16 flop per two bytes.  A stream is the rows of one KV head
+// that share it, 64 flop or more per two bytes.  A stream is the rows of one KV head
 // of one sequence; all streams are concatenated in units of 16 rows and cut into
-// equal slices, one per CTA (two CTAs per SM), so every CTA moves the same bytes
-// whatever the mix of lengths.  A producer warp copies tiles of 64 or 128 rows
-// into a three-stage ring (bulk copies of at most 16 rows: inside a page); four
-// warps take 16 keys of a tile each: S = Q K^T by m16n8k16 products (the 16 query
-// rows are the M side), online softmax in fp32 registers in the log2 domain,
-// O += P V.  The four warps' (max, sum, O) are joined in shared memory at the end
+// equal slices, one per CTA, so every CTA moves the same bytes whatever the mix of
+// lengths.  A producer warp copies tiles of 64 or 128 rows into a ring (bulk
+// copies of at most 16 rows: inside a page); for each 16 query rows four warps take
+// 16 keys of a tile each: S = Q K^T by m16n8k16 products (the query rows are the M
+// side), online softmax in fp32 registers in the log2 domain, O += P V.  The four
+// warps' (max, sum, O) are joined in shared memory at the end
 // of a stream's part; a stream inside one slice is written as output, the parts
 // of others go to the workspace and a merge kernel joins them.
 #include <algorithm>
@@ -21,36 +21,45 @@ namespace picoattn {
 
 namespace {
 
-constexpr int kRows = 16;      // query rows (M of the products)
 constexpr int kUnit = 16;      // cache rows per unit
-constexpr int kWarps = 4;      // compute warps
-constexpr int kThreads = 32 * (kWarps + 1);
-constexpr int kStages = 3;
+constexpr int kKeyWarps = 4;   // warps that share the keys of a tile
+constexpr int kMostRows = 32;
+constexpr long long kTwoGroupBytes = 128ll << 20;
+constexpr int kMaxParts = 512;  // most CTAs of the attention kernel
+constexpr int kSlots = kMaxParts * kMostRows;  // partial rows in the workspace: two parts of each CTA
 constexpr int kWholeBytes = 256 << 10;
 constexpr int kMinUnits = 4;   // least units per CTA: a slice shorter than a tile gains nothing
 
-template <int HD>
+// MT: groups of 16 query rows.  One: two CTAs per SM with a ring of three stages;
+// two: one CTA with a ring of six.
+template <int HD, int MT>
 struct Few {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kWarps = kKeyWarps * MT;         // compute warps
+    static constexpr int kThreads = 32 * (kWarps + 1);
+    static constexpr int kCtas = MT == 1 ? 2 : 1;         // per SM
+    static constexpr int kMaxCtas = MT == 1 ? kMaxParts : kMaxParts / 2;
+    static constexpr int kStages = MT == 1 ? 3 : 6;
     static constexpr int T = 8192 / HD;        // cache rows per tile: 16 KB of K
     static constexpr int GR = T / 8;           // a tile is 8 groups of GR rows, each padded by 16 bytes
     static constexpr int ROW = HD * 2;
     static constexpr int GS = GR * ROW + 16;   // group stride: 8 rows of a product, one per group, on 8 bank quads
     static constexpr int TILE = 8 * GS;
     static constexpr int RG = T / 16;          // 16-key groups per tile
-    static constexpr int off_prefix = 128;     // [kThreads + 1] first unit of each thread's sequences
+    static constexpr int off_prefix = 384;     // [kThreads + 1] first unit of each thread's sequences
     static constexpr int off_ml = off_prefix + 8 * (kThreads + 1) + 8;  // [kWarps][16] (max, sum)
-    static constexpr int off_join = off_ml + 8 * kWarps * kRows;
+    static constexpr int off_join = (off_ml + 8 * kWarps * 16 + 15) / 16 * 16;
     static constexpr int JS = 36;              // floats per row of the join buffer (32 columns, padded)
-    static constexpr int off_tiles = (off_join + 4 * kWarps * kRows * JS + 127) / 128 * 128;
+    static constexpr int off_tiles = (off_join + 4 * kWarps * 16 * JS + 127) / 128 * 128;
     static constexpr int bytes = off_tiles + kStages * 2 * TILE;
-    static_assert(2 * (bytes + 1024) <= 228 * 1024, "two CTAs per SM");
+    static_assert(kCtas * (bytes + 1024) <= 228 * 1024, "CTAs per SM");
 };
 
 struct FewArgs {
     PagedAttnArgs a;
     long long* prefix;  // [n_seqs + 1] first unit of each sequence
-    float2* part_ml;    // [2 * grid][16]
-    float* part_o;      // [2 * grid][16][hd]
+    float2* part_ml;    // [2 * grid][rows]
+    float* part_o;      // [2 * grid][rows][hd]
     int whole;          // a stream per CTA: nothing is cut, nothing merged
 };
 
@@ -131,16 +140,17 @@ __device__ __forceinline__ void nan_rows(const PagedAttnArgs& a, int b, int h, i
                           make_float4(nan, nan, nan, nan));
 }
 
-template <class T, int HD>
-__global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
-    using F = Few<HD>;
+template <class T, int HD, int MT>
+__global__ void __launch_bounds__(Few<HD, MT>::kThreads, Few<HD, MT>::kCtas) paged_few_kernel(FewArgs fa) {
+    using F = Few<HD, MT>;
+    constexpr int kRows = F::kRows, kWarps = F::kWarps, kThreads = F::kThreads, kStages = F::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     const PagedAttnArgs& a = fa.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem);
     uint64_t* empty = full + kStages;
     int* poison = reinterpret_cast<int*>(empty + kStages);  // [kStages] the tile read a page that does not exist
-    long long* warp_tot = reinterpret_cast<long long*>(smem + 64);  // [kWarps + 1]
+    long long* warp_tot = reinterpret_cast<long long*>(smem + 192);  // [kWarps + 1]
     long long* chunk = reinterpret_cast<long long*>(smem + F::off_prefix);
     float2* ml = reinterpret_cast<float2*>(smem + F::off_ml);
     float* join = reinterpret_cast<float*>(smem + F::off_join);
@@ -243,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
     }
 
     // ---------------- compute warps ----------------
-    const int gid = lane >> 2, tig = lane & 3;
+    const int gid = lane >> 2, tig = lane & 3, kw = warp % kKeyWarps, mt = warp / kKeyWarps;
     // ldmatrix rows (matrix lane >> 3, its row lane & 7 = tile group): K (keys 0-7 | dims 0-7, keys 0-7 | dims 8-15,
     // keys 8-15 | ..), V transposed (keys 0-7 | dims 0-7, keys 8-15 | dims 0-7, ..); key 8j + q of 16-key group rg is
     // tile row GR q + 2 rg + j
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
         int lim[2];  // keys below it are visible to the lane's rows gid, gid + 8
 #pragma unroll
         for (int half = 0; half < 2; half++) {
-            const int r = gid + 8 * half;
+            const int r = 16 * mt + gid + 8 * half;
             const int i = r / a.g;
             lim[half] = sp.len - sp.n + i + 1;
             const uint32_t* src = reinterpret_cast<const uint32_t*>(
@@ -283,11 +293,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
             const bool mask = row0 + F::T > sp.len - sp.n + 1 || valid < F::T;
             const int lim0 = min(lim[0] - row0, valid), lim1 = min(lim[1] - row0, valid);
 #pragma unroll
-            for (int rg = warp; rg < F::RG; rg += kWarps) {
+            for (int rg = kw; rg < F::RG; rg += kKeyWarps) {
                 if (2 * rg >= valid) continue;
                 if (valid < F::T) {
                     // rows past the part hold anything: their V must not meet the zero weights as a NaN.  This warp
-                    // alone reads the rows of its key groups
+                    // alone reads the rows of its key groups, or with the same warps of the other query rows, which
+                    // write the same zeros
                     for (int e = lane; e < 16 * (F::ROW / 16); e += 32) {
                         const int key = e / (F::ROW / 16), q = key & 7, u = 2 * rg + (key >> 3);
                         if (F::GR * q + u >= valid)
@@ -357,28 +368,30 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
             if (lane == 0) mbar_arrive(&empty[s]);
         }
 
-        // join the four warps' (max, sum, O): thread (row tid / 8, four columns)
+        // join the key warps' (max, sum, O): thread (row tid / 8, four columns)
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-            if (tig == 0) ml[warp * kRows + gid + 8 * half] = make_float2(m[half], l[half]);
+            if (tig == 0) ml[warp * 16 + gid + 8 * half] = make_float2(m[half], l[half]);
         }
         named_bar_sync(1, 32 * kWarps);
         float wgt[2];
 #pragma unroll
         for (int half = 0; half < 2; half++) {
-            float M = ml[gid + 8 * half].x;
+            const float2* x = ml + mt * kKeyWarps * 16 + gid + 8 * half;
+            float M = x[0].x;
 #pragma unroll
-            for (int w = 1; w < kWarps; w++) M = fmaxf(M, ml[w * kRows + gid + 8 * half].x);
+            for (int w = 1; w < kKeyWarps; w++) M = fmaxf(M, x[w * 16].x);
             wgt[half] = ex2(m[half] - M);
         }
         const int jr = tid >> 3, jc = (tid & 7) * 4;
-        float M = ml[jr].x, Ls = 0.f;
+        const int jw = (jr >> 4) * kKeyWarps * 16 + (jr & 15);  // the row in its first key warp's 16
+        float M = ml[jw].x, Ls = 0.f;
 #pragma unroll
-        for (int w = 1; w < kWarps; w++) M = fmaxf(M, ml[w * kRows + jr].x);
+        for (int w = 1; w < kKeyWarps; w++) M = fmaxf(M, ml[jw + w * 16].x);
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) Ls += ml[w * kRows + jr].y * ex2(ml[w * kRows + jr].x - M);
+        for (int w = 0; w < kKeyWarps; w++) Ls += ml[jw + w * 16].y * ex2(ml[jw + w * 16].x - M);
         const bool whole = u0 == 0 && u1 == stream_units;
         const size_t slot = 2 * (size_t)blockIdx.x + (u0 == 0 ? 1 : 0);
         const int ji = jr / a.g;
@@ -388,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
         for (int c = 0; c < HD / 32; c++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float* d = join + (warp * kRows + gid) * F::JS + 8 * i + 2 * tig;
+                float* d = join + (warp * 16 + gid) * F::JS + 8 * i + 2 * tig;
                 *reinterpret_cast<float2*>(d) = make_float2(o[4 * c + i][0] * wgt[0], o[4 * c + i][1] * wgt[0]);
                 *reinterpret_cast<float2*>(d + 8 * F::JS) = make_float2(o[4 * c + i][2] * wgt[1], o[4 * c + i][3] * wgt[1]);
             }
@@ -396,8 +409,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
             if (jr < rows) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) {
-                    const float4 x = *reinterpret_cast<const float4*>(join + (w * kRows + jr) * F::JS + jc);
+                for (int w = 0; w < kKeyWarps; w++) {
+                    const float4 x = *reinterpret_cast<const float4*>(join + (jw + w * 16) * F::JS + jc);
                     v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
                 }
                 if (whole) {
@@ -418,10 +431,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_few_kernel(FewArgs fa) {
 // once: the merge is one round trip to L2.  Rows of a sequence outside the
 // host's bounds become NaN here.
 constexpr int kMergeThreads = 128;
-constexpr int kMaxParts = 512;  // most CTAs of the attention kernel; sizes the workspace
 
 template <class T, int HD>
-__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs fa, int grid) {
+__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs fa, int grid, int rows) {
     constexpr int C4 = HD / 4, NG = kMergeThreads / C4, RPT = 40 / NG;
     __shared__ float w_s[kMaxParts], red[kMergeThreads / 32][2];
     __shared__ float4 acc_s[kMergeThreads];
@@ -444,7 +456,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     const int parts = hi - lo + 1;
     auto slot = [&](int p) -> size_t {  // the first part begins its stream, the others are their CTA's first
         const bool begins = p == 0;
-        return ((size_t)(lo + p) * 2 + (begins ? 1 : 0)) * kRows + r;
+        return ((size_t)(lo + p) * 2 + (begins ? 1 : 0)) * rows + r;
     };
     float4 v[RPT];
 #pragma unroll
@@ -503,12 +515,12 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     }
 }
 
-template <class T, int HD>
-cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
-    using F = Few<HD>;
+template <class T, int HD, int MT>
+cudaError_t launch_rows(const PagedAttnArgs& a, cudaStream_t stream) {
+    using F = Few<HD, MT>;
     static PerDeviceOnce setup;
     cudaError_t e = setup.run([] {
-        return cudaFuncSetAttribute(paged_few_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::bytes);
+        return cudaFuncSetAttribute(paged_few_kernel<T, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::bytes);
     });
     if (e != cudaSuccess) return e;
     FewArgs fa{};
@@ -518,27 +530,45 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     // kernel is then not launched at all (one token over 512 rows of 4 KV heads of
     // 64: 8.0 us cut, 6.2 whole).
     fa.whole = (long long)a.b.max_len * HD * 4 <= kWholeBytes;
+    auto kernel = paged_few_kernel<T, HD, MT>;
     if (fa.whole)
-        return launch_pdl(paged_few_kernel<T, HD>, dim3(a.b.n_seqs * a.hkv), dim3(kThreads), (size_t)F::bytes, stream, fa);
+        return launch_pdl(kernel, dim3(a.b.n_seqs * a.hkv), dim3(F::kThreads), (size_t)F::bytes, stream, fa);
     const long long units = (long long)a.b.n_seqs * a.hkv * ((a.b.max_len + kUnit - 1) / kUnit);
-    const int grid = (int)std::min<long long>(std::min(2 * device_sm_count(), kMaxParts), (units + kMinUnits - 1) / kMinUnits);
+    const int grid = (int)std::min<long long>(std::min(F::kCtas * device_sm_count(), F::kMaxCtas),
+                                              (units + kMinUnits - 1) / kMinUnits);
+    static_assert(2 * F::kMaxCtas * F::kRows <= kSlots, "workspace");
     fa.part_ml = reinterpret_cast<float2*>(a.ws);
-    fa.part_o = reinterpret_cast<float*>(a.ws + (size_t)2 * kMaxParts * kRows * 8);
-    fa.prefix = reinterpret_cast<long long*>(a.ws + (size_t)2 * kMaxParts * kRows * (8 + 4 * HD));
-    e = launch_pdl(paged_few_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)F::bytes, stream, fa);
+    fa.part_o = reinterpret_cast<float*>(a.ws + (size_t)kSlots * 8);
+    fa.prefix = reinterpret_cast<long long*>(a.ws + (size_t)kSlots * (8 + 4 * HD));
+    e = launch_pdl(kernel, dim3(grid), dim3(F::kThreads), (size_t)F::bytes, stream, fa);
     if (e != cudaSuccess) return e;
     return launch_pdl(paged_few_merge_kernel<T, HD>, dim3(a.b.max_new * a.g, a.b.n_seqs * a.hkv), dim3(kMergeThreads), 0,
-                      stream, fa, grid);
+                      stream, fa, grid, F::kRows);
+}
+
+template <class T, int HD>
+cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
+    const int rows = a.b.max_new * a.g;
+    return rows <= 16 ? launch_rows<T, HD, 1>(a, stream) : launch_rows<T, HD, 2>(a, stream);
 }
 
 }  // namespace
 
+// Up to 16 rows this kernel reads the cache at the memory's rate.  A second group
+// of 16 rows doubles the products and the softmax per byte: it is then bound by
+// them at 1.2 TB/s (hd 128) to 4 TB/s, but starts sooner than the chunk kernel,
+// so it takes what is short: 24 rows over 2,000 keys of 4 x 64 12.2 us against
+// 18.8, 28 rows over 9 sequences of 3,500 of 4 x 128 26 against 30; over 32 of
+// 4,000 (260 MB) 63 against 55.  Four groups (35 rows and up) were slower on the
+// whole: 18 against 13 us for one sequence of 300, 53 against 30 for 9 of 3,500.
 bool paged_few_fits(const PagedAttnArgs& a) {
-    return (long long)a.b.max_new * a.g <= kRows && (long long)a.b.n_seqs * a.hkv <= 65535;
+    const long long rows = (long long)a.b.max_new * a.g, streams = (long long)a.b.n_seqs * a.hkv;
+    if (streams > 65535) return false;
+    return rows <= 16 || (rows <= kMostRows && streams * a.b.max_len * a.hd * 4 <= kTwoGroupBytes);
 }
 
 size_t paged_few_bytes(int hd, int n_seqs) {
-    return align_up((size_t)2 * kMaxParts * kRows * (8 + 4 * hd) + (size_t)(n_seqs + 1) * 8, 256);
+    return align_up((size_t)kSlots * (8 + 4 * hd) + (size_t)(n_seqs + 1) * 8, 256);
 }
 
 cudaError_t launch_paged_few(const PagedAttnArgs& a, cudaStream_t stream) {
