@@ -7,7 +7,7 @@ namespace picoattn {
 
 // Both paths keep their partial results in the same place: a call runs one of them.
 size_t paged_workspace_bytes(const picoattn_config_t& cfg, int n_seqs) {
-    return kWsHeaderBytes + align_up(std::max(paged_few_bytes(cfg.head_dim, n_seqs), paged_chunk_bytes(cfg.head_dim)), 256);
+    return kWsHeaderBytes + align_up(std::max(paged_few_bytes(cfg.head_dim), paged_chunk_bytes(cfg.head_dim)), 256);
 }
 
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t stream) {

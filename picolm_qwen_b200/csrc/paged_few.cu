@@ -5,14 +5,21 @@
 // that share it, 64 flop or more per two bytes.  A stream is the rows of one KV head
 // of one sequence; all streams are concatenated in units of 16 rows and cut into
 // equal slices, one per CTA, so every CTA moves the same bytes whatever the mix of
-// lengths.  A producer warp copies tiles of 64 or 128 rows into a ring (bulk
-// copies of at most 16 rows: inside a page); for each 16 query rows four warps take
-// 16 keys of a tile each: S = Q K^T by m16n8k16 products (the query rows are the M
-// side), online softmax in fp32 registers in the log2 domain, O += P V.  The four
-// warps' (max, sum, O) are joined in shared memory at the end
-// of a stream's part; a stream inside one slice is written as output, the parts
-// of others go to the workspace and a merge kernel joins them.
+// lengths (a cut near a stream's end moves there).  A producer warp copies tiles of
+// 64 or 128 rows into a ring (bulk copies of at most 16 rows: inside a page); for
+// each 16 query rows four warps take 16 keys of a tile each: S = Q K^T by m16n8k16
+// products (the query rows are the M side), online softmax in fp32 registers in the
+// log2 domain, O += P V.  The four warps' (max, sum, O) are joined in shared memory
+// at the end of a stream's part; a stream inside one slice is written as output, the
+// parts of others go to the workspace and a merge kernel joins them.
+//
+// Measured, f16: one token of 64 sequences of 1,025 to 8,193 rows of 4 x 128 105 us
+// (5.7 TB/s), three of one sequence of 131,072 rows of 8 x 128 90 us (5.9 TB/s, 0.91
+// of the copy rate); one token over 512 rows of 4 x 64 6.4 us.  What is left of the
+// batch's time over its bytes: the plan and first loads (2 us), a CTA's second part
+// (1.7 us), the merge kernel and the tail of the slices (3 to 4 us).
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "paged_common.cuh"
@@ -27,7 +34,7 @@ constexpr int kMostRows = 32;
 constexpr long long kTwoGroupBytes = 128ll << 20;
 constexpr int kMaxParts = 512;  // most CTAs of the attention kernel
 constexpr int kSlots = kMaxParts * kMostRows;  // partial rows in the workspace: two parts of each CTA
-constexpr int kWholeBytes = 256 << 10;
+constexpr int kSnapBytes = 64 << 10;
 constexpr int kMinUnits = 4;   // least units per CTA: a slice shorter than a tile gains nothing
 
 // MT: groups of 16 query rows.  One: two CTAs per SM with a ring of three stages;
@@ -38,6 +45,10 @@ struct Few {
     static constexpr int kWarps = kKeyWarps * MT;         // compute warps
     static constexpr int kThreads = 32 * (kWarps + 1);
     static constexpr int kCtas = MT == 1 ? 2 : 1;         // per SM
+    // Two CTAs have three warps on a quarter SM: 144 registers leave room there for a warp of the merge kernel, which
+    // then starts while they finish (two sequences of 5,000 rows of 4 x 64: 12.8 us, with 152 registers 14.3).  At hd 128
+    // its 72 registers would fit too, but 144 spill (2 us slower on the same sequences of 8 x 128).
+    static constexpr int kRegs = HD == 64 ? 144 : 168;
     static constexpr int kMaxCtas = MT == 1 ? kMaxParts : kMaxParts / 2;
     static constexpr int kStages = MT == 1 ? 3 : 6;
     static constexpr int T = 8192 / HD;        // cache rows per tile: 16 KB of K
@@ -46,8 +57,7 @@ struct Few {
     static constexpr int GS = GR * ROW + 16;   // group stride: 8 rows of a product, one per group, on 8 bank quads
     static constexpr int TILE = 8 * GS;
     static constexpr int RG = T / 16;          // 16-key groups per tile
-    static constexpr int off_prefix = 384;     // [kThreads + 1] first unit of each thread's sequences
-    static constexpr int off_ml = off_prefix + 8 * (kThreads + 1) + 8;  // [kWarps][16] (max, sum)
+    static constexpr int off_ml = 256;         // [kWarps][16] (max, sum)
     static constexpr int off_join = (off_ml + 8 * kWarps * 16 + 15) / 16 * 16;
     static constexpr int JS = 36;              // floats per row of the join buffer (32 columns, padded)
     static constexpr int off_tiles = (off_join + 4 * kWarps * 16 * JS + 127) / 128 * 128;
@@ -57,10 +67,10 @@ struct Few {
 
 struct FewArgs {
     PagedAttnArgs a;
-    long long* prefix;  // [n_seqs + 1] first unit of each sequence
+    int4* cut;          // streams for the merge kernel: (stream, its first CTA, its parts)
     float2* part_ml;    // [2 * grid][rows]
     float* part_o;      // [2 * grid][rows][hd]
-    int whole;          // a stream per CTA: nothing is cut, nothing merged
+    int by_cta;         // `cut` has an entry for each CTA (the stream that begins there and goes on), else for each stream
 };
 
 __device__ __forceinline__ long long seq_units(const SeqSpan& s, int hkv) {
@@ -77,6 +87,20 @@ __device__ __forceinline__ int cta_of(long long unit, long long units, int ctas)
     while (i + 1 < ctas && first_unit(i + 1, units, ctas) <= unit) i++;
     while (i > 0 && first_unit(i, units, ctas) > unit) i--;
     return i;
+}
+// A cut this near to a stream's end moves there: a second part costs a CTA 1.7 us
+// (its Q rows, the join), 64 KB more of the cache up to 1 us.  Less than half a
+// slice, so that no two cuts meet.
+template <int HD>
+__device__ __forceinline__ int most_moved(long long units, int ctas) {
+    return (int)min((long long)(kSnapBytes / (kUnit * 4 * HD)), quotient(units, ctas) / 2);
+}
+struct Cut {
+    int b;                // the sequence
+    long long from, at;   // its first unit, the cut's
+};
+__device__ __forceinline__ long long moved(long long cut, long long s0, long long s1, int most) {
+    return cut - s0 <= most ? s0 : (s1 - cut <= most ? s1 : cut);
 }
 
 template <class T>
@@ -127,21 +151,22 @@ __device__ __forceinline__ void for_each_part(const PagedAttnArgs& a, int b0, lo
     }
 }
 
-// NaN into the rows of a sequence outside the host's bounds, those of KV head h
-// that are i, i + n, ... (as far as they lie in out).
+// NaN into the rows of KV head h of a sequence outside the host's bounds (as far
+// as they lie in out).
 template <class T, int HD>
-__device__ __forceinline__ void nan_rows(const PagedAttnArgs& a, int b, int h, int i, int n, int tid, int threads) {
+__device__ __forceinline__ void nan_rows(const PagedAttnArgs& a, int b, int h, int tid, int threads) {
     constexpr int C4 = HD / 4;
     const int t0 = max(a.b.q_start[b], 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
     const float nan = __int_as_float(0x7fc00000);
-    for (long long x = i; x < (long long)(t1 - t0) * a.g; x += n)
-        for (int c = tid; c < C4; c += threads)
-            store_out4<T>(a, ((size_t)(t0 + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * c,
-                          make_float4(nan, nan, nan, nan));
+    for (long long i = tid; i < (long long)(t1 - t0) * a.g * C4; i += threads) {
+        const long long x = i / C4;
+        store_out4<T>(a, ((size_t)(t0 + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * (i % C4),
+                      make_float4(nan, nan, nan, nan));
+    }
 }
 
-template <class T, int HD, int MT>
-__global__ void __launch_bounds__(Few<HD, MT>::kThreads, Few<HD, MT>::kCtas) paged_few_kernel(FewArgs fa) {
+template <class T, int HD, int MT, bool kWhole>
+__global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
     using F = Few<HD, MT>;
     constexpr int kRows = F::kRows, kWarps = F::kWarps, kThreads = F::kThreads, kStages = F::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -150,8 +175,8 @@ __global__ void __launch_bounds__(Few<HD, MT>::kThreads, Few<HD, MT>::kCtas) pag
     uint64_t* full = reinterpret_cast<uint64_t*>(smem);
     uint64_t* empty = full + kStages;
     int* poison = reinterpret_cast<int*>(empty + kStages);  // [kStages] the tile read a page that does not exist
-    long long* warp_tot = reinterpret_cast<long long*>(smem + 192);  // [kWarps + 1]
-    long long* chunk = reinterpret_cast<long long*>(smem + F::off_prefix);
+    long long* warp_tot = reinterpret_cast<long long*>(smem + 176);  // [kWarps + 1]
+    Cut* cuts = reinterpret_cast<Cut*>(smem + 128);  // [2]
     float2* ml = reinterpret_cast<float2*>(smem + F::off_ml);
     float* join = reinterpret_cast<float*>(smem + F::off_join);
     uint8_t* tiles = smem + F::off_tiles;
@@ -164,26 +189,27 @@ __global__ void __launch_bounds__(Few<HD, MT>::kThreads, Few<HD, MT>::kCtas) pag
     pdl_wait();
     int b0;
     long long base, c0, c1;
-    if (fa.whole) {  // a stream per CTA
+    if constexpr (kWhole) {  // a stream per CTA
         b0 = (int)(blockIdx.x / (unsigned)a.hkv);
         const int h = (int)blockIdx.x - b0 * a.hkv;
         const SeqSpan sp = seq_span(a.b, b0);
         if (!sp.ok) {
             if (h == 0 && tid == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
-            nan_rows<T, HD>(a, b0, h, 0, 1, tid, kThreads);
+            nan_rows<T, HD>(a, b0, h, tid, kThreads);
         }
         if (!sp.ok || sp.n == 0) return;
         const int per_head = (sp.len + kUnit - 1) / kUnit;
         base = 0, c0 = (long long)h * per_head, c1 = c0 + per_head;
         __syncthreads();  // the barriers
     } else {
-        // first units of every thread's sequences
+        // the units of each thread's sequences, and of those before them
         const int per = (a.b.n_seqs + kThreads - 1) / kThreads;
         const int lo = min(tid * per, a.b.n_seqs), hi = min(lo + per, a.b.n_seqs);
         long long mine = 0;
+        bool bad = false;
         for (int b = lo; b < hi; b++) {
             const SeqSpan sp = seq_span(a.b, b);
-            if (!sp.ok && blockIdx.x == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+            bad |= !sp.ok;
             mine += seq_units(sp, a.hkv);
         }
         long long incl = mine;
@@ -192,39 +218,64 @@ __global__ void __launch_bounds__(Few<HD, MT>::kThreads, Few<HD, MT>::kCtas) pag
             if (lane >= o) incl += v;
         }
         if (lane == 31) warp_tot[warp] = incl;
-        __syncthreads();
-        long long first = incl - mine;
-        for (int w = 0; w < warp; w++) first += warp_tot[w];
-        chunk[tid] = first;
-        if (tid == kThreads - 1) chunk[kThreads] = first + mine;
-        if (blockIdx.x == 0) {  // for the merge kernel
-            long long run = first;
-            for (int b = lo; b < hi; b++) {
-                fa.prefix[b] = run;
-                run += seq_units(seq_span(a.b, b), a.hkv);
-            }
-            if (tid == kThreads - 1) fa.prefix[a.b.n_seqs] = first + mine;
+        if (tid == 0 && fa.by_cta) fa.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        bad = __syncthreads_or(bad);
+        long long first = incl - mine, units = 0;
+        for (int w = 0; w <= kWarps; w++) {
+            units += warp_tot[w];
+            if (w < warp) first += warp_tot[w];
         }
-        __syncthreads();
-        const long long units = chunk[kThreads];
         const int ctas = ctas_used(units, gridDim.x);
-        if ((int)blockIdx.x >= ctas) return;
-        c0 = first_unit(blockIdx.x, units, ctas), c1 = first_unit(blockIdx.x + 1, units, ctas);
-        int l = 0, h = kThreads;  // the last thread whose first unit is <= c0
-        while (h - l > 1) {
-            const int mid = (l + h) >> 1;
-            if (chunk[mid] <= c0) l = mid;
-            else h = mid;
+        if ((int)blockIdx.x < ctas) {
+            const int most = most_moved<HD>(units, ctas);
+            const long long begin = first_unit(blockIdx.x, units, ctas);
+            // the thread that has a cut's sequence finds the sequence, its first unit, and where the cut goes
+            for (int e = 0; e < 2; e++) {
+                const long long cut = e ? first_unit(blockIdx.x + 1, units, ctas) : begin;
+                if (cut < first || cut >= first + mine) continue;
+                long long from = first;
+                for (int b = lo; b < hi; b++) {
+                    const SeqSpan sp = seq_span(a.b, b);
+                    const long long n = seq_units(sp, a.hkv);
+                    if (from + n > cut) {
+                        const int per_head = (sp.len + kUnit - 1) / kUnit, h = (int)quotient(cut - from, per_head);
+                        const long long s0 = from + (long long)h * per_head, s1 = s0 + per_head;
+                        const long long at = moved(cut, s0, s1, most);
+                        cuts[e] = {b, from, at};
+                        if (e == 1 && at > s0 && at < s1 && begin - s0 <= most) {
+                            // the stream begins here and goes on, to the CTA of its last unit, or where that one's first
+                            // cut moves to the stream's end the one before
+                            int last = cta_of(s1 - 1, units, ctas);
+                            if (last > (int)blockIdx.x + 1 && s1 - first_unit(last, units, ctas) <= most) last--;
+                            const int stream = b * a.hkv + h;
+                            fa.cut[fa.by_cta ? (int)blockIdx.x : stream] =
+                                make_int4(stream, blockIdx.x, last - (int)blockIdx.x + 1, 0);
+                        }
+                        break;
+                    }
+                    from += n;
+                }
+            }
         }
-        b0 = l * per;
-        base = chunk[l];
+        if (bad) {  // each CTA its share of the sequences
+            if (blockIdx.x == 0 && tid == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+            for (int b = blockIdx.x; b < a.b.n_seqs; b += gridDim.x)
+                if (!seq_span(a.b, b).ok)
+                    for (int h = 0; h < a.hkv; h++) nan_rows<T, HD>(a, b, h, tid, kThreads);
+        }
+        __syncthreads();
+        if ((int)blockIdx.x >= ctas) return;
+        b0 = cuts[0].b, base = cuts[0].from, c0 = cuts[0].at;
+        c1 = (int)blockIdx.x + 1 < ctas ? cuts[1].at : units;
     }
 
     if (warp == kWarps) {
         // ---------------- producer: lanes 0-7 the K groups, 8-15 the V groups ----------------
         int t = 0;
         const uint8_t* pool = static_cast<const uint8_t*>(lane & 8 ? a.v_pool : a.k_pool);
-        for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int) {
+        for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
+            if (!kWhole && lane == 0 && !fa.by_cta && u0 == 0 && u1 == stream_units)
+                fa.cut[b * a.hkv + h] = make_int4(0, 0, 1, 0);  // not cut
             const int r1 = min(u1 * kUnit, sp.len);
             const int* table = a.b.page_table + (size_t)b * a.b.page_cols;
             for (int row0 = u0 * kUnit; row0 < r1; row0 += F::T, t++) {
@@ -392,7 +443,7 @@ __global__ void __launch_bounds__(Few<HD, MT>::kThreads, Few<HD, MT>::kCtas) pag
         for (int w = 1; w < kKeyWarps; w++) M = fmaxf(M, ml[jw + w * 16].x);
 #pragma unroll
         for (int w = 0; w < kKeyWarps; w++) Ls += ml[jw + w * 16].y * ex2(ml[jw + w * 16].x - M);
-        const bool whole = u0 == 0 && u1 == stream_units;
+        const bool whole = kWhole || (u0 == 0 && u1 == stream_units);
         const size_t slot = 2 * (size_t)blockIdx.x + (u0 == 0 ? 1 : 0);
         const int ji = jr / a.g;
         const size_t orow = ((size_t)(sp.t0 + ji) * a.hq + (size_t)(h * a.g + jr - ji * a.g)) * HD;
@@ -426,14 +477,14 @@ __global__ void __launch_bounds__(Few<HD, MT>::kThreads, Few<HD, MT>::kCtas) pag
 }
 
 // out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the parts of one
-// query row of a stream cut across CTAs; block (row, stream), thread (part
+// query row of a stream cut across CTAs; block (row, stream or the
+// CTA where it begins), thread (part
 // group, four columns).  All loads of a row's first parts are in flight at
-// once: the merge is one round trip to L2.  Rows of a sequence outside the
-// host's bounds become NaN here.
+// once: the merge is one round trip to L2.
 constexpr int kMergeThreads = 128;
 
 template <class T, int HD>
-__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs fa, int grid, int rows) {
+__global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs fa, int rows) {
     constexpr int C4 = HD / 4, NG = kMergeThreads / C4, RPT = 40 / NG;
     __shared__ float w_s[kMaxParts], red[kMergeThreads / 32][2];
     __shared__ float4 acc_s[kMergeThreads];
@@ -441,19 +492,15 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     pdl_wait();
     const PagedAttnArgs& a = fa.a;
     const int tid = threadIdx.x, c4 = tid % C4, grp = tid / C4;
-    const int b = (int)(blockIdx.y / a.hkv), h = (int)(blockIdx.y % a.hkv), r = blockIdx.x;
+    const int r = blockIdx.x;
+    const int4 cut = __ldcg(fa.cut + blockIdx.y);
+    if (fa.by_cta && cut.x < 0) return;
+    const int stream = fa.by_cta ? cut.x : (int)blockIdx.y;
+    const int b = stream / a.hkv, h = stream - b * a.hkv;
     const SeqSpan sp = seq_span(a.b, b);
-    if (!sp.ok) {
-        nan_rows<T, HD>(a, b, h, r, gridDim.x, tid, kMergeThreads);
-        return;
-    }
-    if (r >= sp.n * a.g) return;
-    const long long units = fa.prefix[a.b.n_seqs];
-    const int per_head = (sp.len + kUnit - 1) / kUnit, ctas = ctas_used(units, grid);
-    const long long s0 = fa.prefix[b] + (long long)h * per_head;
-    const int lo = cta_of(s0, units, ctas), hi = cta_of(s0 + per_head - 1, units, ctas);
-    if (lo == hi) return;  // written by the attention kernel
-    const int parts = hi - lo + 1;
+    if (!sp.ok || r >= sp.n * a.g) return;  // a stream without keys has no entry
+    const int lo = cut.y, parts = cut.z;
+    if (parts == 1) return;  // written by the attention kernel
     auto slot = [&](int p) -> size_t {  // the first part begins its stream, the others are their CTA's first
         const bool begins = p == 0;
         return ((size_t)(lo + p) * 2 + (begins ? 1 : 0)) * rows + r;
@@ -515,35 +562,50 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     }
 }
 
+// Short sequences: a stream per CTA, nothing merged.  An SM takes in 65 KB a
+// microsecond, the merge kernel and a stream's second part cost 3 to 4: up to
+// 256 KB a stream (bf16, 4 x 64: 300 rows 6.1 us against 8.8, 800 rows 9.0 both,
+// 1,500 rows 13.3 against 9.0), and up to 512 KB where the streams are many
+// enough to keep the memory busy (64 of 700 rows of 8 x 128, 4 rows each: 32 us
+// against 40; at 1,000 rows 128 streams 19.3 against 22.6, 400 streams 43 both).
+// More would gain where all lengths are alike, but the longest decides here.
+bool whole_streams(const PagedAttnArgs& a) {
+    const long long bytes = (long long)a.b.max_len * a.hd * 4;
+    return bytes <= (256 << 10) ||
+           (bytes <= (512 << 10) && (long long)a.b.n_seqs * a.hkv * 3 >= 2 * device_sm_count());
+}
+
 template <class T, int HD, int MT>
 cudaError_t launch_rows(const PagedAttnArgs& a, cudaStream_t stream) {
     using F = Few<HD, MT>;
     static PerDeviceOnce setup;
     cudaError_t e = setup.run([] {
-        return cudaFuncSetAttribute(paged_few_kernel<T, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::bytes);
+        const cudaError_t w = cudaFuncSetAttribute(paged_few_kernel<T, HD, MT, true>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, F::bytes);
+        return w != cudaSuccess ? w
+                                : cudaFuncSetAttribute(paged_few_kernel<T, HD, MT, false>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, F::bytes);
     });
     if (e != cudaSuccess) return e;
     FewArgs fa{};
     fa.a = a;
-    // Short sequences: a stream per CTA.  An SM takes in 65 KB a microsecond, so up
-    // to kWholeBytes a stream takes less time than cutting it saves, as the merge
-    // kernel is then not launched at all (one token over 512 rows of 4 KV heads of
-    // 64: 8.0 us cut, 6.2 whole).
-    fa.whole = (long long)a.b.max_len * HD * 4 <= kWholeBytes;
-    auto kernel = paged_few_kernel<T, HD, MT>;
-    if (fa.whole)
-        return launch_pdl(kernel, dim3(a.b.n_seqs * a.hkv), dim3(F::kThreads), (size_t)F::bytes, stream, fa);
+    if (whole_streams(a))
+        return launch_pdl(paged_few_kernel<T, HD, MT, true>, dim3(a.b.n_seqs * a.hkv), dim3(F::kThreads),
+                          (size_t)F::bytes, stream, fa);
     const long long units = (long long)a.b.n_seqs * a.hkv * ((a.b.max_len + kUnit - 1) / kUnit);
     const int grid = (int)std::min<long long>(std::min(F::kCtas * device_sm_count(), F::kMaxCtas),
                                               (units + kMinUnits - 1) / kMinUnits);
     static_assert(2 * F::kMaxCtas * F::kRows <= kSlots, "workspace");
     fa.part_ml = reinterpret_cast<float2*>(a.ws);
     fa.part_o = reinterpret_cast<float*>(a.ws + (size_t)kSlots * 8);
-    fa.prefix = reinterpret_cast<long long*>(a.ws + (size_t)kSlots * (8 + 4 * HD));
-    e = launch_pdl(kernel, dim3(grid), dim3(F::kThreads), (size_t)F::bytes, stream, fa);
+    fa.cut = reinterpret_cast<int4*>(a.ws + (size_t)kSlots * (8 + 4 * HD));
+    // at most one stream begins in a CTA and goes on in the next: with many streams (512 of 16 rows: 8,192 blocks,
+    // most of them with nothing to do) the merge goes by those
+    fa.by_cta = (long long)a.b.n_seqs * a.hkv > grid;
+    e = launch_pdl(paged_few_kernel<T, HD, MT, false>, dim3(grid), dim3(F::kThreads), (size_t)F::bytes, stream, fa);
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_few_merge_kernel<T, HD>, dim3(a.b.max_new * a.g, a.b.n_seqs * a.hkv), dim3(kMergeThreads), 0,
-                      stream, fa, grid, F::kRows);
+    return launch_pdl(paged_few_merge_kernel<T, HD>, dim3(a.b.max_new * a.g, fa.by_cta ? grid : a.b.n_seqs * a.hkv),
+                      dim3(kMergeThreads), 0, stream, fa, F::kRows);
 }
 
 template <class T, int HD>
@@ -563,12 +625,12 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
 // whole: 18 against 13 us for one sequence of 300, 53 against 30 for 9 of 3,500.
 bool paged_few_fits(const PagedAttnArgs& a) {
     const long long rows = (long long)a.b.max_new * a.g, streams = (long long)a.b.n_seqs * a.hkv;
-    if (streams > 65535) return false;
+    if (streams > INT_MAX) return false;
     return rows <= 16 || (rows <= kMostRows && streams * a.b.max_len * a.hd * 4 <= kTwoGroupBytes);
 }
 
-size_t paged_few_bytes(int hd, int n_seqs) {
-    return align_up((size_t)kSlots * (8 + 4 * hd) + (size_t)(n_seqs + 1) * 8, 256);
+size_t paged_few_bytes(int hd) {
+    return align_up((size_t)kSlots * (8 + 4 * hd) + (size_t)kMaxParts * 16, 256);
 }
 
 cudaError_t launch_paged_few(const PagedAttnArgs& a, cudaStream_t stream) {

@@ -504,6 +504,63 @@ def test_random_batches_one_after_the_other(rt, seed):
                                    f"tolerance, first at {bad.nonzero()[0].tolist()}")
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches_of_few_rows(rt, seed):
+    """Tokens and short drafts, one sequence to hundreds, short and long: streams inside a CTA, cut over several, cut near
+    their ends, more streams than CTAs; twice in turn with a batch of one sequence."""
+    import random
+    rng = random.Random(100 + seed)
+    two = []
+    for one in (False, True):
+        hq, hkv, hd = rng.choice([(32, 4, 64), (14, 2, 64), (28, 4, 128), (32, 8, 128), (40, 8, 128), (6, 3, 64), (16, 1, 128)])
+        most = rng.choice([1, 16 // (hq // hkv), 32 // (hq // hkv)])
+        n = 1 if one else rng.choice([2, 5, 17, 33, 60, 150])
+        longest = rng.choice([20, 300, 700, 1500] + ([6000, 16000] if one else [3000] if n < 40 else []))
+        new = [rng.randrange(0 if n > 4 else 1, most + 1) for _ in range(n)]
+        new[0] = most
+        past = [rng.choice([longest, rng.randrange(longest), rng.randrange(16)]) for _ in new]
+        B = Batch(rt, new, past, hq, hkv, hd, rng.choice([16, 32, 64, 128, 256]), rng.choice(["f16", "bf16"]), layers=1,
+                  pad=rng.randrange(3), seed=seed)
+        B.fill(0)
+        B.q = B.rand(B.n_tok, hq, hd).to(B.dt)
+        B.outs = [torch.full((B.n_tok, hq, hd), float("nan"), device="cuda", dtype=B.dt) for _ in range(2)]
+        two.append(B)
+    torch.cuda.synchronize()
+    for r in range(2):
+        for B in two:
+            B.cache.attend(0, B.batch, B.q, B.outs[r])
+    for B in two:
+        assert B.batch.status() == 0
+        want, err = gpu_attn(B, 0, B.q)
+        tol = err + HALF[B.dt] * (want.abs() + err) + TINY[B.dt]
+        for r, y in enumerate(B.outs):
+            d = (y.double() - want).abs()[:B.start[-1]]
+            bad = ~(d <= tol[:B.start[-1]])
+            assert not bad.any(), (f"run {r}: {int(bad.sum())} off, worst {float((d / tol[:B.start[-1]]).max()):.3g} of the "
+                                   f"tolerance, first at {bad.nonzero()[0].tolist()}")
+
+
+@pytest.mark.parametrize("n,past", [(3, 5000), (200, 900), (200, 100)])
+def test_bad_lengths_among_few_rows(rt, n, past):
+    """Sequences outside the host's bounds beside good ones: NaN in their rows, the others' rows as ever, in each way that a
+    batch of single tokens is split."""
+    from picolm_qwen_b200 import abi
+    B = Batch(rt, [1] * n, [past] * n, 4, 2, 128, 64, "f16")
+    B.fill(0)
+    q = B.rand(B.n_tok, 4, 128).half()
+    want, err = gpu_attn(B, 0, q)
+    off = [1, n - 1]
+    B.kv_len[off[0]] = 0
+    B.kv_len[off[1]] = past + 1000000
+    y = torch.zeros((B.n_tok, 4, 128), device="cuda").half()
+    B.cache.attend(0, B.batch, q, y)
+    assert B.batch.status() == abi.DEV_BAD_POS
+    keep = [i for i in range(n) if i not in off]
+    assert y[off].isnan().all()
+    tol = err + HALF[B.dt] * (want.abs() + err) + TINY[B.dt]
+    assert ((y.double() - want).abs() <= tol)[keep].all()
+
+
 def test_many_sequences(rt):
     """More sequences than a block has threads, some of them empty."""
     n = 1500
