@@ -730,8 +730,14 @@ int32_t picoattn_paged_append(const picoattn_config_t* cfg, const picoattn_paged
  * Scores, sums and outputs accumulate in fp32; the weights exp(s - max) are
  * rounded to the cache's type for the product with V.  A page table entry
  * outside [0, n_pages) sets PICOATTN_DEV_BAD_PAGE and the outputs that would
- * have read it are NaN (others of that sequence may be).  Rows past a sequence's length are never used, whatever
- * they hold.
+ * have read it are NaN (others of that sequence may be).  Rows past a
+ * sequence's length are never used, whatever they hold.  A NaN or an infinity in
+ * a V row of the call's own new tokens may reach earlier new tokens of that
+ * sequence, from which causality hides the row: their weight 0 times it is NaN.
+ * Batches whose work does not fit 32-bit counts (with T = 2*floor(128 / q heads
+ * per KV head): max_new/T * max_len/32 or (n_tok/T + n_seqs) * n_kv_heads) are
+ * PICOATTN_EUNSUPPORTED.
+ * After PICOATTN_DEV_TIMEOUT the outputs of the call are not defined.
  */
 int32_t picoattn_paged_attn(const picoattn_config_t* cfg, const picoattn_paged_cache_t* cache, int32_t layer,
                             const picoattn_paged_batch_t* batch, const void* q, int64_t q_stride,

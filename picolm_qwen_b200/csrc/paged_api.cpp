@@ -228,6 +228,12 @@ int32_t picoattn_paged_attn(const picoattn_config_t* cfg, const picoattn_paged_c
     if (out_dtype != PICOATTN_DTYPE_F32 && out_dtype != cache->dtype) return PICOATTN_EUNSUPPORTED;
     const int64_t qw = (int64_t)cfg->n_heads * cfg->head_dim;
     if (q_stride < qw || q_stride > kMaxStride || q_stride % 8) return PICOATTN_EINVAL;
+    // the chunk kernel's work list counts a head's blocks, their costs and the batch's blocks in 32 bits
+    const int64_t per = 2 * (128 / (cfg->n_heads / cfg->n_kv_heads));
+    const int64_t blocks = (batch->max_new + per - 1) / per, tiles = (batch->max_len + 127) / 128;
+    if (blocks * (4 * tiles + 4) > INT32_MAX ||
+        (batch->n_tok / per + (int64_t)batch->n_seqs) * cfg->n_kv_heads > INT32_MAX)
+        return PICOATTN_EUNSUPPORTED;
     if (overlap(extent(out, batch->n_tok, qw, qw, elem_size(out_dtype)), extent(q, batch->n_tok, q_stride, qw, 2)))
         return PICOATTN_EINVAL;
     st = picoattn_device_check();

@@ -19,7 +19,6 @@
 // batch's time over its bytes: the plan and first loads (2 us), a CTA's second part
 // (1.7 us), the merge kernel and the tail of the slices (3 to 4 us).
 #include <algorithm>
-#include <climits>
 #include <cmath>
 
 #include "paged_common.cuh"
@@ -625,8 +624,7 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
 // whole: 18 against 13 us for one sequence of 300, 53 against 30 for 9 of 3,500.
 bool paged_few_fits(const PagedAttnArgs& a) {
     const long long rows = (long long)a.b.max_new * a.g, streams = (long long)a.b.n_seqs * a.hkv;
-    if (streams > INT_MAX) return false;
-    return rows <= 16 || (rows <= kMostRows && streams * a.b.max_len * a.hd * 4 <= kTwoGroupBytes);
+    return rows <= 16 || (rows <= kMostRows && streams <= kTwoGroupBytes / ((long long)a.b.max_len * a.hd * 4));
 }
 
 size_t paged_few_bytes(int hd) {

@@ -151,6 +151,20 @@ def test_attn_refuses(kw, want):
     assert attn(**kw) == want
 
 
+@pytest.mark.parametrize("kw,want", [
+    # a head's blocks x key tiles past 32 bits: 2 tokens a block at 128 q heads per KV head, 36 at 7
+    (dict(c=cfg(n_heads=128, n_kv_heads=1, max_seq_len=1 << 20), b=batch(n_tok=1 << 20, max_new=1 << 20, max_len=1 << 20,
+                                                                        page_cols=1 << 16), qs=128 * 128), UNS),
+    (dict(c=cfg(n_heads=128, n_kv_heads=1, max_seq_len=1 << 20), b=batch(n_tok=1 << 20, max_new=1 << 16, max_len=1 << 20,
+                                                                        page_cols=1 << 16), qs=128 * 128,
+          out=ADDR["q"] + (1 << 40)), None),
+    (dict(b=batch(n_seqs=(1 << 29) + 1)), UNS),  # sequences x KV heads past 32 bits
+])
+def test_attn_refuses_what_its_work_list_cannot_count(kw, want):
+    st = attn(**kw)
+    assert st in ACCEPTED if want is None else st == want
+
+
 def test_packed_arguments_have_the_structs_layout():
     """abi.ROPE_ARGS / PAGED_APPEND_ARGS pack what the C structs (and their ctypes forms) hold."""
     r = abi.RopeArgs(1, 0, 64, 32, 1, 7, 99, 2, 11, 12, 13, abi.RopeRows(21, 22, 23, 24, 25),
