@@ -45,8 +45,10 @@ constexpr int kThreads = 384;
 constexpr int kPlan = 32;          // runs of sequences whose costs are added up, a lane each
 constexpr int kMaxCtas = 160;
 constexpr int kItemCost = 4;       // of a block, whatever its tiles
-constexpr int kMinCost = 16;       // least cost per CTA of a slice
+constexpr int kMinCost = 8;        // least cost per CTA of a slice
 constexpr int kSliceOverhead = 32; // what cutting blocks costs, in the same unit (measured, see launch)
+constexpr int kCutOverhead = 32;
+constexpr int kMostMoved = 16;
 constexpr int kPartRows = 2 * BM;
 constexpr int kRing = 4;           // stages of 64 keys, K and V each
 constexpr float kNone = -1e30f;    // running maximum before any key
@@ -60,6 +62,7 @@ struct ChunkMeta {  // the cut block whose first part a CTA holds (nt 0: none)
 struct ChunkArgs {
     PagedAttnArgs a;
     int tq;              // tokens per tile
+    int single;          // whole blocks, at most one per CTA: no counter, nothing to merge
     int* counter;        // next whole block; zero between calls
     ChunkMeta* meta;     // [grid]
     float2* part_ml;     // [2 * grid][256]
@@ -151,18 +154,22 @@ __device__ __forceinline__ int make_plan(const ChunkArgs& c, Plan* plan, int per
 #pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
         all += __shfl_xor_sync(0xffffffffu, all, o);
-        const int io = __shfl_up_sync(0xffffffffu, items, o);
-        if (lane >= o) items += io;
     }
-    if (lane == 0) plan->first_item[0] = 0;
-    plan->first_item[lane + 1] = items;
-    most = __reduce_max_sync(0xffffffffu, most);
-    items = __shfl_sync(0xffffffffu, items, 31);
+    const int longest = __reduce_max_sync(0xffffffffu, most), blocks = __reduce_add_sync(0xffffffffu, items);
     // whole blocks end when the longest does, or, dealt out one by one, some 15% after the mean
     const float n = fminf((float)grid, all * (1.0f / kMinCost)), mean = all / fmaxf(n, 1.0f);
-    const float whole = fmaxf((float)most, items <= grid ? 0.f : 1.15f * mean);
-    __syncwarp();
-    if (mean + kSliceOverhead >= whole) return 0;
+    const float whole = fmaxf((float)longest, blocks <= grid ? 0.f : 1.15f * mean);
+    if (c.single || mean + (blocks <= n ? kCutOverhead : kSliceOverhead) >= whole) {
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const int io = __shfl_up_sync(0xffffffffu, items, o);
+            if (lane >= o) items += io;
+        }
+        if (lane == 0) plan->first_item[0] = 0;
+        plan->first_item[lane + 1] = items;
+        __syncwarp();
+        return 0;
+    }
 #pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
         const long long co = __shfl_up_sync(0xffffffffu, cost, o);
@@ -172,17 +179,25 @@ __device__ __forceinline__ int make_plan(const ChunkArgs& c, Plan* plan, int per
     plan->first_cost[lane + 1] = cost;
     cost = __shfl_sync(0xffffffffu, cost, 31);
     __syncwarp();
-    return (int)min((long long)grid, (cost + kMinCost - 1) / kMinCost);
+    const int slices = (int)min((long long)grid, (cost + kMinCost - 1) / kMinCost);
+    const int over = slices % blocks;
+    return over * 8 <= slices && over < slices ? slices - over : slices;  // blocks alike are cut alike, at their ends
 }
 
 __device__ __forceinline__ long long slice_first(long long i, long long cost, int n) {
     return quotient(i * cost, n);
 }
 
+// A cut this near to a block's ends moves there: less than half a slice, so that no two cuts meet.
+__device__ __forceinline__ int most_moved(long long cost, int n) { return (int)min((long long)kMostMoved, quotient(cost, n) / 2); }
 // A part's first (or end) tile for a slice that begins (ends) at cost unit x of a block from `start`.
-__device__ __forceinline__ int tile_at(long long x, long long start, int unit, int nt) {
+__device__ __forceinline__ int tile_at(long long x, long long start, int unit, int nt, int most) {
     start += kItemCost;
-    return x <= start ? 0 : (int)min((long long)nt, quotient(x - start + unit - 1, unit));
+    const long long end = start + (long long)nt * unit;
+    if (x >= end) return nt;  // a block may be shorter than `most`
+    if (x <= start + most) return 0;
+    if (x >= end - most) return nt;
+    return (int)quotient(x - start + unit - 1, unit);
 }
 
 // Where a CTA is in its work (the producer warp, the same in every lane).
@@ -193,6 +208,7 @@ struct Walk {
     Blocks x;
     bool open;                // b .. start are set
     int taken;                // whole blocks so far
+    int most;                 // most_moved
 };
 
 // The slice's first cost unit -> its sequence, head and block.
@@ -236,6 +252,7 @@ __device__ __forceinline__ bool next_item(const ChunkArgs& c, const Plan* plan, 
     if (!slices) {  // whole blocks: the CTA's own first one, then by the counter
         int idx = blockIdx.x;
         if (wk.taken++) {
+            if (c.single) return false;
             if (lane == 0) idx = (int)gridDim.x + atomicAdd(c.counter, 1);
             idx = __shfl_sync(0xffffffffu, idx, 0);
         }
@@ -256,7 +273,7 @@ __device__ __forceinline__ bool next_item(const ChunkArgs& c, const Plan* plan, 
     while (wk.at < wk.end) {
         if (!wk.open) walk_find(c, wk, lane);
         const int nt = wk.x.tiles(wk.blk), u = wk.x.unit(wk.blk);
-        const int j0 = tile_at(wk.at, wk.start, u, nt), j1 = tile_at(wk.end, wk.start, u, nt);
+        const int j0 = tile_at(wk.at, wk.start, u, nt, wk.most), j1 = tile_at(wk.end, wk.start, u, nt, wk.most);
         if (j0 < j1) {
             it.b = wk.b, it.h = wk.h;
             it.tok0 = wk.x.t0 + wk.blk * wk.x.per, it.ntok = wk.x.ntok(wk.blk);
@@ -551,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const long long cost = plan->first_cost[kPlan];
             wk.at = slice_first(blockIdx.x, cost, slices);
             wk.end = slice_first(blockIdx.x + 1, cost, slices);
+            wk.most = most_moved(cost, slices);
             const int run = __popc(__ballot_sync(0xffffffffu, plan->first_cost[lane + 1] <= wk.at));
             wk.b = run * per;
             wk.base = plan->first_cost[run];
@@ -909,12 +927,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the parts of the blocks that slices cut: block (CTA that holds a cut
 // block's first part, row group), thread (row, four columns).  Also sets the
 // work counter back.
-constexpr int kMergeBlocks = 8;  // per cut block
+constexpr int kMergeRows = 32, kMergeBlocks = kPartRows / kMergeRows, kMergeThreads = 256;
 
 template <class T, int HD>
-__global__ void __launch_bounds__(256) paged_chunk_merge_kernel(ChunkArgs c) {
-    constexpr int C4 = HD / 4, RB = 256 / C4;
-    static_assert(kMaxCtas <= 256, "a thread per part");
+__global__ void __launch_bounds__(kMergeThreads) paged_chunk_merge_kernel(ChunkArgs c) {
+    constexpr int C4 = HD / 4, RB = kMergeThreads / C4;
+    static_assert(kMaxCtas <= kMergeThreads, "a thread per part");
+    __shared__ float2 ml_s[kMaxCtas * kMergeRows];
+    __shared__ float inv_s[kMergeRows];
     pdl_trigger();
     pdl_wait();
     const PagedAttnArgs& a = c.a;
@@ -925,35 +945,62 @@ __global__ void __launch_bounds__(256) paged_chunk_merge_kernel(ChunkArgs c) {
     const int unit = x.unit(mt.blk);
     // the parts are those of this CTA and the ones after it, as the attention kernel cut them
     const int i = blockIdx.x + threadIdx.x;
-    const bool has = i < mt.slices && tile_at(slice_first(i, mt.cost, mt.slices), mt.start, unit, mt.nt) <
-                                          tile_at(slice_first(i + 1, mt.cost, mt.slices), mt.start, unit, mt.nt);
+    const int most = most_moved(mt.cost, mt.slices);
+    const bool has = i < mt.slices && tile_at(slice_first(i, mt.cost, mt.slices), mt.start, unit, mt.nt, most) <
+                                          tile_at(slice_first(i + 1, mt.cost, mt.slices), mt.start, unit, mt.nt, most);
     const int parts = __syncthreads_count(has);
     auto slot = [&](int p) { return (size_t)(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * kPartRows; };
-    const int c4 = threadIdx.x % C4, ntok = x.ntok(mt.blk);
-    for (int row = blockIdx.y * RB + threadIdx.x / C4; row < kPartRows; row += kMergeBlocks * RB) {
+    // (max, sum) of the parts of this block's rows -> their weights
+    const int row0 = blockIdx.y * kMergeRows, ntok = x.ntok(mt.blk);
+    const int last = (ntok > c.tq ? BM : 0) + ((ntok > c.tq ? ntok - c.tq : ntok) * a.g) - 1;  // valid row
+    if (row0 > last) return;
+    for (int i = threadIdx.x; i < parts * kMergeRows; i += kMergeThreads)
+        ml_s[i] = __ldcg(c.part_ml + slot(i / kMergeRows) + row0 + i % kMergeRows);
+    __syncthreads();
+    {
+        constexpr int kSub = kMergeThreads / kMergeRows;  // threads of a row, side by side
+        const int row = threadIdx.x / kSub, sub = threadIdx.x % kSub;
+        float M = -INFINITY, L = 0.f;
+        for (int p = sub; p < parts; p += kSub) M = fmaxf(M, ml_s[p * kMergeRows + row].x);
+        for (int o = 1; o < kSub; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        for (int p = sub; p < parts; p += kSub) {
+            float2& v = ml_s[p * kMergeRows + row];
+            v.x = ex2(v.x - M);
+            L += v.y * v.x;
+        }
+        for (int o = 1; o < kSub; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (sub == 0) inv_s[row] = 1.0f / L;
+    }
+    __syncthreads();
+    constexpr int NR = kMergeRows / RB;
+    const int c4 = threadIdx.x % C4, r0 = threadIdx.x / C4;
+    float4 acc[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < parts; p++) {
+        const float4* o = reinterpret_cast<const float4*>(c.part_o + (slot(p) + row0) * HD) + c4;
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const int r = r0 + i * RB;
+            const float4 v = __ldcg(o + (size_t)r * C4);
+            const float w = ml_s[p * kMergeRows + r].x;
+            acc[i].x += v.x * w, acc[i].y += v.y * w, acc[i].z += v.z * w, acc[i].w += v.w * w;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int row = row0 + r0 + i * RB;
         const int rt = (row % BM) / a.g, rh = row % BM - rt * a.g, tok = row / BM * c.tq + rt;
         if (rt >= c.tq || tok >= ntok) continue;
-        float M = -INFINITY;
-#pragma unroll 4
-        for (int p = 0; p < parts; p++) M = fmaxf(M, __ldcg(c.part_ml + slot(p) + row).x);
-        float L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int p = 0; p < parts; p++) {
-            const float2 ml = __ldcg(c.part_ml + slot(p) + row);
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(c.part_o + (slot(p) + row) * HD) + c4);
-            const float w = ex2(ml.x - M);
-            L += ml.y * w;
-            acc.x += o.x * w, acc.y += o.y * w, acc.z += o.z * w, acc.w += o.w * w;
-        }
-        const float inv = 1.0f / L;
+        const float inv = inv_s[r0 + i * RB];
         const size_t at = ((size_t)(x.t0 + mt.blk * x.per + tok) * a.hq + mt.h * a.g + rh) * HD + 4 * c4;
-        acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
+        acc[i].x *= inv, acc[i].y *= inv, acc[i].z *= inv, acc[i].w *= inv;
         if (a.out_dtype == PICOATTN_DTYPE_F32)
-            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = acc;
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = acc[i];
         else
             *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
-                make_uint2(Elem<T>::pack2(acc.x, acc.y), Elem<T>::pack2(acc.z, acc.w));
+                make_uint2(Elem<T>::pack2(acc[i].x, acc[i].y), Elem<T>::pack2(acc[i].z, acc[i].w));
     }
 }
 
@@ -1021,10 +1068,13 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
         return cudaErrorInvalidValue;
     const long long blocks = (long long)a.b.n_seqs * a.hkv * ((a.b.max_new + 2 * c.tq - 1) / (2 * c.tq));
     const long long tiles = (a.b.max_len + BN - 1) / BN;  // a slice has at least kMinCost units, a whole block a CTA
-    const int grid = (int)std::min<long long>(std::min(device_sm_count(), kMaxCtas), blocks * tiles);
+    const int ctas = std::min(device_sm_count(), kMaxCtas);
+    // make_plan hands out whole blocks then, whatever the lengths
+    c.single = blocks <= ctas && tiles * 4 + kItemCost <= kCutOverhead;
+    const int grid = (int)std::min<long long>(ctas, c.single ? blocks : blocks * tiles);
     e = launch_pdl(paged_chunk_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)L::kDyn, stream, mq, mk, mv, mo, mp, c);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(paged_chunk_merge_kernel<T, HD>, dim3(grid, kMergeBlocks), dim3(256), 0, stream, c);
+    if (e != cudaSuccess || c.single) return e;
+    return launch_pdl(paged_chunk_merge_kernel<T, HD>, dim3(grid, kMergeBlocks), dim3(kMergeThreads), 0, stream, c);
 }
 
 }  // namespace
