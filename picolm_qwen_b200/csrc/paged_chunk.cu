@@ -18,14 +18,24 @@
 // blocks (few new tokens): the groups take alternate key tiles of the same rows
 // and their (max, sum, O) are joined at the end.
 //
-// Compute-bound for two-tile blocks (per key tile and SM 2,048 cycles of tensor
-// work and as many of exponentials), HBM-bound for one-tile blocks.
+// Compute-bound for two-tile blocks (at hd 128 2,560 cycles of tensor work per key
+// tile and SM, 2,048 of exponentials), HBM-bound for one-tile blocks.
 //
-// Work split: the blocks' costs (key tiles, twice for two-tile blocks) are known
-// to every CTA from the lengths.  Either whole blocks are handed out, longest
-// of each sequence first, by a counter; or, where blocks are too few or too
-// uneven, all their tiles are concatenated and cut into equal slices, the parts
-// of a cut block going to the workspace for a merge kernel.
+// Work split: the blocks' costs are known to every CTA from the lengths.  Either
+// whole blocks are handed out, longest of each sequence first, by a counter; or,
+// where blocks are too few or too uneven, all their tiles are concatenated and cut
+// into equal slices, the parts of a cut block going to the workspace for a merge
+// kernel.
+//
+// Measured, hd 128: two chunks of 1,024 tokens over 19,000 rows of 8 KV heads,
+// bf16, 32 q heads 710 to 750 us (650 GFLOP: 0.52 to 0.56 of the burst rate, 0.62
+// to 0.67 of the rate cuBLAS holds under the same power cap); a prompt of 2,048
+// 49 us (0.42); 24 single tokens and chunks of 291, 337 and 413 tokens over up to
+// 4,000 rows of 4 KV heads 76 us.  A two-tile key tile takes 3,400 to 3,900 cycles:
+// the softmax of a half (its exponentials alone 512 on the SM's four units, with the
+// rest of its instructions some 800) and the round trip of its products (issue,
+// commit, wait: 550) follow one another within a group, and two groups cover
+// each other only in part.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -44,11 +54,16 @@ constexpr int BM = 128, BN = 128, BH = BN / 2;
 constexpr int kThreads = 384;
 constexpr int kPlan = 32;          // runs of sequences whose costs are added up, a lane each
 constexpr int kMaxCtas = 160;
+// Costs, in units of a quarter of a two-tile block's key tile (some 900 cycles):
 constexpr int kItemCost = 4;       // of a block, whatever its tiles
-constexpr int kMinCost = 8;        // least cost per CTA of a slice
-constexpr int kSliceOverhead = 32; // what cutting blocks costs, in the same unit (measured, see launch)
-constexpr int kCutOverhead = 32;
-constexpr int kMostMoved = 16;
+constexpr int kMinCost = 8;        // least per CTA of a slice (40 new over 3,000 rows of 4 x 128: 26 us; 16: 31, 4: 29)
+// What cutting blocks costs: their epilogues, the parts written and read again, the merge.  With 16 a prompt of
+// 2,048 (longest block 68, mean 66) stays at 49 us, but one of 600 over 100 goes from 19 to 21 and 24 tokens beside
+// three chunks from 76 to 92; with 8 the prompt takes 75.
+constexpr int kSliceOverhead = 32;
+// A cut this near to a block's end moves there (200 new over 3,000 rows of 4 x 128: 38 us without, 28; two such and
+// two single tokens of 4 x 64: 36, with 16 37).
+constexpr int kMostMoved = 8;
 constexpr int kPartRows = 2 * BM;
 constexpr int kRing = 4;           // stages of 64 keys, K and V each
 constexpr float kNone = -1e30f;    // running maximum before any key
@@ -159,7 +174,7 @@ __device__ __forceinline__ int make_plan(const ChunkArgs& c, Plan* plan, int per
     // whole blocks end when the longest does, or, dealt out one by one, some 15% after the mean
     const float n = fminf((float)grid, all * (1.0f / kMinCost)), mean = all / fmaxf(n, 1.0f);
     const float whole = fmaxf((float)longest, blocks <= grid ? 0.f : 1.15f * mean);
-    if (c.single || mean + (blocks <= n ? kCutOverhead : kSliceOverhead) >= whole) {
+    if (c.single || mean + kSliceOverhead >= whole) {
 #pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
             const int io = __shfl_up_sync(0xffffffffu, items, o);
@@ -1070,7 +1085,7 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     const long long tiles = (a.b.max_len + BN - 1) / BN;  // a slice has at least kMinCost units, a whole block a CTA
     const int ctas = std::min(device_sm_count(), kMaxCtas);
     // make_plan hands out whole blocks then, whatever the lengths
-    c.single = blocks <= ctas && tiles * 4 + kItemCost <= kCutOverhead;
+    c.single = blocks <= ctas && tiles * 4 + kItemCost <= kSliceOverhead;
     const int grid = (int)std::min<long long>(ctas, c.single ? blocks : blocks * tiles);
     e = launch_pdl(paged_chunk_kernel<T, HD>, dim3(grid), dim3(kThreads), (size_t)L::kDyn, stream, mq, mk, mv, mo, mp, c);
     if (e != cudaSuccess || c.single) return e;
