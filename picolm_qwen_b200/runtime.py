@@ -220,7 +220,8 @@ class PagedBatch:
     cache's device; their values may change between calls (a captured step reads
     them when it is replayed).  n_tok: rows of q, k, v and out; max_new, max_len:
     bounds on a sequence's new tokens and rows.  Steps that may run at the same
-    time need batches of their own."""
+    time need batches of their own.  The workspace's header is cleared on the
+    current stream; a step on another one waits for that first."""
 
     def __init__(self, cache: "PagedCache", page_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor,
                  n_tok: int, max_new: int, max_len: int):
