@@ -13,7 +13,7 @@ namespace picoattn {
 
 namespace {
 
-constexpr int kAppendWarps = 8;
+constexpr int kAppendWarps = 4;  // 8 (and half the blocks): 3% slower
 
 // The sequence of token row t: the number of q_start[1..] entries <= t, 32 at a
 // time (q_start does not decrease).  n_seqs: none.
@@ -38,14 +38,16 @@ __device__ __forceinline__ void store_pieces(const float (&x)[16], TC* head, con
 
 // A warp step = up to HPS heads of one kind (q, k or v) of one token, hd/16
 // lanes a head; a unit = up to kSteps steps of one kind of one token.  Bound by
-// instruction issue as much as by memory (about 130 instructions per step of
-// 512 elements): the loads of a unit are issued first, its token's sequence,
-// position, page and table entries are found while they travel, and units are
-// numbered kind by kind, so that the warps of an SM run the same code.  Measured:
-// 2,048 tokens of 32/8 heads of 128 with QK-norm in fp16 14.3 us (51 MB: 3.6 TB/s,
-// 0.55 of the copy rate, as the contiguous prefill's prep kernel takes; a ring of
-// cp.async copies of the next units took 20.5, the shared memory it needs being
-// taken from the cache that the lookups live in); 64 tokens 3.3 us.
+// latency and instruction issue (about 130 instructions per step of 512 elements;
+// 80 registers, so 24 warps an SM): the loads of a unit are issued first, its
+// token's sequence, position, page and table entries are found while they travel,
+// and units are numbered kind by kind, so that the warps of an SM run the same
+// code.  Measured: 2,048 tokens of 32/8 heads of 128 with QK-norm in fp16 13.9 us
+// (51 MB: 3.7 TB/s, 0.57 of the copy rate, as the contiguous prefill's prep kernel
+// takes); 64 tokens 3.3 us.  Slower: a ring of cp.async copies of the next units
+// 20.5 us (its shared memory comes out of the cache that the lookups live in), the
+// next unit's loads issued before this one's work 16 (100 registers), 64 registers
+// 17, a step a unit 18.
 constexpr int kSteps = 2;
 
 struct AppendSplit {
@@ -172,7 +174,7 @@ cudaError_t launch_hd(const PagedAppendArgs& a, cudaStream_t stream) {
     const long long units = (long long)a.b.n_tok * (sp.q_per + 2 * sp.kv_per);
     sp.q_units = (unsigned)a.b.n_tok * sp.q_per;
     sp.kv_units = (unsigned)a.b.n_tok * sp.kv_per;
-    const unsigned grid = (unsigned)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, 6LL * device_sm_count());
+    const unsigned grid = (unsigned)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, 12LL * device_sm_count());
     return launch_pdl(paged_append_kernel<TI, TC, HD>, dim3(grid), dim3(kAppendWarps * 32), 0, stream, a, sp);
 }
 

@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
 // write of every element): a unit is up to kSteps steps of one tensor of one
 // token, whose loads are all issued before the first rotation and which share
 // the lane's table entries.  Measured at 8,192 tokens of 32 + 8 heads of 128 in
-// bf16, far positions: 28.7 us = 6.0 TB/s, 0.92 of the copy rate (4 steps: 31 us,
+// bf16, far positions: 28.5 us = 6.0 TB/s, 0.93 of the copy rate (4 steps: 31 us,
 // more registers and so fewer warps); 2,047 tokens of 28 + 4 heads in fp32, half
 // of each rotated, backward: 13.6 us = 5.0 TB/s (2 steps: 13.8).
 template <class T>
