@@ -29,7 +29,7 @@
 //
 // Measured, hd 128: two chunks of 1,024 tokens over 19,000 rows of 8 KV heads,
 // bf16, 32 q heads 710 to 750 us (650 GFLOP: 0.52 to 0.56 of the burst rate, 0.62
-// to 0.67 of the rate cuBLAS holds under the same power cap); a prompt of 2,048
+// to 0.67 of what a plain bf16 product holds under the same power cap); a prompt of 2,048
 // 49 us (0.42); 24 single tokens and chunks of 291, 337 and 413 tokens over up to
 // 4,000 rows of 4 KV heads 76 us.  A two-tile key tile takes 3,400 to 3,900 cycles:
 // the softmax of a half (its exponentials alone 512 on the SM's four units, with the

@@ -46,7 +46,8 @@ struct Few {
     static constexpr int kCtas = MT == 1 ? 2 : 1;         // per SM
     // Two CTAs have three warps on a quarter SM: 144 registers leave room there for a warp of the merge kernel, which
     // then starts while they finish (two sequences of 5,000 rows of 4 x 64: 12.8 us, with 152 registers 14.3).  At hd 128
-    // its 72 registers would fit too, but 144 spill (2 us slower on the same sequences of 8 x 128).
+    // its 72 registers would fit too, but 144 spill (two sequences of
+    // 16,000 rows of 8 x 128: 36.5 us against 34.1).
     static constexpr int kRegs = HD == 64 ? 144 : 168;
     static constexpr int kMaxCtas = MT == 1 ? kMaxParts : kMaxParts / 2;
     static constexpr int kStages = MT == 1 ? 3 : 6;
@@ -616,12 +617,13 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 // Up to 16 rows this kernel reads the cache at the memory's rate.  A second group
-// of 16 rows doubles the products and the softmax per byte: it is then bound by
-// them at 1.2 TB/s (hd 128) to 4 TB/s, but starts sooner than the chunk kernel,
-// so it takes what is short: 24 rows over 2,000 keys of 4 x 64 12.2 us against
-// 18.8, 28 rows over 9 sequences of 3,500 of 4 x 128 26 against 30; over 32 of
-// 4,000 (260 MB) 63 against 55.  Four groups (35 rows and up) were slower on the
-// whole: 18 against 13 us for one sequence of 300, 53 against 30 for 9 of 3,500.
+// of 16 rows doubles the products and the softmax per byte: 4.0 TB/s at hd 64, 4.8
+// to 5.8 at hd 128, where the chunk kernel gets to 4.0 and 6.3.  But this one starts
+// sooner, so it takes what is short: 24 rows over 2,000 keys of 4 x 64 12.2 us
+// against 18.8, 28 rows over 9 sequences of 3,500 of 4 x 128 26 against 30; over 32
+// of 4,000 (260 MB) 63 against 55.  Four groups (35 rows and up) were slower on the
+// whole: 18 against 13 us for one sequence of 300, 53 against 30 for 9 of 3,500 (17
+// warps leave 96 registers each).
 bool paged_few_fits(const PagedAttnArgs& a) {
     const long long rows = (long long)a.b.max_new * a.g, streams = (long long)a.b.n_seqs * a.hkv;
     return rows <= 16 || (rows <= kMostRows && streams <= kTwoGroupBytes / ((long long)a.b.max_len * a.hd * 4));

@@ -83,7 +83,7 @@ struct PagedAttnArgs {
     uint8_t* ws;  // workspace past the header
 };
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t stream);
-// At most 16 query rows per KV head and sequence (paged_few.cu)
+// Few query rows per KV head and sequence (paged_few.cu)
 bool paged_few_fits(const PagedAttnArgs& a);
 size_t paged_few_bytes(int hd);
 cudaError_t launch_paged_few(const PagedAttnArgs& a, cudaStream_t stream);
