@@ -728,7 +728,9 @@ int32_t picoattn_paged_append(const picoattn_config_t* cfg, const picoattn_paged
  *   out_dtype the cache's type or PICOATTN_DTYPE_F32
  *   out       [n_tok][n_heads*head_dim], 16-byte aligned
  * Scores, sums and outputs accumulate in fp32; the weights exp(s - max) are
- * rounded to the cache's type for the product with V.  A page table entry
+ * rounded to the cache's type for the product with V (F16 weights below 2^-32 of
+ * a row's largest may count as zero there).  Scores beyond 2^24 in magnitude,
+ * which fp32 holds in whole steps, may give NaN.  A page table entry
  * outside [0, n_pages) sets PICOATTN_DEV_BAD_PAGE and the outputs that would
  * have read it are NaN (others of that sequence may be).  Rows past a
  * sequence's length are never used, whatever they hold.  A NaN or an infinity in

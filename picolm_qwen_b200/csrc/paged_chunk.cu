@@ -68,6 +68,9 @@ constexpr int kPartRows = 2 * BM;
 constexpr int kRing = 4;           // stages of 64 keys, K and V each
 constexpr float kNone = -1e30f;    // running maximum before any key
 constexpr float kStaleSum = 32768.0f;
+// Of weights (weight_lift): 64 keys at their maximum sum to 2^13, which leaves the maximum room to grow by 2^2 and more
+// (as much again as most of the 64 lie below it) before a half is done again; fp16 weights vanish below 2^-32 of the largest.
+constexpr int kWeightLift = 7;
 
 struct ChunkMeta {  // the cut block whose first part a CTA holds (nt 0: none)
     int b, h, blk, nt, slices;
@@ -344,6 +347,7 @@ template <class T, int HD, class WaitPrevPV>
 __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool first, int lim, bool mask, float scale,
                                              float& m, float& l, WaitPrevPV wait_prev_pv) {
     using P2 = Pair16<T>;
+    constexpr float lift = weight_lift<T>(kWeightLift);
     const uint64_t sc2 = f2_pack(scale, scale);
     uint32_t pk[BH / 2], sr[2][32];
     // p of the keys against m into pk; returns their sum
@@ -376,12 +380,12 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool firs
     tmem_ld32(tS, sr[0]);
     tmem_ld_wait();
     tmem_ld32(tS + 32, sr[1]);
-    if (first) {  // start from the maximum of the first 32 keys
+    if (first) {  // start from the maximum of the first 32 keys, less the lift
         float m0 = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 32; e++)
             if (!mask || e < lim) m0 = fmaxf(m0, __uint_as_float(sr[0][e]));
-        m = fmaxf(m0 * scale, kNone);
+        m = fmaxf(m0 * scale - lift, kNone);
     }
     float sum = p_pass();
     if (__any_sync(0xffffffffu, !(sum <= kStaleSum))) {
@@ -394,7 +398,7 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, bool firs
 #pragma unroll
             for (int e = 0; e < 32; e++)
                 if (!mask || c * 32 + e < lim) mx = fmaxf(mx, __uint_as_float(sr[c][e]));
-        const float m_new = fmaxf(mx * scale, first ? kNone : m);
+        const float m_new = fmaxf(mx * scale - lift, first ? kNone : m);
         if (!first) {
             const float corr = ex2(m - m_new);
             wait_prev_pv();

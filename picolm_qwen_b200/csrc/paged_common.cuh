@@ -3,6 +3,8 @@
 #pragma once
 
 #include <cstdint>
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -151,6 +153,19 @@ __device__ __forceinline__ void rotate_pieces_fused(float* x, const float* c, co
 #pragma unroll
         for (int j = 0; j < V; j++) rotate_pair_fused(x[2 * j], x[2 * j + 1], c[j], s[j]);
     }
+}
+
+// The softmax weights go into the product with V in the cache's 16 bits: that is
+// what its tensor instructions take, and it costs an output half a step of the
+// type at most, as its own rounding does.  An fp16 weight is subnormal below
+// 2^-14 and nothing below 2^-25, which over a long context is more than that: all
+// of 131,072 keys at 2^-26 of a strong one make up 0.2% of the output.  So the
+// running maximum is held `lift` (log2) too low and every weight is 2^lift times as
+// large; sums and outputs carry the factor and it cancels at the end.  bf16 has
+// fp32's range.
+template <class T>
+__host__ __device__ constexpr float weight_lift(int lift) {
+    return std::is_same<T, __half>::value ? (float)lift : 0.f;
 }
 
 // Orders this thread's shared-memory writes before later async-proxy (TMA) accesses of them.

@@ -312,6 +312,8 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
     const uint32_t v_lane = (uint32_t)((lane & 7) * F::GS + ((lane >> 3) & 1) * F::ROW + (lane >> 4) * 16);
     const uint32_t tiles_u32 = smem_u32(tiles);
     const float scale = 1.4426950408889634f / sqrtf((float)HD);
+    // weights of up to 2^15 of fp16's 2^16 (weight_lift): below 2^-40 of the largest they vanish
+    constexpr float lift = weight_lift<T>(15);
     int t = 0;
     for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
         const int rows = sp.n * a.g;  // <= kRows
@@ -384,7 +386,7 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
                 mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
                 mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
                 mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-                const float mn0 = fmaxf(m[0], mx0), mn1 = fmaxf(m[1], mx1);
+                const float mn0 = fmaxf(m[0], mx0 - lift), mn1 = fmaxf(m[1], mx1 - lift);
                 const float f0 = ex2(m[0] - mn0), f1 = ex2(m[1] - mn1);
                 m[0] = mn0;
                 m[1] = mn1;

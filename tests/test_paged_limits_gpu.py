@@ -1,0 +1,48 @@
+"""The paged operators where a step is at the edge of what its description allows, against the formulas in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import pagedref as ref
+from test_paged_gpu import Batch, f64, rt  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+U_P = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}     # a weight's rounding
+TINY_P = {"f16": 2.0 ** -32, "bf16": 2.0 ** -130}  # the largest weight that may vanish, of a largest of 1
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("new,past", [([1], [300]), ([1, 3], [3000, 700]), ([40], [300]), ([70, 9], [200, 3000])])
+@pytest.mark.parametrize("strong_last", [False, True])
+def test_weights_far_below_the_largest(rt, new, past, cache, strong_last):  # noqa: F811
+    """One key takes nearly all of the weight and its V is 0, so that the output is what the others add up to: 2^-26 to
+    2^-28 each.  Tolerance: ref.attention's, with weights off by half a step or by 2^-32 of the largest."""
+    hq, hkv, hd, page = 4, 2, 64, 16
+    B = Batch(rt, new, past, hq, hkv, hd, page, cache, layers=1)
+    for b, t in enumerate(B.total):
+        ids = B.pages[b, :-(-t // page)].long()
+        r = torch.arange(len(ids) * page, device="cuda")
+        strong = past[b] - 1 if strong_last else 0
+        far = -18.5 + 0.5 * (r % 3 - 1)  # natural units: 2^-26 to 2^-27.4
+        k = torch.zeros((len(ids) * page, hkv, hd), device="cuda")
+        k[..., 0] = torch.where(r == strong, 0.0, far)[:, None]
+        v = torch.where(r == strong, 0.0, 1.0)[:, None, None].expand_as(k).clone()
+        k[t:], v[t:] = float("nan"), float("nan")
+        for pool, x in ((B.cache.k_pool, k), (B.cache.v_pool, v)):
+            pool[0, ids] = x.to(B.dt).view(len(ids), page, hkv, hd).permute(0, 2, 1, 3)
+    q = torch.zeros((B.n_tok, hq, hd), device="cuda")
+    q[..., 0] = hd ** 0.5
+    q = q.to(B.dt)
+    y = torch.full((B.n_tok, hq, hd), float("nan"), device="cuda")
+    B.cache.attend(0, B.batch, q, y)
+    assert B.batch.status() == 0
+    got, qd = f64(y), f64(q)
+    for b in range(len(new)):
+        a, e = B.start[b], B.start[b + 1]
+        k, v = (f64(B.rows(p, 0, b, B.total[b])) for p in (B.cache.k_pool, B.cache.v_pool))
+        for h in range(hq):
+            w, err = ref.attention(qd[a:e, h], k[:, h // 2], v[:, h // 2], past[b], hd ** -0.5, U_P[cache], TINY_P[cache])
+            d = np.abs(got[a:e, h] - w)
+            tol = err + 2.0 ** -24 * w
+            assert (w > 0).all() and (d <= tol).all(), f"sequence {b} head {h}: {(d / tol).max():.3g} of the tolerance"
