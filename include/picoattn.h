@@ -683,7 +683,9 @@ int32_t picoattn_paged_check(const picoattn_config_t* cfg, const picoattn_paged_
 /* Bytes of a workspace for picoattn_paged_append and picoattn_paged_attn on
  * batches of up to n_seqs sequences, whatever their lengths (0: the config or
  * n_seqs is not accepted).  Call picoattn_workspace_init once on it; calls that
- * may run at the same time need workspaces of their own. */
+ * may run at the same time need workspaces of their own.  Calls of the other
+ * entries whose workspace has a header may use it in between (not picoattn_ffn
+ * and picoattn_logits, which keep data there). */
 size_t picoattn_paged_workspace_size(const picoattn_config_t* cfg, int32_t n_seqs);
 
 /* Inputs and output of picoattn_paged_append. */

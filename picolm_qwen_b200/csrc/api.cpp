@@ -286,7 +286,7 @@ int32_t picoattn_prefill_staged(const picoattn_config_t* cfg, int32_t layer, int
     a.q = q, a.k = k, a.v = v, a.qn_w = q_norm_w, a.kn_w = k_norm_w, a.rope_cos = rope_cos, a.rope_sin = rope_sin;
     a.k_cache = k_cache, a.v_cache = v_cache, a.out = out;
     a.status = reinterpret_cast<unsigned int*>(w);
-    a.work_counter = reinterpret_cast<int*>(w + 64);
+    a.work_counter = &reinterpret_cast<WsHeader*>(w)->prefill_work;
     a.q16 = reinterpret_cast<__half*>(w + kWsHeaderBytes);
     return cuda_status(launch_prefill(a, (cudaStream_t)stream, stages));
 }

@@ -1067,7 +1067,7 @@ cudaError_t launch_types(const PagedAttnArgs& a, cudaStream_t stream) {
     ChunkArgs c{};
     c.a = a;
     c.tq = BM / a.g;
-    c.counter = reinterpret_cast<int*>(a.b.status) + 16;  // in the workspace header
+    c.counter = &reinterpret_cast<WsHeader*>(a.b.status)->paged_work;
     c.meta = reinterpret_cast<ChunkMeta*>(a.ws);
     c.part_ml = reinterpret_cast<float2*>(a.ws + kMetaBytes);
     c.part_o = reinterpret_cast<float*>(a.ws + kMetaBytes + kMlBytes);

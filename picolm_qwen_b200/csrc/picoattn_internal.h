@@ -15,9 +15,14 @@ namespace picoattn {
 // Workspace header: the first 256 bytes of every workspace.
 struct WsHeader {
     unsigned int status;  // sticky PICOATTN_DEV_* bits
-    unsigned int pad[63];
+    unsigned int pad0[15];
+    int prefill_work;     // picoattn_prefill's queue: set by each call's prep kernel, left as its attention ends
+    unsigned int pad1[15];
+    int paged_work;       // picoattn_paged_attn's queue: zero between calls, so no other call may use the word
+    unsigned int pad2[31];
 };
 constexpr size_t kWsHeaderBytes = 256;
+static_assert(sizeof(WsHeader) == kWsHeaderBytes, "the header");
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 

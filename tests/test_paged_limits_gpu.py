@@ -46,3 +46,22 @@ def test_weights_far_below_the_largest(rt, new, past, cache, strong_last):  # no
             d = np.abs(got[a:e, h] - w)
             tol = err + 2.0 ** -24 * w
             assert (w > 0).all() and (d <= tol).all(), f"sequence {b} head {h}: {(d / tol).max():.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("new,past", [([2000], [40]), ([1, 1], [600, 40])])
+def test_a_workspace_that_a_prefill_used(rt, new, past):  # noqa: F811
+    """Calls one after the other may share a workspace, those of the contiguous entries too."""
+    from picolm_qwen_b200 import abi
+    hq, hkv, hd, n = 32, 8, 64, 700
+    B = Batch(rt, new, past, hq, hkv, hd, 16, "f16")
+    B.fill(0)
+    q = B.rand(B.n_tok, hq, hd).half()
+    want, got = (torch.full((B.n_tok, hq, hd), float("nan"), device="cuda").half() for _ in range(2))
+    B.cache.attend(0, B.batch, q, want)
+    cfg = abi.Config.make(1, hq, hkv, hd, n, 1e4)
+    st = rt.AttnState(cfg)
+    out = torch.empty((n, hq * hd), device="cuda")
+    assert st.prefill(0, 0, B.rand(n, hq * hd), B.rand(n, hkv * hd), B.rand(n, hkv * hd), out,
+                      workspace=B.batch.workspace) == 0
+    B.cache.attend(0, B.batch, q, got)
+    assert B.batch.status() == 0 and torch.equal(got, want)
