@@ -759,10 +759,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const SeqSpan sp = seq_span(a.b, b);
             if (sp.ok) continue;
             if (tid == 0) atomicOr(status, PICOATTN_DEV_BAD_POS);
-            const int t0 = max(sp.t0, 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
-            const long long n = t1 > t0 ? (long long)(t1 - t0) * a.hq * HD : 0;
-            for (long long i = tid; i < n; i += 256) {
-                const size_t at = (size_t)t0 * a.hq * HD + i;
+            const RowRange rows = rows_inside(a.b, b);
+            for (long long i = tid; i < rows.n * a.hq * HD; i += 256) {
+                const size_t at = (size_t)rows.first * a.hq * HD + i;
                 if (a.out_dtype == PICOATTN_DTYPE_F32) static_cast<float*>(a.out)[at] = __int_as_float(0x7fc00000);
                 else static_cast<T*>(a.out)[at] = Elem<T>::round(__int_as_float(0x7fc00000));
             }

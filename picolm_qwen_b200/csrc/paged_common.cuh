@@ -191,9 +191,19 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedBatch& a, int b) {
     s.t0 = a.q_start[b];
     const int t1 = a.q_start[b + 1];
     s.len = a.kv_len[b];
-    s.n = t1 - s.t0;  // wraps only for spans that fail the range test
+    s.n = (int)((unsigned)t1 - (unsigned)s.t0);  // wraps only for spans that fail the range test
     s.ok = s.t0 >= 0 && t1 >= s.t0 && t1 <= a.n_tok && s.n <= a.max_new && s.len >= s.n && s.len <= a.max_len;
     return s;
+}
+
+// The rows of a sequence outside the bounds that lie inside [0, n_tok).
+struct RowRange {
+    int first;
+    long long n;  // 0: none
+};
+__device__ __forceinline__ RowRange rows_inside(const PagedBatch& a, int b) {
+    const int t0 = max(a.q_start[b], 0), t1 = min(a.q_start[b + 1], a.n_tok);
+    return {t0, t1 > t0 ? t1 - t0 : 0};  // both ends may be any 32-bit values: t1 - t0 only where it cannot wrap
 }
 
 }  // namespace picoattn

@@ -156,11 +156,11 @@ __device__ __forceinline__ void for_each_part(const PagedAttnArgs& a, int b0, lo
 template <class T, int HD>
 __device__ __forceinline__ void nan_rows(const PagedAttnArgs& a, int b, int h, int tid, int threads) {
     constexpr int C4 = HD / 4;
-    const int t0 = max(a.b.q_start[b], 0), t1 = min(a.b.q_start[b + 1], a.b.n_tok);
+    const RowRange rows = rows_inside(a.b, b);
     const float nan = __int_as_float(0x7fc00000);
-    for (long long i = tid; i < (long long)(t1 - t0) * a.g * C4; i += threads) {
+    for (long long i = tid; i < rows.n * a.g * C4; i += threads) {
         const long long x = i / C4;
-        store_out4<T>(a, ((size_t)(t0 + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * (i % C4),
+        store_out4<T>(a, ((size_t)(rows.first + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * (i % C4),
                       make_float4(nan, nan, nan, nan));
     }
 }

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import pagedref as ref
-from test_paged_gpu import Batch, f64, rt  # noqa: F401
+from test_paged_gpu import HALF, TINY, Batch, f64, gpu_attn, rt  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,47 @@ def test_a_workspace_that_a_prefill_used(rt, new, past):  # noqa: F811
                       workspace=B.batch.workspace) == 0
     B.cache.attend(0, B.batch, q, got)
     assert B.batch.status() == 0 and torch.equal(got, want)
+
+
+I32 = 2 ** 31 - 1
+SPANS = [  # q_start of three sequences whose own rows would be 0-1, 2-4, 5
+    [6, 2, -1, 6],                # ends before their beginnings, then a beginning below 0
+    [0, 2, 2 * 10 ** 9, 6],       # past n_tok, then before it
+    [I32, -I32 - 1, 0, 6],        # whose difference passes 32 bits
+    [-5, 2, I32, -2],
+    [-I32 - 1, I32, 6, 6],
+    [0, 2, 5, I32],
+]
+
+
+@pytest.mark.parametrize("spans", SPANS)
+@pytest.mark.parametrize("form", ["streams", "slices", "blocks", "cut blocks"])
+def test_attention_of_spans_outside_the_batch(rt, spans, form):  # noqa: F811
+    """In each way that a batch is split.  Any values in q_start: a sequence with rows outside [0, n_tok), or an end before its beginning, is flagged; the
+    rows of the step that it covers are NaN, those of no sequence are not written, a good sequence's are the formula's."""
+    from picolm_qwen_b200 import abi
+    past = 3000 if form in ("slices", "cut blocks") else 40
+    B = Batch(rt, [2, 3, 1], [past] * 3, 8, 2, 64, 16, "f16", layers=1)
+    B.batch = B.cache.batch(B.pages, B.q_start, B.kv_len, 6, 6 if form in ("streams", "slices") else 30,
+                            B.cfg.max_seq_len)
+    B.fill(0)
+    q = B.rand(8, 8, 64).half()[1:7]  # a row more on both sides of q and out
+    area = torch.full((8, 8, 64), 7.0, device="cuda").half()
+    want, err = gpu_attn(B, 0, q)
+    tol = err + HALF[B.dt] * (want.abs() + err) + TINY[B.dt]
+    B.q_start.copy_(torch.tensor(spans, dtype=torch.int64).to(torch.int32))
+    B.cache.attend(0, B.batch, q, area[1:7])
+    assert B.batch.status() == abi.DEV_BAD_POS
+    assert (area[[0, 7]] == 7).all()
+    for t in range(6):
+        covers = [b for b in range(3) if max(spans[b], 0) <= t < min(spans[b + 1], 6)]
+        bad = [b for b in covers if not 0 <= spans[b] <= spans[b + 1] <= 6]
+        y = area[1 + t]
+        if not covers:
+            assert (y == 7).all(), t
+        elif bad:
+            assert y.isnan().all(), t
+        elif spans[covers[0]:covers[0] + 2] == B.start[covers[0]:covers[0] + 2]:
+            assert ((y.double() - want[t]).abs() <= tol[t]).all(), t
+        else:
+            assert y.isfinite().all(), t
