@@ -665,7 +665,8 @@ typedef struct {
  * device values: a sequence with more than max_new new tokens, a kv_len above
  * max_len or below its new tokens, or rows outside [0, n_tok) sets
  * PICOATTN_DEV_BAD_POS, leaves the cache as it was, and its q_out / out rows
- * (those inside [0, n_tok)) are NaN. */
+ * (those inside [0, n_tok)) are NaN.  So does a q_start that decreases; tokens
+ * that another sequence's span covers as well may then be NaN and not stored. */
 typedef struct {
     int32_t n_seqs;            /* at least 1 */
     int32_t n_tok;             /* rows of q, k, v, out; at least 1 */

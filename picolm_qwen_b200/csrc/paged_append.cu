@@ -84,13 +84,15 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(PagedAp
         const int b = seq_of(a.b, (int)tok, lane);
         if (b >= a.b.n_seqs) continue;       // a row behind the last sequence
         const SeqSpan span = seq_span(a.b, b);
-        if ((int)tok < span.t0) continue;    // a row before the first sequence
-        if (!span.ok && lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
-        const int pos = span.ok ? span.len - span.n + ((int)tok - span.t0) : 0;
+        if (b == 0 && (int)tok < span.t0) continue;  // a row before the first sequence
+        // seq_of takes q_start as not decreasing: one that decreases may give a sequence without this token
+        const bool ok = span.ok && (int)tok >= span.t0 && (int)tok - span.t0 < span.n;
+        if (!ok && lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+        const int pos = ok ? span.len - span.n + ((int)tok - span.t0) : 0;
         TC* dst = static_cast<TC*>(a.q_out) + ((long long)tok * a.hq + h0) * HD;
         int hop = HPS * HD;
         if (kind != 0) {
-            if (!span.ok) continue;
+            if (!ok) continue;
             const int page = a.b.page_table[(size_t)b * a.b.page_cols + (pos >> a.b.page_shift)];
             if (page < 0 || page >= a.b.n_pages) {
                 if (lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_PAGE);
@@ -155,7 +157,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(PagedAp
             if (kind == 1) {
                 store_pieces<TC, true>(x, dst + (size_t)i * hop, at);
             } else {
-                if (!span.ok) {
+                if (!ok) {
 #pragma unroll
                     for (int j = 0; j < 16; j++) x[j] = __int_as_float(0x7fc00000);
                 }

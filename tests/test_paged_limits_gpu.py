@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import pagedref as ref
-from test_paged_gpu import HALF, TINY, Batch, f64, gpu_attn, rt  # noqa: F401
+from test_paged_gpu import HALF, TINY, Batch, f64, gpu_attn, rt, table  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,28 @@ def test_attention_of_spans_outside_the_batch(rt, spans, form):  # noqa: F811
             assert ((y.double() - want[t]).abs() <= tol[t]).all(), t
         else:
             assert y.isfinite().all(), t
+
+
+def test_append_of_a_decreasing_q_start(rt):  # noqa: F811
+    """Tokens that are not their sequence's own by its span: flagged, NaN, and no row of the cache is written for them."""
+    from picolm_qwen_b200 import abi
+    hq, hkv, hd, page, n = 4, 2, 64, 16, 100
+    B = Batch(rt, [n, 0, 3], [7, 40, 21], hq, hkv, hd, page, "f16", layers=2)
+    B.fill(1, upto=B.past)
+    pools = B.cache.k_pool, B.cache.v_pool
+    before = [p.clone() for p in pools]
+    B.batch = B.cache.batch(B.pages, B.q_start, B.kv_len, n, n, max(B.total))
+    B.q_start.copy_(torch.tensor([0, n, 2, 5], dtype=torch.int32))
+    q, k, v = B.rand(n, hq, hd), B.rand(n, hkv, hd), B.rand(n, hkv, hd)
+    qo = torch.full((n, hq, hd), 7.0, device="cuda").half()
+    B.cache.append(1, B.batch, q, k, v, *table(B.cfg.max_seq_len, hd), qo)
+    assert B.batch.status() == abi.DEV_BAD_POS
+    nan = qo.isnan().flatten(1)
+    assert not nan[:2].any() and nan[2:].all()  # 2 to 4 go to the second sequence by number, the others to the third
+    written = {(0, 7): 0, (0, 8): 1}  # positions of the first sequence
+    for pool, old in zip(pools, before):
+        same = ((pool == old) | (pool.isnan() & old.isnan())).all(-1)  # [layer, page, head, row]
+        changed = {(i, p, r) for i, p, h, r in (~same).nonzero().tolist()}
+        assert changed == {(1, int(B.pages[b, r // page]), r % page) for b, r in written}
+    for (b, r), t in written.items():
+        assert (B.rows(pools[1], 1, b, r + 1)[r].float() - v[t]).abs().max() <= 2.0 ** -11 * 8  # |v| < 8
