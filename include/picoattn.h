@@ -742,7 +742,9 @@ int32_t picoattn_paged_append(const picoattn_config_t* cfg, const picoattn_paged
  * Batches whose work does not fit 32-bit counts (with T = 2*floor(128 / q heads
  * per KV head): max_new/T * max_len/32 or (n_tok/T + n_seqs) * n_kv_heads) are
  * PICOATTN_EUNSUPPORTED.
- * After PICOATTN_DEV_TIMEOUT the outputs of the call are not defined.
+ * After PICOATTN_DEV_TIMEOUT the outputs of the call are not defined, nor those of
+ * calls on the workspace until the status has been read: their waits give up at
+ * once.
  */
 int32_t picoattn_paged_attn(const picoattn_config_t* cfg, const picoattn_paged_cache_t* cache, int32_t layer,
                             const picoattn_paged_batch_t* batch, const void* q, int64_t q_stride,

@@ -272,8 +272,10 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
     if (warp == kWarps) {
         // ---------------- producer: lanes 0-7 the K groups, 8-15 the V groups ----------------
         int t = 0;
+        bool ok = true;  // no wait has run out: then nothing more is copied
         const uint8_t* pool = static_cast<const uint8_t*>(lane & 8 ? a.v_pool : a.k_pool);
         for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
+            if (!ok) return;
             if (!kWhole && lane == 0 && !fa.by_cta && u0 == 0 && u1 == stream_units)
                 fa.cut[b * a.hkv + h] = make_int4(0, 0, 1, 0);  // not cut
             const int r1 = min(u1 * kUnit, sp.len);
@@ -286,7 +288,10 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
                 const bool bad = page < 0 || page >= a.b.n_pages;
                 const int any_bad = __any_sync(0xffffffffu, bad);
                 const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, copy)) * (uint32_t)(F::GR * F::ROW);
-                if (t >= kStages) mbar_wait(&empty[s], (uint32_t)((t / kStages - 1) & 1), a.b.status);
+                if (t >= kStages) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)((t / kStages - 1) & 1), a.b.status));
+                    if (!ok) return;
+                }
                 if (lane == 0) {
                     if (any_bad) atomicOr(a.b.status, PICOATTN_DEV_BAD_PAGE);
                     poison[s] = any_bad;
@@ -300,6 +305,9 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
                 }
             }
         });
+        // the compute warps may have given up on copies still on their way: they land before the CTA ends
+        if (lane == 0)
+            for (int c = max(0, t - kStages); c < t; c++) mbar_settle(&full[c % kStages], (uint32_t)((c / kStages) & 1));
         return;
     }
 
@@ -315,7 +323,9 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
     // weights of up to 2^15 of fp16's 2^16 (weight_lift): below 2^-40 of the largest they vanish
     constexpr float lift = weight_lift<T>(15);
     int t = 0;
+    bool ok = true;  // no wait of this warp has run out (of any compute warp, between parts): then nothing more is stored
     for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
+        if (!ok) return;
         const int rows = sp.n * a.g;  // <= kRows
         uint32_t qa[HD / 16][4];
         int lim[2];  // keys below it are visible to the lane's rows gid, gid + 8
@@ -339,7 +349,8 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
         const int r1 = min(u1 * kUnit, sp.len);
         for (int row0 = u0 * kUnit; row0 < r1; row0 += F::T, t++) {
             const int s = t % kStages;
-            mbar_wait(&full[s], (uint32_t)((t / kStages) & 1), a.b.status);
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (uint32_t)((t / kStages) & 1), a.b.status));
+            if (!ok) break;  // the stage is not given back either
             const uint32_t kbase = tiles_u32 + (uint32_t)(s * 2 * F::TILE), vbase = kbase + F::TILE;
             const int valid = r1 - row0;
             if (poison[s]) l[0] = l[1] = __int_as_float(0x7fc00000);
@@ -428,7 +439,8 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
             if (tig == 0) ml[warp * 16 + gid + 8 * half] = make_float2(m[half], l[half]);
         }
-        named_bar_sync(1, 32 * kWarps);
+        ok = named_bar_all(1, 32 * kWarps, ok);
+        if (!ok) return;
         float wgt[2];
 #pragma unroll
         for (int half = 0; half < 2; half++) {
@@ -496,6 +508,7 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     const int tid = threadIdx.x, c4 = tid % C4, grp = tid / C4;
     const int r = blockIdx.x;
     const int4 cut = __ldcg(fa.cut + blockIdx.y);
+    if (__ldcg(a.b.status) & PICOATTN_DEV_TIMEOUT) return;  // entries and parts may not have been written
     if (fa.by_cta && cut.x < 0) return;
     const int stream = fa.by_cta ? cut.x : (int)blockIdx.y;
     const int b = stream / a.hkv, h = stream - b * a.hkv;

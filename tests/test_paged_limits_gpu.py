@@ -134,3 +134,32 @@ def test_append_of_a_decreasing_q_start(rt):  # noqa: F811
         assert changed == {(1, int(B.pages[b, r // page]), r % page) for b, r in written}
     for (b, r), t in written.items():
         assert (B.rows(pools[1], 1, b, r + 1)[r].float() - v[t]).abs().max() <= 2.0 ** -11 * 8  # |v| < 8
+
+
+@pytest.mark.parametrize("new,past", [([1, 2, 1], [40, 300, 9]), ([1, 2, 1], [9000, 3000, 40]), ([5, 7], [9000, 40])])
+def test_waits_that_give_up(rt, new, past):  # noqa: F811
+    """With the sticky timeout bit set, every wait of the call gives up unless its phase is there already: rows are the
+    formula's or as they were, the bit stays until it is read, the next call is as ever; so is a call on another
+    workspace beside it."""
+    from picolm_qwen_b200 import abi
+    B = Batch(rt, new, past, 8, 2, 64, 16, "f16", layers=1)
+    B.fill(0)
+    other = B.cache.batch(B.pages, B.q_start, B.kv_len, B.n_tok, max(new), max(B.total))
+    q = B.rand(B.n_tok, 8, 64).half()
+    want, err = gpu_attn(B, 0, q)
+    tol = err + HALF[B.dt] * (want.abs() + err) + TINY[B.dt]
+    good = lambda y: ((y.double() - want).abs() <= tol).all(-1)  # noqa: E731
+    side, rest = torch.cuda.Stream(), torch.empty_like(q)
+    y = torch.full_like(q, 7.0)
+    B.batch.workspace[0] = abi.DEV_TIMEOUT
+    torch.cuda.synchronize()
+    for _ in range(20):
+        B.cache.attend(0, B.batch, q, y)
+        B.cache.attend(0, other, q, rest, stream=side)
+    side.synchronize()
+    assert B.batch.status() == abi.DEV_TIMEOUT and other.status() == 0
+    assert good(rest).all()
+    assert (good(y) | (y == 7).all(-1)).all()
+    y.fill_(7.0)
+    B.cache.attend(0, B.batch, q, y)
+    assert B.batch.status() == 0 and good(y).all()
