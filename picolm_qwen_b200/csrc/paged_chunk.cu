@@ -479,7 +479,7 @@ __device__ __forceinline__ bool load_tiles(const PagedAttnArgs& a, const CUtenso
     return true;
 }
 
-// Giving up: the copies still on their way into the ring.
+// The copies still on their way into the ring: what a copy warp ends with, as whoever was to wait for them may have given up.
 __device__ __forceinline__ void settle_ring(uint64_t* full, int t) {
     for (int c = max(0, t - kRing); c < t; c++) mbar_settle(&full[c % kRing], (uint32_t)((c / kRing) & 1));
 }
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             wk.b = run * per;
             wk.base = plan->first_cost[run];
         }
-        int t = 0;
+        int t = 0, loads = 0;  // half tiles of K; Q loads
         bool ok = true;
         for (int k = 0; ok; k++) {
             const int slot = k & 1;
@@ -615,10 +615,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tma_load_3d(smem + L::kQ + w * L::kTile + x * L::kBox, &tmQ, 64 * x, it.h * g, it.tok0 + w * tq,
                                     q_full);
             }
+            loads++;
             ok = load_tiles<HD>(a, tmK, it, &items[slot].poison, smem + L::kK, k_full, k_empty, t, status, lane);
-            if (!ok) mbar_settle(q_full, (uint32_t)(k & 1));
         }
-        if (!ok) settle_ring(k_full, t);
+        if (loads) mbar_settle(q_full, (uint32_t)((loads - 1) & 1));
+        settle_ring(k_full, t);
     } else if (warp == 11) {
         // ---------------- TMA of V ----------------
         int t = 0;
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(&item_empty[slot]);
             if (it.b < 0) break;
         }
-        if (!ok) settle_ring(v_full, t);
+        settle_ring(v_full, t);
     } else if (warp >= 8) {
         // ---------------- MMA issue: one warp per softmax group ----------------
         // Each waits for what is ready early (V, the next K) while its group is still

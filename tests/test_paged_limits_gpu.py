@@ -163,3 +163,29 @@ def test_waits_that_give_up(rt, new, past):  # noqa: F811
     y.fill_(7.0)
     B.cache.attend(0, B.batch, q, y)
     assert B.batch.status() == 0 and good(y).all()
+
+
+@pytest.mark.parametrize("new,past", [([40, 1], [30, 9]), ([400, 1, 33], [900, 3000, 40]), ([2000], [40])])
+def test_waits_of_chunks_that_give_up(rt, new, past):  # noqa: F811
+    """The same for the chunk kernel, whose outputs are not defined then: nothing but them is written, a call on another
+    workspace beside it and the next one are as ever."""
+    from picolm_qwen_b200 import abi
+    B = Batch(rt, new, past, 8, 2, 64, 16, "f16", layers=1)
+    B.fill(0)
+    other = B.cache.batch(B.pages, B.q_start, B.kv_len, B.n_tok, max(new), max(B.total))
+    q = B.rand(B.n_tok, 8, 64).half()
+    want, err = gpu_attn(B, 0, q)
+    tol = err + HALF[B.dt] * (want.abs() + err) + TINY[B.dt]
+    good = lambda y: ((y.double() - want).abs() <= tol).all()  # noqa: E731
+    side, rest = torch.cuda.Stream(), torch.empty_like(q)
+    area = torch.full((B.n_tok + 2, 8, 64), 7.0, device="cuda").half()
+    B.batch.workspace[0] = abi.DEV_TIMEOUT
+    torch.cuda.synchronize()
+    for _ in range(20):
+        B.cache.attend(0, B.batch, q, area[1:-1])
+        B.cache.attend(0, other, q, rest, stream=side)
+    side.synchronize()
+    assert B.batch.status() == abi.DEV_TIMEOUT and other.status() == 0
+    assert good(rest) and (area[[0, -1]] == 7).all()
+    B.cache.attend(0, B.batch, q, area[1:-1])
+    assert B.batch.status() == 0 and good(area[1:-1])
