@@ -61,11 +61,17 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(PagedAp
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (blockIdx.x == 0) {  // the bounds of all sequences, those without a row in this call too
+        bool bad = false;
+        for (int b = threadIdx.x; b < a.b.n_seqs; b += kAppendWarps * 32) bad |= !seq_span(a.b, b).ok;
+        if (bad) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
+        return;
+    }
     const bool neox = a.mode == PICOATTN_ROPE_NEOX;
     const PieceAt at = piece_at<8>(lane % LPH, a.rot, neox);
     const bool vec = (((uintptr_t)a.cos_t | (uintptr_t)a.sin_t | (uintptr_t)a.qn_w | (uintptr_t)a.kn_w) & 15) == 0;
     const unsigned units = sp.q_units + 2 * sp.kv_units;
-    for (unsigned u = blockIdx.x * kAppendWarps + warp; u < units; u += gridDim.x * kAppendWarps) {
+    for (unsigned u = (blockIdx.x - 1) * kAppendWarps + warp; u < units; u += (gridDim.x - 1) * kAppendWarps) {
         const int kind = u < sp.q_units ? 0 : (u < sp.q_units + sp.kv_units ? 1 : 2);
         const unsigned i0 = u - (kind == 0 ? 0 : (kind == 1 ? sp.q_units : sp.q_units + sp.kv_units));
         const unsigned per = kind == 0 ? sp.q_per : sp.kv_per, tok = i0 / per;
@@ -85,9 +91,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(PagedAp
         if (b >= a.b.n_seqs) continue;       // a row behind the last sequence
         const SeqSpan span = seq_span(a.b, b);
         if (b == 0 && (int)tok < span.t0) continue;  // a row before the first sequence
-        // seq_of takes q_start as not decreasing: one that decreases may give a sequence without this token
+        // seq_of takes q_start as not decreasing: one that decreases (and is flagged) may give a sequence without this
+        // token
         const bool ok = span.ok && (int)tok >= span.t0 && (int)tok - span.t0 < span.n;
-        if (!ok && lane == 0) atomicOr(a.b.status, PICOATTN_DEV_BAD_POS);
         const int pos = ok ? span.len - span.n + ((int)tok - span.t0) : 0;
         TC* dst = static_cast<TC*>(a.q_out) + ((long long)tok * a.hq + h0) * HD;
         int hop = HPS * HD;
@@ -177,7 +183,7 @@ cudaError_t launch_hd(const PagedAppendArgs& a, cudaStream_t stream) {
     sp.q_units = (unsigned)a.b.n_tok * sp.q_per;
     sp.kv_units = (unsigned)a.b.n_tok * sp.kv_per;
     const unsigned grid = (unsigned)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, 12LL * device_sm_count());
-    return launch_pdl(paged_append_kernel<TI, TC, HD>, dim3(grid), dim3(kAppendWarps * 32), 0, stream, a, sp);
+    return launch_pdl(paged_append_kernel<TI, TC, HD>, dim3(1 + grid), dim3(kAppendWarps * 32), 0, stream, a, sp);
 }
 
 template <class TI, class TC>

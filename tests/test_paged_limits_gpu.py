@@ -189,3 +189,27 @@ def test_waits_of_chunks_that_give_up(rt, new, past):  # noqa: F811
     assert good(rest) and (area[[0, -1]] == 7).all()
     B.cache.attend(0, B.batch, q, area[1:-1])
     assert B.batch.status() == 0 and good(area[1:-1])
+
+
+@pytest.mark.parametrize("bad", ["kv_len", "rows"])
+def test_append_flags_sequences_without_a_row(rt, bad):  # noqa: F811
+    """A sequence outside the bounds is flagged whether or not one of the call's rows is its own, as by the attention."""
+    from picolm_qwen_b200 import abi
+    B = Batch(rt, [3, 0, 0], [20, 9, 4], 4, 2, 64, 16, "f16", layers=1)
+    B.fill(0)
+    q, k, v = B.rand(3, 4, 64), B.rand(3, 2, 64), B.rand(3, 2, 64)
+    tab = table(B.cfg.max_seq_len, 64)
+    want, got = (torch.full((3, 4, 64), float("nan"), device="cuda").half() for _ in range(2))
+    B.cache.append(0, B.batch, q, k, v, *tab, want)
+    assert B.batch.status() == 0
+    if bad == "kv_len":
+        B.kv_len[1] = -1
+    else:
+        B.q_start[3] = 5  # the last sequence's rows lie behind n_tok
+    for name in ("append", "attend"):
+        if name == "append":
+            B.cache.append(0, B.batch, q, k, v, *tab, got)
+        else:
+            B.cache.attend(0, B.batch, got, torch.empty_like(got))
+        assert B.batch.status() == abi.DEV_BAD_POS, name
+    assert torch.equal(got, want)
