@@ -213,3 +213,35 @@ def test_append_flags_sequences_without_a_row(rt, bad):  # noqa: F811
             B.cache.attend(0, B.batch, got, torch.empty_like(got))
         assert B.batch.status() == abi.DEV_BAD_POS, name
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1, 1], [40, 1, 3, 70, 9]])
+def test_good_sequences_beside_bad_ones(rt, new):  # noqa: F811
+    """Bad pages and lengths beside good sequences, whose rows are the formula's."""
+    from picolm_qwen_b200 import abi
+    B = Batch(rt, new, [300, 20, 50, 10, 400], 8, 2, 128, 16, "f16", layers=1)
+    B.fill(0)
+    q = B.rand(B.n_tok, 8, 128).half()
+    want, err = gpu_attn(B, 0, q)
+    tol = err + HALF[B.dt] * (want.abs() + err) + TINY[B.dt]
+
+    def expect(bits, bad):
+        y = torch.full((B.n_tok, 8, 128), 7.0, device="cuda").half()
+        B.cache.attend(0, B.batch, q, y)
+        assert B.batch.status() == bits
+        for b in range(5):
+            rows = slice(B.start[b], B.start[b + 1])
+            if b in bad:
+                assert y[rows].isnan().all(), b
+            else:
+                d = (y[rows].double() - want[rows]).abs()
+                assert (d <= tol[rows]).all(), f"sequence {b}: {float((d / tol[rows]).max()):.3g} of the tolerance"
+
+    pages = B.pages.clone()
+    B.pages[0, 2] = B.cache.k_pool.shape[1]
+    B.pages[3, 0] = -1
+    expect(abi.DEV_BAD_PAGE, {0, 3})
+    B.pages.copy_(pages)
+    B.kv_len[1] = 0
+    B.kv_len[4] = 1 << 30
+    expect(abi.DEV_BAD_POS, {1, 4})
