@@ -117,13 +117,13 @@ def _dtype(t: torch.Tensor) -> int:
 
 
 def _heads(t: torch.Tensor, n: int, heads: int, hd: int, what: str) -> int:
-    """The row stride of t, [n, heads, hd] or [n, heads*hd], each row's heads contiguous."""
+    """The row stride of t, [n, heads, hd] or [n, heads*hd], each row's heads contiguous (one row's may be any number)."""
     shape, st = t.shape, t.stride()
     if len(shape) == 3:
         if shape == (n, heads, hd) and st[2] == 1 and (st[1] == hd or heads == 1):
-            return st[0]
+            return st[0] if n != 1 else heads * hd
     elif shape == (n, heads * hd) and st[1] == 1:
-        return st[0]
+        return st[0] if n != 1 else heads * hd
     raise ValueError(f"{what}: [{n}, {heads}, {hd}] or [{n}, {heads * hd}] with contiguous rows, got {tuple(shape)} "
                      f"strides {st}")
 

@@ -245,3 +245,25 @@ def test_good_sequences_beside_bad_ones(rt, new):  # noqa: F811
     B.kv_len[1] = 0
     B.kv_len[4] = 1 << 30
     expect(abi.DEV_BAD_POS, {1, 4})
+
+
+def test_one_token_tensors_of_any_stride(rt):  # noqa: F811
+    """A dimension of size 1 may have any stride, such as one token's heads turned to the front."""
+    hq, hkv, hd = 4, 2, 64
+    B = Batch(rt, [1], [35], hq, hkv, hd, 16, "f16", layers=1)
+    B.fill(0, upto=[35])
+    cos, sin = table(B.cfg.max_seq_len, hd)
+    pos, ws = torch.tensor([35], device="cuda", dtype=torch.int32), rt.status_workspace()
+    plain = [B.rand(1, h, hd).half() for h in (hq, hkv, hkv)]
+    turned = [torch.empty_strided(t.shape, (hd, hd, 1), device="cuda", dtype=t.dtype).copy_(t) for t in plain]
+    got = []
+    for q, k, v in (plain, turned):
+        assert q.is_contiguous()
+        r, o, qo = (torch.empty_strided(q.shape, q.stride(), device="cuda", dtype=q.dtype) for _ in range(3))
+        rk = torch.empty_strided(k.shape, k.stride(), device="cuda", dtype=k.dtype)
+        rt.rope(q, k, pos, cos, sin, r, rk, ws)
+        B.cache.append(0, B.batch, q, k, v, cos, sin, qo)
+        B.cache.attend(0, B.batch, qo, o)
+        got.append([t.clone() for t in (r, rk, qo, o, B.rows(B.cache.k_pool, 0, 0, 36), B.rows(B.cache.v_pool, 0, 0, 36))])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
