@@ -148,7 +148,12 @@ def _launch(index: int, stream, what: str, call, *args) -> None:
     """call(*args, stream) with device `index` current (whichever the caller has), its error raised."""
     if index < 0:
         raise ValueError(f"{what}: tensors on the CPU")
-    handle = _raw_stream(index) if stream is None else stream.cuda_stream
+    if stream is None:
+        handle = _raw_stream(index)
+    else:
+        if stream.device_index != index:
+            raise ValueError(f"{what}: a stream of device {stream.device_index}, tensors on device {index}")
+        handle = stream.cuda_stream
     if torch.cuda.current_device() == index:
         st = call(*args, handle)
     else:
@@ -231,6 +236,7 @@ class PagedBatch:
             if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"{name}: contiguous int32 {shape}, got {tuple(t.shape)} {t.dtype}")
         _same_device(cache.index, "batch", page_table, q_start, kv_len)
+        self.index = cache.index
         self.tensors = (page_table, q_start, kv_len)  # kept alive with the struct
         self.n_tok = n_tok
         self.desc = abi.PagedBatchDesc(n, n_tok, max_new, max_len, page_table.shape[1], page_table.data_ptr(),
@@ -301,6 +307,8 @@ class PagedCache:
                     raise ValueError(f"norm weights: both, contiguous fp32 [{hd}]")
             qn, kn = q_norm_w.data_ptr(), k_norm_w.data_ptr()
         _same_device(self.index, "append", q, k, v, rope_cos, rope_sin, q_out, q_norm_w, k_norm_w)
+        if batch.index != self.index:
+            raise ValueError(f"append: a batch on device {batch.index}, the cache on device {self.index}")
         _launch(self.index, stream, "picoattn_paged_append", abi.lib().picoattn_paged_append, self.cfg_ref, self.ref,
                 layer, batch.ref,
                 abi.PAGED_APPEND_ARGS.pack(_dtype(k), rot, q_ptr, q_stride, k.data_ptr(), _heads(k, n, hkv, hd, "k"),
@@ -318,6 +326,8 @@ class PagedCache:
             raise ValueError(f"q: {self.dtype}, out: contiguous; got {q.dtype}, strides {out.stride()}")
         _heads(out, n, hq, hd, "out")
         _same_device(self.index, "attend", q, out)
+        if batch.index != self.index:
+            raise ValueError(f"attend: a batch on device {batch.index}, the cache on device {self.index}")
         _launch(self.index, stream, "picoattn_paged_attn", abi.lib().picoattn_paged_attn, self.cfg_ref, self.ref,
                 layer, batch.ref, q.data_ptr(), _heads(q, n, hq, hd, "q"), _dtype(out), out.data_ptr(), batch.ws_ptr,
                 batch.ws_bytes)

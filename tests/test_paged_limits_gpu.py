@@ -267,3 +267,25 @@ def test_one_token_tensors_of_any_stride(rt):  # noqa: F811
         got.append([t.clone() for t in (r, rk, qo, o, B.rows(B.cache.k_pool, 0, 0, 36), B.rows(B.cache.v_pool, 0, 0, 36))])
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+def test_refuses_what_lies_on_another_device(rt):  # noqa: F811
+    """A batch of another device's cache, a stream of another device (made up: one GPU is enough)."""
+    B = Batch(rt, [1], [3], 4, 2, 64, 16, "f16", layers=1)
+    B.fill(0)
+    q = B.rand(1, 4, 64).half()
+    y = torch.empty_like(q)
+    k, tab = B.rand(1, 2, 64).half(), table(B.cfg.max_seq_len, 64)
+
+    class Stream:
+        device_index, cuda_stream = B.cache.index + 1, torch.cuda.current_stream().cuda_stream
+
+    with pytest.raises(ValueError):
+        B.cache.attend(0, B.batch, q, y, stream=Stream())
+    with pytest.raises(ValueError):
+        rt.rope(q, None, B.kv_len, *tab, y, None, rt.status_workspace(), stream=Stream())
+    B.batch.index = B.cache.index + 1
+    with pytest.raises(ValueError):
+        B.cache.attend(0, B.batch, q, y)
+    with pytest.raises(ValueError):
+        B.cache.append(0, B.batch, q, k, k, *tab, y)
