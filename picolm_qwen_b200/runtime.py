@@ -168,10 +168,11 @@ def status_workspace(device: str | torch.device = "cuda") -> torch.Tensor:
     return torch.zeros(256, dtype=torch.uint8, device=device)
 
 
-def workspace_status(ws: torch.Tensor) -> int:
-    """The sticky device status bits (abi.DEV_*) of a workspace; synchronises and clears them."""
+def workspace_status(ws: torch.Tensor, stream: torch.cuda.Stream | None = None) -> int:
+    """The sticky device status bits (abi.DEV_*) of a workspace, after the calls on `stream` (default: the current
+    one); waits for that stream and clears them."""
     v = C.c_uint32(0)
-    _launch(ws.get_device(), None, "workspace_status",
+    _launch(ws.get_device(), stream, "workspace_status",
             lambda handle: abi.lib().picoattn_workspace_status(ws.data_ptr(), handle, C.byref(v)))
     return v.value
 
@@ -248,8 +249,9 @@ class PagedBatch:
         self.workspace[:256].zero_()  # its header
         self.ref, self.ws_ptr, self.ws_bytes = C.addressof(self.desc), self.workspace.data_ptr(), ws
 
-    def status(self) -> int:
-        return workspace_status(self.workspace)
+    def status(self, stream: torch.cuda.Stream | None = None) -> int:
+        """workspace_status of the batch: `stream` is the one that its calls ran on."""
+        return workspace_status(self.workspace, stream)
 
 
 class PagedCache:

@@ -289,3 +289,19 @@ def test_refuses_what_lies_on_another_device(rt):  # noqa: F811
         B.cache.attend(0, B.batch, q, y)
     with pytest.raises(ValueError):
         B.cache.append(0, B.batch, q, k, k, *tab, y)
+
+
+def test_status_of_a_step_on_another_stream(rt):  # noqa: F811
+    from picolm_qwen_b200 import abi
+    B = Batch(rt, [1, 1], [30, 40], 4, 2, 64, 16, "f16", layers=1)
+    B.fill(0)
+    B.pages[1, 0] = -1
+    q = B.rand(2, 4, 64).half()
+    y = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # some 25 ms
+    B.cache.attend(0, B.batch, q, y, stream=side)
+    assert B.batch.status(side) == abi.DEV_BAD_PAGE
+    assert B.batch.status() == 0
