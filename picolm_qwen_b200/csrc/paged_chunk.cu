@@ -761,7 +761,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (sp.ok) continue;
             if (tid == 0) atomicOr(status, PICOATTN_DEV_BAD_POS);
             const RowRange rows = rows_inside(a.b, b);
-            for (long long i = tid; i < rows.n * a.hq * HD; i += 256) {
+            const long long n = (long long)(rows.end - rows.first) * a.hq * HD;
+            for (long long i = tid; i < n; i += 256) {
                 const size_t at = (size_t)rows.first * a.hq * HD + i;
                 if (a.out_dtype == PICOATTN_DTYPE_F32) static_cast<float*>(a.out)[at] = __int_as_float(0x7fc00000);
                 else static_cast<T*>(a.out)[at] = Elem<T>::round(__int_as_float(0x7fc00000));

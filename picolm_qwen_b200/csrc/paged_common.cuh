@@ -198,12 +198,11 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedBatch& a, int b) {
 
 // The rows of a sequence outside the bounds that lie inside [0, n_tok).
 struct RowRange {
-    int first;
-    long long n;  // 0: none
+    int first, end;  // end - first does not wrap, whatever 32-bit values the span has
 };
 __device__ __forceinline__ RowRange rows_inside(const PagedBatch& a, int b) {
-    const int t0 = max(a.q_start[b], 0), t1 = min(a.q_start[b + 1], a.n_tok);
-    return {t0, t1 > t0 ? t1 - t0 : 0};  // both ends may be any 32-bit values: t1 - t0 only where it cannot wrap
+    const int t0 = max(a.q_start[b], 0);
+    return {t0, max(t0, min(a.q_start[b + 1], a.n_tok))};
 }
 
 }  // namespace picoattn

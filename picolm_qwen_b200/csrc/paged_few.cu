@@ -158,7 +158,8 @@ __device__ __forceinline__ void nan_rows(const PagedAttnArgs& a, int b, int h, i
     constexpr int C4 = HD / 4;
     const RowRange rows = rows_inside(a.b, b);
     const float nan = __int_as_float(0x7fc00000);
-    for (long long i = tid; i < rows.n * a.g * C4; i += threads) {
+    const long long n = (long long)(rows.end - rows.first) * a.g * C4;
+    for (long long i = tid; i < n; i += threads) {
         const long long x = i / C4;
         store_out4<T>(a, ((size_t)(rows.first + x / a.g) * a.hq + (size_t)h * a.g + x % a.g) * HD + 4 * (i % C4),
                       make_float4(nan, nan, nan, nan));
@@ -175,6 +176,7 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
     uint64_t* full = reinterpret_cast<uint64_t*>(smem);
     uint64_t* empty = full + kStages;
     int* poison = reinterpret_cast<int*>(empty + kStages);  // [kStages] the tile read a page that does not exist
+    int* gave_up = reinterpret_cast<int*>(smem + 124);      // a wait of a compute warp has run out: nothing more is stored
     long long* warp_tot = reinterpret_cast<long long*>(smem + 176);  // [kWarps + 1]
     Cut* cuts = reinterpret_cast<Cut*>(smem + 128);  // [2]
     float2* ml = reinterpret_cast<float2*>(smem + F::off_ml);
@@ -184,6 +186,7 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
     pdl_trigger();
     if (tid == 0) {
         for (int s = 0; s < kStages; s++) mbar_init(&full[s], 1), mbar_init(&empty[s], kWarps);
+        *gave_up = 0;
         fence_mbar_init();
     }
     pdl_wait();
@@ -275,9 +278,9 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
         bool ok = true;  // no wait has run out: then nothing more is copied
         const uint8_t* pool = static_cast<const uint8_t*>(lane & 8 ? a.v_pool : a.k_pool);
         for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
-            if (!ok) return;
             if (!kWhole && lane == 0 && !fa.by_cta && u0 == 0 && u1 == stream_units)
-                fa.cut[b * a.hkv + h] = make_int4(0, 0, 1, 0);  // not cut
+                fa.cut[b * a.hkv + h] = make_int4(0, 0, 1, 0);  // not cut; written whatever runs out: the merge goes by it
+            if (!ok) return;
             const int r1 = min(u1 * kUnit, sp.len);
             const int* table = a.b.page_table + (size_t)b * a.b.page_cols;
             for (int row0 = u0 * kUnit; row0 < r1; row0 += F::T, t++) {
@@ -288,8 +291,10 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
                 const bool bad = page < 0 || page >= a.b.n_pages;
                 const int any_bad = __any_sync(0xffffffffu, bad);
                 const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, copy)) * (uint32_t)(F::GR * F::ROW);
-                if (t >= kStages) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (uint32_t)((t / kStages - 1) & 1), a.b.status));
+                if (t >= kStages) {  // its last tile there (a warp that gave up may give it back before), and given back
+                    const uint32_t last = (uint32_t)((t / kStages - 1) & 1);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&full[s], last, a.b.status) &&
+                                                     mbar_wait(&empty[s], last, a.b.status));
                     if (!ok) return;
                 }
                 if (lane == 0) {
@@ -323,9 +328,7 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
     // weights of up to 2^15 of fp16's 2^16 (weight_lift): below 2^-40 of the largest they vanish
     constexpr float lift = weight_lift<T>(15);
     int t = 0;
-    bool ok = true;  // no wait of this warp has run out (of any compute warp, between parts): then nothing more is stored
     for_each_part(a, b0, base, c0, c1, [&](int b, const SeqSpan& sp, int h, int u0, int u1, int stream_units) {
-        if (!ok) return;
         const int rows = sp.n * a.g;  // <= kRows
         uint32_t qa[HD / 16][4];
         int lim[2];  // keys below it are visible to the lane's rows gid, gid + 8
@@ -349,8 +352,9 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
         const int r1 = min(u1 * kUnit, sp.len);
         for (int row0 = u0 * kUnit; row0 < r1; row0 += F::T, t++) {
             const int s = t % kStages;
-            ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (uint32_t)((t / kStages) & 1), a.b.status));
-            if (!ok) break;  // the stage is not given back either
+            // a wait that ran out is noted and the warp goes on, over whatever the stage holds (to leave here, with a vote
+            // and a flag in a register, costs 2 to 4%)
+            if (!mbar_wait(&full[s], (uint32_t)((t / kStages) & 1), a.b.status)) *gave_up = 1;
             const uint32_t kbase = tiles_u32 + (uint32_t)(s * 2 * F::TILE), vbase = kbase + F::TILE;
             const int valid = r1 - row0;
             if (poison[s]) l[0] = l[1] = __int_as_float(0x7fc00000);
@@ -439,8 +443,9 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
             l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
             if (tig == 0) ml[warp * 16 + gid + 8 * half] = make_float2(m[half], l[half]);
         }
-        ok = named_bar_all(1, 32 * kWarps, ok);
-        if (!ok) return;
+        named_bar_sync(1, 32 * kWarps);
+        // the same for all: who sets it for the next part has been through all of this one's barriers
+        const bool store = *gave_up == 0;
         float wgt[2];
 #pragma unroll
         for (int half = 0; half < 2; half++) {
@@ -461,7 +466,8 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
         const size_t slot = 2 * (size_t)blockIdx.x + (u0 == 0 ? 1 : 0);
         const int ji = jr / a.g;
         const size_t orow = ((size_t)(sp.t0 + ji) * a.hq + (size_t)(h * a.g + jr - ji * a.g)) * HD;
-        if (!whole && (tid & 7) == 0 && jr < rows) fa.part_ml[slot * kRows + jr] = make_float2(M, Ls);
+        if (!whole && (tid & 7) == 0 && jr < rows)
+            fa.part_ml[slot * kRows + jr] = make_float2(M, store ? Ls : __int_as_float(0x7fc00000));
 #pragma unroll
         for (int c = 0; c < HD / 32; c++) {
 #pragma unroll
@@ -471,7 +477,7 @@ __global__ void __maxnreg__((Few<HD, MT>::kRegs)) paged_few_kernel(FewArgs fa) {
                 *reinterpret_cast<float2*>(d + 8 * F::JS) = make_float2(o[4 * c + i][2] * wgt[1], o[4 * c + i][3] * wgt[1]);
             }
             named_bar_sync(1, 32 * kWarps);
-            if (jr < rows) {
+            if (jr < rows && store) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < kKeyWarps; w++) {
@@ -508,7 +514,6 @@ __global__ void __launch_bounds__(kMergeThreads) paged_few_merge_kernel(FewArgs 
     const int tid = threadIdx.x, c4 = tid % C4, grp = tid / C4;
     const int r = blockIdx.x;
     const int4 cut = __ldcg(fa.cut + blockIdx.y);
-    if (__ldcg(a.b.status) & PICOATTN_DEV_TIMEOUT) return;  // entries and parts may not have been written
     if (fa.by_cta && cut.x < 0) return;
     const int stream = fa.by_cta ? cut.x : (int)blockIdx.y;
     const int b = stream / a.hkv, h = stream - b * a.hkv;

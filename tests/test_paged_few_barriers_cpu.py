@@ -1,9 +1,10 @@
 """The ring of the few-row attention kernel when waits run out, on the CPU.
 
 A model of paged_few.cu's copy warp and compute warps under random schedules (paged_chunk.cu's copy warps end alike).  A wait whose phase is not there may run
-out at any time; after the first one that did, others do soon (the status bit is sticky).  Whatever runs out: nobody is
-stuck, no tile is read that has not landed, a part is stored by all warps or by none, and the CTA does not end with a
-copy on its way.
+out at any time; after the first one that did, others do soon (the status bit is sticky).  A compute warp notes it for the whole
+CTA and goes on; the copy warp stops.  Whatever runs out: nobody is stuck, no stage is filled again before its last copy
+has landed, a part is stored by all warps or by none, only what was read from landed tiles is stored, and the CTA does
+not end with a copy on its way.
 """
 import random
 
@@ -12,13 +13,14 @@ import pytest
 from test_paged_barriers_cpu import Bar
 
 
-def run(seed, settle="always"):
+def run(seed, settle="always", check_full=True):
     r = random.Random(seed)
     stages, warps = r.choice([(3, 4), (6, 8)])
     parts = [r.randint(1, 8) for _ in range(r.randint(1, 5))]
     full, empty = [Bar(1) for _ in range(stages)], [Bar(warps) for _ in range(stages)]
     stage, flight, stored = [None] * stages, [], [0] * len(parts)
-    joins = [[] for _ in parts]  # what each warp brings to a part's named barrier
+    joins, ends = [[] for _ in parts], [[] for _ in parts]  # a part's named barriers, before and after its stores
+    noted = []                   # the CTA's flag
     timeouts = r.random() < .8
 
     def copy():
@@ -27,7 +29,8 @@ def run(seed, settle="always"):
             for _ in range(n):
                 s = t % stages
                 if t >= stages:
-                    ok = yield empty[s], t // stages - 1
+                    ok = not check_full or (yield full[s], t // stages - 1)
+                    ok = ok and (yield empty[s], t // stages - 1)
                 if not ok:
                     break
                 full[s].arrive(1)
@@ -46,20 +49,21 @@ def run(seed, settle="always"):
     def compute():
         t = 0
         for p, n in enumerate(parts):
-            ok = True
+            right = True
             for _ in range(n):
                 s = t % stages
-                ok = yield full[s], t // stages
-                if not ok:
-                    break
-                assert stage[s] == t
+                if not (yield full[s], t // stages):
+                    noted.append(True)
+                right = right and stage[s] == t
                 empty[s].arrive()
                 t += 1
-            joins[p].append(ok)
+            joins[p].append(right)
             yield joins[p]
-            if not all(joins[p]):
-                return
-            stored[p] += 1
+            if not noted:
+                assert all(joins[p])
+                stored[p] += 1
+            ends[p].append(None)
+            yield ends[p]
 
     roles = [copy()] + [compute() for _ in range(warps)]
     waits = [next(g, None) for g in roles]
@@ -83,7 +87,7 @@ def run(seed, settle="always"):
             continue
         w = waits[a]
         there = isinstance(w, list) or w[0].passes(w[1])
-        if there and not isinstance(w, list):
+        if there and not out and not isinstance(w, list):
             assert w[0].phase == w[1] + 1, f"a wait passed for another phase: {seed}"
         out |= not there
         try:
@@ -101,13 +105,14 @@ def test_waits_that_run_out(block):
         run(seed)
 
 
-@pytest.mark.parametrize("settle", ["never", "own"])
-def test_the_model_finds_copies_that_nobody_waits_for(settle):
-    """Neither may the copy warp leave its copies alone, nor wait for them only where a wait of its own ran out."""
+@pytest.mark.parametrize("form", [dict(settle="never"), dict(settle="own"), dict(check_full=False)])
+def test_the_model_finds(form):
+    """Copies that nobody waits for (a copy warp that leaves them alone, or waits only where a wait of its own ran out), and
+    stages filled again before their last copy has landed."""
     failed = 0
-    for seed in range(400):
+    for seed in range(1600):
         try:
-            run(seed, settle)
+            run(seed, **form)
         except AssertionError:
             failed += 1
     assert failed
