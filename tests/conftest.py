@@ -1,3 +1,4 @@
+import inspect
 import os
 import sys
 
@@ -10,6 +11,14 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200, sm_100a)")
+
+
+def pytest_collection_modifyitems(items):
+    """Where the reference's own library is not built, the tests that fail without it run last: a run that stops at its
+    first failure has been through all others by then."""
+    from oracle.pyoracle import REF_SO
+    if not os.path.exists(REF_SO):
+        items.sort(key=lambda i: "ref" in i.fixturenames or "RefHarness()" in inspect.getsource(i.function))
 
 
 @pytest.fixture(scope="session")
