@@ -144,16 +144,19 @@ def _same_device(index: int, what: str, *tensors) -> None:
             raise ValueError(f"{what}: a tensor on {t.device}, the others on device {index}")
 
 
-def _launch(index: int, stream, what: str, call, *args) -> None:
-    """call(*args, stream) with device `index` current (whichever the caller has), its error raised."""
+def _stream(index: int, stream, what: str) -> int:
+    """The handle of `stream` (None: the current one) of device `index`."""
     if index < 0:
         raise ValueError(f"{what}: tensors on the CPU")
     if stream is None:
-        handle = _raw_stream(index)
-    else:
-        if stream.device_index != index:
-            raise ValueError(f"{what}: a stream of device {stream.device_index}, tensors on device {index}")
-        handle = stream.cuda_stream
+        return _raw_stream(index)
+    if stream.device_index != index:
+        raise ValueError(f"{what}: a stream of device {stream.device_index}, tensors on device {index}")
+    return stream.cuda_stream
+
+
+def _launch(index: int, handle: int, what: str, call, *args) -> None:
+    """call(*args, handle) with device `index` current (whichever the caller has), its error raised."""
     if torch.cuda.current_device() == index:
         st = call(*args, handle)
     else:
@@ -172,7 +175,8 @@ def workspace_status(ws: torch.Tensor, stream: torch.cuda.Stream | None = None) 
     """The sticky device status bits (abi.DEV_*) of a workspace, after the calls on `stream` (default: the current
     one); waits for that stream and clears them."""
     v = C.c_uint32(0)
-    _launch(ws.get_device(), stream, "workspace_status",
+    index = ws.get_device()
+    _launch(index, _stream(index, stream, "workspace_status"), "workspace_status",
             lambda handle: abi.lib().picoattn_workspace_status(ws.data_ptr(), handle, C.byref(v)))
     return v.value
 
@@ -212,7 +216,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: torch.Tensor, rope_cos: t
         if k.dtype is not dt or k_out.dtype is not dt:
             raise ValueError("k, k_out: of q's type")
         krows = (k.data_ptr(), _heads(k, n, kh, hd, "k"), k_out.data_ptr(), _heads(k_out, n, kh, hd, "k_out"), kh)
-    _launch(index, stream, "picoattn_rope", abi.lib().picoattn_rope,
+    _launch(index, _stream(index, stream, "rope"), "picoattn_rope", abi.lib().picoattn_rope,
             abi.ROPE_ARGS.pack(_dtype(q), rope_mode, hd, rot, 1 if inverse else 0, n, rope_cos.shape[0],
                                1 if k is None else 2, pos.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
                                *rows, *krows),
@@ -248,6 +252,18 @@ class PagedBatch:
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=cache.device)
         self.workspace[:256].zero_()  # its header
         self.ref, self.ws_ptr, self.ws_bytes = C.addressof(self.desc), self.workspace.data_ptr(), ws
+        self.streams = {_raw_stream(self.index)}  # those that the allocator knows the workspace to be used on
+
+    def stream(self, stream: torch.cuda.Stream | None, what: str) -> int:
+        """The handle of a call's stream.  Where it is not the batch's own, the batch's memory is not handed out again
+        before the call is through, even if the batch is dropped."""
+        handle = _stream(self.index, stream, what)
+        if handle not in self.streams:
+            s = torch.cuda.current_stream(self.index) if stream is None else stream
+            for t in (self.workspace, *self.tensors):
+                t.record_stream(s)
+            self.streams.add(handle)
+        return handle
 
     def status(self, stream: torch.cuda.Stream | None = None) -> int:
         """workspace_status of the batch: `stream` is the one that its calls ran on."""
@@ -311,7 +327,7 @@ class PagedCache:
         _same_device(self.index, "append", q, k, v, rope_cos, rope_sin, q_out, q_norm_w, k_norm_w)
         if batch.index != self.index:
             raise ValueError(f"append: a batch on device {batch.index}, the cache on device {self.index}")
-        _launch(self.index, stream, "picoattn_paged_append", abi.lib().picoattn_paged_append, self.cfg_ref, self.ref,
+        _launch(self.index, batch.stream(stream, "append"), "picoattn_paged_append", abi.lib().picoattn_paged_append, self.cfg_ref, self.ref,
                 layer, batch.ref,
                 abi.PAGED_APPEND_ARGS.pack(_dtype(k), rot, q_ptr, q_stride, k.data_ptr(), _heads(k, n, hkv, hd, "k"),
                                            v.data_ptr(), _heads(v, n, hkv, hd, "v"), qn, kn, rope_cos.data_ptr(),
@@ -330,7 +346,7 @@ class PagedCache:
         _same_device(self.index, "attend", q, out)
         if batch.index != self.index:
             raise ValueError(f"attend: a batch on device {batch.index}, the cache on device {self.index}")
-        _launch(self.index, stream, "picoattn_paged_attn", abi.lib().picoattn_paged_attn, self.cfg_ref, self.ref,
+        _launch(self.index, batch.stream(stream, "attend"), "picoattn_paged_attn", abi.lib().picoattn_paged_attn, self.cfg_ref, self.ref,
                 layer, batch.ref, q.data_ptr(), _heads(q, n, hq, hd, "q"), _dtype(out), out.data_ptr(), batch.ws_ptr,
                 batch.ws_bytes)
 

@@ -305,3 +305,29 @@ def test_status_of_a_step_on_another_stream(rt):  # noqa: F811
     B.cache.attend(0, B.batch, q, y, stream=side)
     assert B.batch.status(side) == abi.DEV_BAD_PAGE
     assert B.batch.status() == 0
+
+
+def test_a_batch_dropped_while_another_stream_uses_it(rt):  # noqa: F811
+    """The memory of a batch is not handed out again before its calls on other streams are through."""
+    B = Batch(rt, [1, 1], [30, 4000], 4, 2, 64, 16, "f16", layers=1)
+    B.fill(0)
+    q = B.rand(2, 4, 64).half()
+    want, y = torch.empty_like(q), torch.empty_like(q)
+    B.cache.attend(0, B.batch, q, want)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for explicit in (True, False):
+        batch = B.cache.batch(B.pages, B.q_start, B.kv_len, 2, 1, max(B.total))
+        n, at = batch.workspace.numel(), batch.workspace.data_ptr()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)  # some 50 ms
+            if not explicit:
+                B.cache.attend(0, batch, q, y)
+        if explicit:
+            B.cache.attend(0, batch, q, y, stream=side)
+        del batch
+        other = torch.empty(n, dtype=torch.uint8, device="cuda")
+        assert not side.query() and other.data_ptr() != at
+        side.synchronize()
+        assert torch.equal(y, want)
