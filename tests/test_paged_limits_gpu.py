@@ -331,3 +331,48 @@ def test_a_batch_dropped_while_another_stream_uses_it(rt):  # noqa: F811
         assert not side.query() and other.data_ptr() != at
         side.synchronize()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("spans", SPANS + [[0, 2, 5, 6]])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_of_spans_outside_the_batch(rt, spans, norm):  # noqa: F811
+    """Any values in q_start: only rows of good sequences' own positions are stored, and they hold what the good step
+    stores; q_out rows are the good step's or NaN, and none outside the step is written."""
+    from picolm_qwen_b200 import abi
+    hq, hkv, hd, page = 4, 2, 64, 16
+    B = Batch(rt, [2, 3, 1], [7, 40, 21], hq, hkv, hd, page, "f16", layers=2)
+    B.batch = B.cache.batch(B.pages, B.q_start, B.kv_len, 6, 6, B.cfg.max_seq_len)
+    B.fill(0, upto=B.past)
+    pools = B.cache.k_pool, B.cache.v_pool
+    before = [p.clone() for p in pools]
+    q, k, v = B.rand(6, hq, hd), B.rand(6, hkv, hd), B.rand(6, hkv, hd)
+    w = (1 + 0.1 * B.rand(hd), 1 + 0.1 * B.rand(hd)) if norm else (None, None)
+    tab = table(B.cfg.max_seq_len, hd)
+    good = torch.empty((6, hq, hd), device="cuda").half()
+    B.cache.append(0, B.batch, q, k, v, *tab, good, *w)
+    assert B.batch.status() == 0
+    full = [p.clone() for p in pools]
+    for p, old in zip(pools, before):
+        p.copy_(old)
+    B.q_start.copy_(torch.tensor(spans, dtype=torch.int64).to(torch.int32))
+    area = torch.full((8, hq, hd), 7.0, device="cuda").half()
+    B.cache.append(0, B.batch, q, k, v, *tab, area[1:7], *w)
+    ok = [0 <= a <= e <= 6 and e - a <= t for a, e, t in zip(spans, spans[1:], B.total)]
+    assert B.batch.status() == (0 if all(ok) else abi.DEV_BAD_POS)
+    assert (area[[0, 7]] == 7).all()
+    same_as_good = spans[:2] == [0, 2], spans[1:3] == [2, 5], spans[2:4] == [5, 6]
+    for t in range(6):
+        b = 0 if t < 2 else (1 if t < 5 else 2)
+        y = area[1 + t]
+        if all(ok) or (same_as_good[b] and spans == sorted(spans)):
+            assert torch.equal(y, good[t])
+        else:  # of another span, of a bad one, of none
+            assert y.isfinite().all() if not y.isnan().any() else y.isnan().all()
+    for p, old, new in zip(pools, before, full):
+        same = ((p == old) | (p.isnan() & old.isnan())).all(-1)
+        changed = {(i, g, r) for i, g, h, r in (~same).nonzero().tolist()}
+        mine = {(0, int(B.pages[b, r // page]), r % page) for b in range(3) if ok[b]
+                for r in range(B.total[b] - (spans[b + 1] - spans[b]), B.total[b])}
+        assert changed <= mine
+        if all(ok):
+            assert changed == mine and torch.equal(p.view(torch.int16), new.view(torch.int16))
