@@ -376,3 +376,42 @@ def test_append_of_spans_outside_the_batch(rt, spans, norm):  # noqa: F811
         assert changed <= mine
         if all(ok):
             assert changed == mine and torch.equal(p.view(torch.int16), new.view(torch.int16))
+
+
+@pytest.mark.parametrize("wtype", ["F16", "Q8_0", "Q4_K"])
+def test_a_layer_of_the_librarys_own_projections(rt, wtype):  # noqa: F811
+    """matvec -> append -> attend -> matvec, as a host with a paged cache runs a layer, beside decode_layer on the same rows in
+    slabs.  Both are within 2e-3 + 1e-2 |x| of the reference's chain by the tests of decode_layer (rows and outputs to
+    fp32 rounding of the projections, one step of fp16 in the new cache rows)."""
+    from picolm_qwen_b200 import abi
+    from tests import weightgen as wg
+    hq, hkv, hd, dim, page = 16, 4, 64, 1024, 16
+    past = [0, 76, 599]
+    t = {v: k for k, v in wg.NAMES.items()}[wtype]
+    rng = np.random.default_rng(8)
+    B = Batch(rt, [1, 1, 1], past, hq, hkv, hd, page, "f16", layers=2)
+    B.fill(1, upto=past)
+    st = rt.AttnState(B.cfg, n_seqs=3, max_ctx=B.cfg.max_seq_len)
+    for b, n in enumerate(past):
+        for pool, slab in ((B.cache.k_pool, st.k_cache), (B.cache.v_pool, st.v_cache)):
+            slab[b, 1, :n] = B.rows(pool, 1, b, n).reshape(n, hkv * hd).view(torch.int16)
+    shapes = ((dim, hq * hd), (dim, hkv * hd), (dim, hkv * hd), (hq * hd, dim))
+    w = [torch.from_numpy(wg.make(t, n_in, n_out, rng)).cuda() for n_in, n_out in shapes]
+    bias = [0.1 * B.rand(n_out) for _, n_out in shapes]
+    proj = rt.LayerProj(*w, (t,) * 4, *bias)
+    xb, x = B.rand(3, dim), B.rand(3, dim)
+    slab_x = x.clone()
+    st.decode_layer(1, dim, xb, proj, torch.tensor(past, dtype=torch.int32, device="cuda"), slab_x)
+    q, k, v = (torch.empty((3, n_out), device="cuda") for _, n_out in shapes[:3])
+    for y, wy, by, (n_in, n_out) in zip((q, k, v), w, bias, shapes):
+        rt.matvec(wy, t, n_in, n_out, xb, y, by)
+    qo, out = torch.empty((3, hq * hd), device="cuda").half(), torch.empty((3, hq * hd), device="cuda")
+    B.cache.append(1, B.batch, q, k, v, st.rope_cos, st.rope_sin, qo)
+    B.cache.attend(1, B.batch, qo, out)
+    rt.matvec(w[3], t, hq * hd, dim, out, x, bias[3], accumulate=True)
+    assert B.batch.status() == 0 and st.status() == 0
+    assert ((x - slab_x).abs() <= 2 * (2e-3 + 1e-2 * slab_x.abs())).all()
+    for b, n in enumerate(past):
+        for pool, slab in ((B.cache.k_pool, st.k_cache), (B.cache.v_pool, st.v_cache)):
+            a, e = B.rows(pool, 1, b, n + 1)[n].reshape(-1).view(torch.int16).int(), slab[b, 1, n].int()
+            assert (a - e).abs().max() <= 1
