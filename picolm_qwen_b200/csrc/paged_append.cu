@@ -39,10 +39,10 @@ __device__ __forceinline__ void store_pieces(const float (&x)[16], TC* head, con
 // A warp step = up to HPS heads of one kind (q, k or v) of one token, hd/16
 // lanes a head; a unit = up to kSteps steps of one kind of one token.  Bound by
 // latency and instruction issue (some 250 instructions per step of 512 elements with
-// QK-norm and its share of the lookups; 80 registers, so 24 warps an SM): the loads of a unit are issued first, its
-// token's sequence, position, page and table entries are found while they travel,
-// and units are numbered kind by kind, so that the warps of an SM run the same
-// code.  Measured: 2,048 tokens of 32/8 heads of 128 with QK-norm in fp16 13.5 us
+// QK-norm and its share of the lookups; 80 registers, so 24 warps an SM): the loads
+// of a unit are issued first, its token's sequence, position, page and table entries
+// are found while they travel, and units are numbered kind by kind, so that the
+// warps of an SM run the same code.  Measured: 2,048 tokens of 32/8 heads of 128 with QK-norm in fp16 13.5 us
 // (51 MB: 3.8 TB/s, 0.58 of the copy rate, as the contiguous prefill's prep kernel
 // takes); 64 tokens 3.0 us.  Slower: a ring of cp.async copies of the next units
 // 20.5 us (its shared memory comes out of the cache that the lookups live in), the

@@ -156,8 +156,8 @@ __device__ __forceinline__ void rotate_pieces_fused(float* x, const float* c, co
 }
 
 // The softmax weights go into the product with V in the cache's 16 bits: that is
-// what its tensor instructions take, and it costs an output half a step of the
-// type at most, as its own rounding does.  An fp16 weight is subnormal below
+// what its tensor instructions take, and it moves an output by at most half a step
+// of the type times the weighted mean of |v|.  An fp16 weight is subnormal below
 // 2^-14 and nothing below 2^-25, which over a long context is more than that: all
 // of 131,072 keys at 2^-26 of a strong one make up 0.2% of the output.  So the
 // running maximum is held `lift` (log2) too low and every weight is 2^lift times as
