@@ -252,7 +252,8 @@ class PagedBatch:
         self.workspace = torch.empty(ws, dtype=torch.uint8, device=cache.device)
         self.workspace[:256].zero_()  # its header
         self.ref, self.ws_ptr, self.ws_bytes = C.addressof(self.desc), self.workspace.data_ptr(), ws
-        self.streams = {_raw_stream(self.index)}  # those that the allocator knows the workspace to be used on
+        # streams that the allocator knows the workspace to be used on
+        self.streams = {_raw_stream(self.index)} if self.index >= 0 else set()
 
     def stream(self, stream: torch.cuda.Stream | None, what: str) -> int:
         """The handle of a call's stream.  Where it is not the batch's own, the batch's memory is not handed out again
